@@ -1,0 +1,663 @@
+// Matrix product of 8-bit integers on the 5th-generation tensor cores:
+//   C[m, n] = (sum_k A[m, k] W[n, k]) * a_scale[m] * w_scale[n]      A [M, K], W [N, K] int8, the sum in 32-bit integers
+// and, gated, C[m, i] = silu(C'[m, 2i]) * C'[m, 2i + 1] over weight rows that alternate gate and up.  The sums are exact (|code| <= 128 and
+// K < 131,072 keep them below 2^31), so a token's result depends neither on how K is cut nor on the batch it is in, to the last bit.
+//
+// Both operands are K-major; TMA brings 128-byte-swizzled tiles (128 codes a row) into a ring of shared-memory stages, one elected thread issues
+// tcgen05.mma.kind::i8 (32 codes of K an instruction), the accumulators lie in tensor memory.  The weights sit in the instruction's M slot, the
+// tokens in its N slot.  Two kernels, chosen by how many tiles there are (choose below):
+//   few tokens (gemm_int8_few_kernel): up to 128 weight rows x 16, 32, 64 or 128 tokens a block, two blocks an SM; K may be cut over a cluster of
+//     2, 4 or 8 blocks, which add their integer tiles through distributed shared memory: no scratch, no flags, one launch;
+//   many tokens (gemm_int8_pair_kernel): 256 weight rows x up to 256 tokens on pairs of blocks, persistent, the accumulator double-buffered.
+// Tails: rows beyond M or N and the end of K are zero-filled by TMA, stores are predicated.  Any K; the rows of A and of W lie a multiple of 16 bytes
+// apart.  No cluster multicast is used.
+//
+// The reference has no integer product (its own are half precision: spymaster2h/spyinfer src/backends/cuda/cublas/sgemm.cu:37-55).
+#include <cuda.h>
+
+#include "common.cuh"
+#include "tcgen05.cuh"
+
+SPY_MODULE(spy_gemm_int8)
+
+namespace {
+
+using namespace tc;
+
+constexpr int BM = 128;            // weight rows of a block = the instruction's M (half of it on pairs)
+constexpr int BK = 128;            // codes of K a stage = bytes of a swizzled row
+constexpr int UMMA_K = 32;
+constexpr int NUM_THREADS = 192;   // warp 0: TMA, warp 1: MMA and tensor memory, warps 2 to 5: epilogue
+constexpr int MAX_K = 131071;
+
+// Instruction descriptor of kind::i8: signed 8-bit operands, both K-major, a 32-bit integer accumulator.
+__device__ __forceinline__ uint32_t instr_desc_s8(int m, int n)
+{
+    uint32_t d = 0;
+    d |= 2u << 4;                      // accumulator S32
+    d |= 1u << 7;                      // A signed 8-bit
+    d |= 1u << 10;                     // B signed 8-bit
+    d |= (uint32_t)(n >> 3) << 17;
+    d |= (uint32_t)(m >> 4) << 24;
+    return d;
+}
+__device__ __forceinline__ void umma_s8(uint32_t tmem_d, uint64_t desc_a, uint64_t desc_b, uint32_t idesc, uint32_t accumulate)
+{
+    asm volatile(
+        "{\n\t.reg .pred p;\n\t"
+        "setp.ne.b32 p, %4, 0;\n\t"
+        "tcgen05.mma.cta_group::1.kind::i8 [%0], %1, %2, %3, p;\n\t}"
+        ::"r"(tmem_d), "l"(desc_a), "l"(desc_b), "r"(idesc), "r"(accumulate)
+        : "memory");
+}
+__device__ __forceinline__ void umma_s8_pair(uint32_t tmem_d, uint64_t desc_a, uint64_t desc_b, uint32_t idesc, uint32_t accumulate)
+{
+    asm volatile(
+        "{\n\t.reg .pred p;\n\t"
+        "setp.ne.b32 p, %4, 0;\n\t"
+        "tcgen05.mma.cta_group::2.kind::i8 [%0], %1, %2, %3, p;\n\t}"
+        ::"r"(tmem_d), "l"(desc_a), "l"(desc_b), "r"(idesc), "r"(accumulate)
+        : "memory");
+}
+
+// silu(g) * u for a bfloat16 result: the fast exponential and division (2 ulp of float each) are far inside the result's rounding.  A gate
+// below -87 gives g / inf = -0, the limit.
+__device__ __forceinline__ float silu_mul(float g, float u) { return __fdividef(g, 1.0f + __expf(-g)) * u; }
+
+__device__ __forceinline__ int4 load_shared_of(uint32_t cluster_addr)
+{
+    int4 v;
+    asm volatile("ld.shared::cluster.v4.s32 {%0, %1, %2, %3}, [%4];" : "=r"(v.x), "=r"(v.y), "=r"(v.z), "=r"(v.w) : "r"(cluster_addr) : "memory");
+    return v;
+}
+
+// ---- few tokens ------------------------------------------------------------------------------------------------------------------
+// Two blocks share an SM, each with AREA bytes of stages.  A tile of fewer than 128 weight rows takes only its own bytes (rounded up to the
+// swizzle's 1 KB); the tensor core still reads 128 rows: the spare ones come from whatever lies behind (the area ends with room for that) and feed
+// accumulator rows that are never stored.  When the sums are complete the ring is free and holds the integer tile, [token][TILE_LD].
+constexpr int TILE_LD = BM + 4;
+template <int BN> struct Tile {
+    static constexpr int Y_BYTES = BN * BK;
+    static constexpr int TMEM_COLS = BN < 32 ? 32 : BN;
+    static constexpr int AREA = 110 * 1024;
+    static constexpr int MAX_STAGES = 12;
+    static constexpr size_t SMEM = (size_t)AREA + 1024 /* alignment slack */ + 256 /* barriers */;
+    __host__ __device__ static constexpr int x_bytes(int tile_rows) { return (tile_rows * BK + 1023) & ~1023; }
+    __host__ __device__ static constexpr int stages(int tile_rows)
+    {
+        const int n = (AREA - (BM * BK - x_bytes(tile_rows))) / (x_bytes(tile_rows) + Y_BYTES);
+        return n < MAX_STAGES ? n : MAX_STAGES;
+    }
+    static_assert(BN * TILE_LD * 4 <= AREA, "the integer tile fits the ring");
+};
+
+// Block (token tile, K range) = (blockIdx.x / splits, blockIdx.x % splits) of weight tile blockIdx.y; the K ranges of a tile are a cluster.
+template <int BN, typename TC, bool GATED>
+__global__ void __launch_bounds__(NUM_THREADS, 2)
+gemm_int8_few_kernel(const __grid_constant__ CUtensorMap map_w, const __grid_constant__ CUtensorMap map_a, const float* __restrict__ w_scale,
+                     const float* __restrict__ a_scale, TC* __restrict__ out, long long ld, int N, int M, int k_blocks, int splits, int tile_rows, int* status)
+{
+    using T = Tile<BN>;
+    extern __shared__ uint8_t smem_raw[];
+    uint8_t* tiles = reinterpret_cast<uint8_t*>((reinterpret_cast<uintptr_t>(smem_raw) + 1023) & ~(uintptr_t)1023);
+    uint64_t* full_bar = reinterpret_cast<uint64_t*>(tiles + T::AREA);
+    uint64_t* empty_bar = full_bar + T::MAX_STAGES;
+    uint64_t* accum_bar = empty_bar + T::MAX_STAGES;
+    uint32_t* tmem_slot = reinterpret_cast<uint32_t*>(accum_bar + 1);
+    volatile int* abort_flag = reinterpret_cast<volatile int*>(tmem_slot + 1);
+
+    const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
+    const int rank = blockIdx.x % splits;                       // the block's place in its cluster
+    const int x0 = blockIdx.y * tile_rows, y0 = blockIdx.x / splits * BN;
+    const int kb0 = (int)((long long)rank * k_blocks / splits), num_kb = (int)((long long)(rank + 1) * k_blocks / splits) - kb0;
+    const uint32_t stage_tx = (uint32_t)tile_rows * BK + T::Y_BYTES;
+    const int x_bytes = T::x_bytes(tile_rows), stage_bytes = x_bytes + T::Y_BYTES, stages = T::stages(tile_rows);
+
+    if (threadIdx.x == 0) {
+#pragma unroll 1
+        for (int s = 0; s < stages; ++s) {
+            mbar_init(full_bar + s, 1);
+            mbar_init(empty_bar + s, 1);
+        }
+        mbar_init(accum_bar, 1);
+        *abort_flag = 0;
+        asm volatile("fence.mbarrier_init.release.cluster;" ::: "memory");
+    }
+    if (warp == 1) tmem_alloc(tmem_slot, T::TMEM_COLS);
+    fence_before_sync();
+    __syncthreads();
+    fence_after_sync();
+    const uint32_t tmem_base = *tmem_slot;
+
+    pdl_launch_dependents();
+    if (warp == 0) {
+        if (lane == 0) {
+            // the weights depend on no earlier kernel: their tiles for the first stages are requested before the wait for the kernels ahead in the stream
+            const int pre = min(num_kb, stages);
+#pragma unroll 1
+            for (int i = 0; i < pre; ++i) {
+                mbar_expect_tx(full_bar + i, stage_tx);
+                tma_load_2d(smem_u32(tiles + (size_t)i * stage_bytes), &map_w, (kb0 + i) * BK, x0, full_bar + i);
+            }
+            pdl_wait();
+#pragma unroll 1
+            for (int i = 0; i < pre; ++i) tma_load_2d(smem_u32(tiles + (size_t)i * stage_bytes + x_bytes), &map_a, (kb0 + i) * BK, y0, full_bar + i);
+            int s = 0;
+            uint32_t phase = 1;   // of the round before: the first wait on a stage is for its first release
+#pragma unroll 1
+            for (int i = pre; i < num_kb; ++i) {
+                if (!mbar_wait(empty_bar + s, phase ^ 1, abort_flag)) break;
+                uint8_t* xs = tiles + (size_t)s * stage_bytes;
+                mbar_expect_tx(full_bar + s, stage_tx);
+                tma_load_2d(smem_u32(xs), &map_w, (kb0 + i) * BK, x0, full_bar + s);
+                tma_load_2d(smem_u32(xs + x_bytes), &map_a, (kb0 + i) * BK, y0, full_bar + s);
+                if (++s == stages) {
+                    s = 0;
+                    phase ^= 1;
+                }
+            }
+        }
+    } else if (warp == 1) {
+        if (lane == 0) {
+            const uint32_t idesc = instr_desc_s8(BM, BN);
+            int s = 0;
+            uint32_t phase = 0;
+#pragma unroll 1
+            for (int i = 0; i < num_kb; ++i) {
+                if (!mbar_wait(full_bar + s, phase, abort_flag)) break;
+                fence_after_sync();
+                const uint8_t* xs = tiles + (size_t)s * stage_bytes;
+                const uint64_t dx = desc_k_major(smem_u32(xs)), dy = desc_k_major(smem_u32(xs + x_bytes));
+#pragma unroll
+                for (int k = 0; k < BK / UMMA_K; ++k) {
+                    const uint64_t adv = (uint64_t)((k * UMMA_K) >> 4);
+                    umma_s8(tmem_base, dx + adv, dy + adv, idesc, (i > 0 || k > 0) ? 1u : 0u);
+                }
+                umma_commit(empty_bar + s);   // the stage is free again when these MMAs have read it
+                if (++s == stages) {
+                    s = 0;
+                    phase ^= 1;
+                }
+            }
+            umma_commit(accum_bar);           // the accumulator is complete when every MMA has finished
+        }
+    } else {
+        // warp w reads tensor-memory lanes 32 (w % 4) .. + 31, i.e. weight rows of the tile; the tile goes to the ring, which every MMA has read
+        const int row = (warp & 3) * 32 + lane;
+        const bool ok = mbar_wait(accum_bar, 0, abort_flag);
+        fence_after_sync();
+        if (ok) {
+            int* staged = reinterpret_cast<int*>(tiles);
+            constexpr int COLS = BN < 32 ? BN : 32;
+#pragma unroll 1
+            for (int c = 0; c < BN; c += COLS) {
+                uint32_t r[COLS];
+                tmem_load<COLS>(tmem_base + ((uint32_t)((warp & 3) * 32) << 16) + (uint32_t)c, r);
+                tmem_wait_ld();
+#pragma unroll
+                for (int j = 0; j < COLS; ++j) staged[(c + j) * TILE_LD + row] = (int)r[j];
+            }
+        }
+    }
+    fence_before_sync();
+    __syncthreads();
+    if (splits > 1) cluster_sync();           // every block's part of the sums lies in its shared memory
+    pdl_wait();                               // the scales and the output belong to kernels ahead in the stream until here
+
+    // the cluster's blocks finish the tile together, four outputs of one token at a time, each a part of them
+    {
+        const int tokens = min(BN, M - y0), outs = min(tile_rows, N - x0), quads = (outs + 3) >> 2;
+        const int total = tokens * quads, first = (int)((long long)rank * total / splits), end = (int)((long long)(rank + 1) * total / splits);
+        const uint32_t own = smem_u32(tiles);
+        constexpr int WIDTH = GATED ? 2 : 4;  // results of a quad
+        TC* base = out + (size_t)y0 * ld + (GATED ? x0 / 2 : x0);
+        const bool whole_rows = ld % WIDTH == 0 && (reinterpret_cast<uintptr_t>(base) & (WIDTH * sizeof(TC) - 1)) == 0;
+#pragma unroll 1
+        for (int i = first + (int)threadIdx.x; i < end; i += NUM_THREADS) {
+            const int t = i / quads, q = i - t * quads, left = outs - 4 * q;
+            const uint32_t at = own + (uint32_t)(t * TILE_LD + 4 * q) * 4;
+            int4 sum = make_int4(0, 0, 0, 0);
+            if (splits == 1) {
+                sum = *reinterpret_cast<const int4*>(tiles + (size_t)(t * TILE_LD + 4 * q) * 4);
+            } else {
+#pragma unroll 2
+                for (int r = 0; r < splits; ++r) {
+                    const int4 v = load_shared_of(map_to_rank(at, r));
+                    sum.x += v.x;
+                    sum.y += v.y;
+                    sum.z += v.z;
+                    sum.w += v.w;
+                }
+            }
+            const float sa = a_scale[y0 + t];
+            const float* sw = w_scale + x0 + 4 * q;
+            float v[4] = {(float)sum.x * sa, (float)sum.y * sa, (float)sum.z * sa, (float)sum.w * sa};
+#pragma unroll
+            for (int e = 0; e < 4; ++e) v[e] = e < left ? v[e] * sw[e] : 0.f;
+            TC* dst = base + (size_t)t * ld + WIDTH * q;
+            if constexpr (GATED) {
+                v[0] = silu_mul(v[0], v[1]);
+                v[1] = silu_mul(v[2], v[3]);
+            }
+            if (left >= 4 && whole_rows) {
+                if constexpr (sizeof(TC) == 4) {
+                    *reinterpret_cast<float4*>(dst) = make_float4(v[0], v[1], v[2], v[3]);
+                } else if constexpr (GATED) {
+                    *reinterpret_cast<uint32_t*>(dst) = pack_bf16(v[0], v[1]);
+                } else {
+                    *reinterpret_cast<uint2*>(dst) = make_uint2(pack_bf16(v[0], v[1]), pack_bf16(v[2], v[3]));
+                }
+            } else {
+#pragma unroll
+                for (int e = 0; e < WIDTH; ++e)
+                    if (e < (GATED ? left / 2 : left)) dst[e] = from_f32<TC>(v[e]);
+            }
+        }
+    }
+
+    __syncthreads();
+    if (*abort_flag) {
+        // a wait ran out: copies that may still be in flight get time to land before the shared memory is released, then it is reported
+        if (threadIdx.x == 0) {
+            const unsigned long long t0 = global_timer();
+            while (global_timer() - t0 < 2000000ull) { }
+            report_status(status, SPY_STATUS_WAIT_TIMEOUT, (int)(blockIdx.x + blockIdx.y * gridDim.x));
+        }
+        __syncthreads();
+    }
+    if (splits > 1) cluster_sync();           // no block leaves while another may still read its shared memory
+    if (warp == 1) {
+        fence_after_sync();
+        tmem_dealloc(tmem_base, T::TMEM_COLS);
+    }
+}
+
+// ---- many tokens -----------------------------------------------------------------------------------------------------------------
+// A cluster of two blocks on neighbouring SMs computes one tile of 256 weight rows and up to 256 tokens: each block loads its 128 weight rows and its
+// half of the tile's tokens, the leader (rank 0) issues tcgen05.mma.cta_group::2 instructions that read both blocks' shared memory and
+// accumulate each block's 128 rows in its own tensor memory; both blocks' four epilogue warps read their halves back and turn them in shared memory
+// on the way out.  The TMA loads of both blocks complete on the leader's full barrier; a commit frees a stage, and publishes an accumulator, in both
+// blocks; the peer's epilogue threads arrive on the leader's accumulator-empty barrier.  Cluster c walks tiles c, c + clusters, ...; tiles are numbered
+// with the token tiles fastest, so that clusters side by side share weight tiles in L2.
+
+// The tokens in `count` tiles whose heights are multiples of 32 and differ by 32 at most: the first `tall` tiles have `rows` tokens, the others 32 fewer.
+struct TokenTiles {
+    int count, rows, tall;
+    __host__ __device__ int first(int t) const { return t * rows - (t > tall ? (t - tall) * 32 : 0); }
+    __host__ __device__ int height(int t) const { return t < tall ? rows : rows - 32; }
+};
+static inline TokenTiles token_tiles(int M, int count)
+{
+    TokenTiles t;
+    const int runs = (M + 31) / 32, each = runs / count, more = runs % count;
+    t.count = count;
+    t.rows = 32 * (more > 0 ? each + 1 : each);
+    t.tall = more > 0 ? more : count;
+    return t;
+}
+
+constexpr int PAIR_BN = 256;                                 // tensor-memory columns of an accumulator
+constexpr int PAIR_MAX_STAGES = 10;
+constexpr int PAIR_X_BYTES = BM * BK;
+constexpr int PAIR_AREA = 6 * 2 * PAIR_X_BYTES;              // the ring: six stages at 256 tokens a tile, more at fewer
+constexpr int TURN_LD = 36;                                  // floats between the tokens of a warp's chunk of 32 tokens x 32 weight rows
+constexpr int TURN_BYTES = 32 * TURN_LD * 4 + 32 * 4;        // and the tokens' scales
+constexpr size_t PAIR_SMEM = (size_t)PAIR_AREA + 4 * TURN_BYTES + 1024 /* alignment slack */ + 256 /* barriers */;
+__host__ __device__ constexpr int pair_stage_bytes(int token_rows) { return PAIR_X_BYTES + token_rows / 2 * BK; }
+__host__ __device__ constexpr int pair_stages(int token_rows)
+{
+    const int n = PAIR_AREA / pair_stage_bytes(token_rows);
+    return n < PAIR_MAX_STAGES ? n : PAIR_MAX_STAGES;
+}
+
+// Finishes one chunk: this lane holds weight row x0 + lane of the 32 tokens from y on.  `turn` is the warp's own place in shared memory, where the
+// chunk is turned so that the results leave in rows.
+template <typename TC, bool GATED>
+__device__ __forceinline__ void store_chunk(TC* __restrict__ out, long long ld, int lane, int x0, int y, int N, int y_end, const uint32_t (&r)[32], float sw,
+                                            const float* __restrict__ a_scale, float* turn)
+{
+    const int count = min(32, y_end - y), outs = min(32, N - x0);
+    if (outs <= 0 || count <= 0) return;      // the same for the whole warp
+    float* sa = turn + 32 * TURN_LD;
+    sa[lane] = lane < count ? a_scale[y + lane] : 0.f;
+    __syncwarp();
+#pragma unroll
+    for (int j = 0; j < 32; j += 4) {
+        const float4 s = *reinterpret_cast<const float4*>(sa + j);
+        turn[j * TURN_LD + lane] = (float)(int)r[j] * s.x * sw;
+        turn[(j + 1) * TURN_LD + lane] = (float)(int)r[j + 1] * s.y * sw;
+        turn[(j + 2) * TURN_LD + lane] = (float)(int)r[j + 2] * s.z * sw;
+        turn[(j + 3) * TURN_LD + lane] = (float)(int)r[j + 3] * s.w * sw;
+    }
+    __syncwarp();
+    constexpr int PER = GATED ? 16 : 32;      // results of a token
+    TC* dst = out + (size_t)y * ld + (GATED ? x0 / 2 : x0);
+    if (outs == 32 && ld * (long long)sizeof(TC) % 16 == 0 && (reinterpret_cast<uintptr_t>(dst) & 15) == 0) {
+        if constexpr (GATED) {
+            // two lanes a token, eight results each
+            const int part = lane & 1;
+#pragma unroll
+            for (int i = 0; i < 2; ++i) {
+                const int t = i * 16 + (lane >> 1);
+                uint32_t w[4];
+#pragma unroll
+                for (int e = 0; e < 4; ++e) {
+                    const float4 v = *reinterpret_cast<const float4*>(turn + t * TURN_LD + part * 16 + 4 * e);
+                    w[e] = pack_bf16(silu_mul(v.x, v.y), silu_mul(v.z, v.w));
+                }
+                if (t < count) *reinterpret_cast<uint4*>(dst + (size_t)t * ld + part * 8) = make_uint4(w[0], w[1], w[2], w[3]);
+            }
+        } else if constexpr (sizeof(TC) == 2) {
+            // four lanes a token, eight results each
+            const int part = lane & 3;
+#pragma unroll
+            for (int i = 0; i < 4; ++i) {
+                const int t = i * 8 + (lane >> 2);
+                const float4 v = *reinterpret_cast<const float4*>(turn + t * TURN_LD + part * 8);
+                const float4 w = *reinterpret_cast<const float4*>(turn + t * TURN_LD + part * 8 + 4);
+                if (t < count)
+                    *reinterpret_cast<uint4*>(dst + (size_t)t * ld + part * 8) =
+                        make_uint4(pack_bf16(v.x, v.y), pack_bf16(v.z, v.w), pack_bf16(w.x, w.y), pack_bf16(w.z, w.w));
+            }
+        } else {
+            const int part = lane & 7;
+#pragma unroll
+            for (int i = 0; i < 8; ++i) {
+                const int t = i * 4 + (lane >> 3);
+                if (t < count) *reinterpret_cast<float4*>(dst + (size_t)t * ld + part * 4) = *reinterpret_cast<const float4*>(turn + t * TURN_LD + part * 4);
+            }
+        }
+    } else {
+        const int results = GATED ? outs / 2 : outs;
+        for (int i = lane; i < count * PER; i += 32) {
+            const int t = i / PER, c = i % PER;
+            if (c < results) {
+                if constexpr (GATED) dst[(size_t)t * ld + c] = from_f32<TC>(silu_mul(turn[t * TURN_LD + 2 * c], turn[t * TURN_LD + 2 * c + 1]));
+                else dst[(size_t)t * ld + c] = from_f32<TC>(turn[t * TURN_LD + c]);
+            }
+        }
+    }
+    __syncwarp();   // the next chunk's numbers may come
+}
+
+template <typename TC, bool GATED>
+__global__ void __launch_bounds__(NUM_THREADS, 1)
+gemm_int8_pair_kernel(const __grid_constant__ CUtensorMap map_w, const __grid_constant__ CUtensorMap map_a, const float* __restrict__ w_scale,
+                      const float* __restrict__ a_scale, TC* __restrict__ out, long long ld, int N, int M, int k_blocks, TokenTiles tokens, int num_tiles,
+                      int* status)
+{
+    const int stages = pair_stages(tokens.rows), stage_bytes = pair_stage_bytes(tokens.rows);   // a lower tile's copies bring spare rows behind its own
+    extern __shared__ uint8_t smem_raw[];
+    uint8_t* tiles = reinterpret_cast<uint8_t*>((reinterpret_cast<uintptr_t>(smem_raw) + 1023) & ~(uintptr_t)1023);
+    uint64_t* full_bar = reinterpret_cast<uint64_t*>(tiles + PAIR_AREA + 4 * TURN_BYTES);   // the leader's are used
+    uint64_t* empty_bar = full_bar + PAIR_MAX_STAGES;   // every block's own
+    uint64_t* acc_full = empty_bar + PAIR_MAX_STAGES;   // [2] every block's own
+    uint64_t* acc_empty = acc_full + 2;                 // [2] the leader's are used: 256 arrivals
+    uint32_t* tmem_slot = reinterpret_cast<uint32_t*>(acc_empty + 2);
+    volatile int* abort_flag = reinterpret_cast<volatile int*>(tmem_slot + 1);
+
+    const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
+    const uint32_t rank = cluster_ctarank();
+    const int cluster = blockIdx.x >> 1, clusters = gridDim.x >> 1;
+    if (threadIdx.x == 0) {
+        for (int s = 0; s < stages; ++s) {
+            mbar_init(full_bar + s, 1);
+            mbar_init(empty_bar + s, 1);
+        }
+        for (int b = 0; b < 2; ++b) {
+            mbar_init(acc_full + b, 1);
+            mbar_init(acc_empty + b, 256);
+        }
+        *abort_flag = 0;
+        asm volatile("fence.mbarrier_init.release.cluster;" ::: "memory");
+    }
+    if (warp == 1) tmem_alloc_pair(tmem_slot, 2u * PAIR_BN);
+    fence_before_sync();
+    __syncthreads();
+    cluster_sync();   // both blocks' barriers are initialised and their tensor memory is allocated before either is used from the other side
+    fence_after_sync();
+    const uint32_t tmem_base = *tmem_slot;
+
+    pdl_launch_dependents();
+    if (warp == 0) {
+        if (lane == 0) {
+            int s = 0;
+            uint32_t phase = 0;   // of the ring's round; the first round's waits end at once
+            bool ok = true, first = true;
+            for (int tile = cluster; ok && tile < num_tiles; tile += clusters) {
+                const int ty = tile % tokens.count;
+                const int x0 = (tile / tokens.count) * (2 * BM) + (int)rank * BM, y0 = tokens.first(ty) + (int)rank * (tokens.height(ty) / 2);
+                int kb = 0;
+                if (first) {
+                    // the weights of the first stages are requested before the wait for the kernels ahead in the stream
+                    const int pre = min(k_blocks, stages);
+                    for (int i = 0; i < pre; ++i) {
+                        if (rank == 0) mbar_expect_tx(full_bar + i, 2u * stage_bytes);
+                        tma_load_2d_pair(smem_u32(tiles + (size_t)i * stage_bytes), &map_w, i * BK, x0, map_to_rank(smem_u32(full_bar + i), 0));
+                    }
+                    pdl_wait();
+                    for (int i = 0; i < pre; ++i)
+                        tma_load_2d_pair(smem_u32(tiles + (size_t)i * stage_bytes + PAIR_X_BYTES), &map_a, i * BK, y0, map_to_rank(smem_u32(full_bar + i), 0));
+                    kb = pre;
+                    if (pre == stages) phase = 1;
+                    else s = pre;
+                    first = false;
+                }
+                for (; kb < k_blocks; ++kb) {
+                    if (!mbar_wait(empty_bar + s, phase ^ 1, abort_flag)) { ok = false; break; }
+                    uint8_t* xs = tiles + (size_t)s * stage_bytes;
+                    if (rank == 0) mbar_expect_tx(full_bar + s, 2u * stage_bytes);   // both blocks' bytes
+                    const uint32_t leader_full = map_to_rank(smem_u32(full_bar + s), 0);
+                    tma_load_2d_pair(smem_u32(xs), &map_w, kb * BK, x0, leader_full);
+                    tma_load_2d_pair(smem_u32(xs + PAIR_X_BYTES), &map_a, kb * BK, y0, leader_full);
+                    if (++s == stages) {
+                        s = 0;
+                        phase ^= 1;
+                    }
+                }
+            }
+        }
+    } else if (warp == 1) {
+        if (lane == 0 && rank == 0) {
+            int s = 0;
+            uint32_t phase = 0;
+            int i = 0;
+            bool ok = true;
+            for (int tile = cluster; ok && tile < num_tiles; tile += clusters, ++i) {
+                const uint32_t idesc = instr_desc_s8(2 * BM, tokens.height(tile % tokens.count));
+                const int buf = i & 1;
+                const uint32_t aph = (uint32_t)(i >> 1) & 1;
+                if (i >= 2) ok = mbar_wait(acc_empty + buf, aph ^ 1, abort_flag);   // both blocks' epilogues have read this buffer's last tile
+                if (!ok) break;
+                fence_after_sync();
+                const uint32_t acc = tmem_base + (uint32_t)buf * PAIR_BN;
+                for (int kb = 0; kb < k_blocks; ++kb) {
+                    ok = mbar_wait(full_bar + s, phase, abort_flag);
+                    if (!ok) break;
+                    fence_after_sync();
+                    const uint8_t* xs = tiles + (size_t)s * stage_bytes;
+                    const uint64_t dx = desc_k_major(smem_u32(xs)), dy = desc_k_major(smem_u32(xs + PAIR_X_BYTES));
+#pragma unroll
+                    for (int k = 0; k < BK / UMMA_K; ++k) {
+                        const uint64_t adv = (uint64_t)((k * UMMA_K) >> 4);
+                        umma_s8_pair(acc, dx + adv, dy + adv, idesc, (kb > 0 || k > 0) ? 1u : 0u);
+                    }
+                    umma_commit_pair(empty_bar + s);
+                    if (++s == stages) {
+                        s = 0;
+                        phase ^= 1;
+                    }
+                }
+                if (ok) umma_commit_pair(acc_full + buf);
+            }
+        }
+    } else {
+        const int quarter = warp & 3;
+        float* turn = reinterpret_cast<float*>(tiles + PAIR_AREA + quarter * TURN_BYTES);
+        pdl_wait();   // the scales and the output belong to kernels ahead in the stream until here
+        int i = 0;
+        for (int tile = cluster; tile < num_tiles; tile += clusters, ++i) {
+            const int buf = i & 1;
+            const uint32_t aph = (uint32_t)(i >> 1) & 1;
+            const int x0 = (tile / tokens.count) * (2 * BM) + (int)rank * BM + quarter * 32, ty = tile % tokens.count;   // the warp's first weight row
+            const int y0 = tokens.first(ty), height = tokens.height(ty), y_end = min(M, y0 + height);
+            const float sw = x0 + lane < N ? w_scale[x0 + lane] : 0.f;
+            if (!mbar_wait(acc_full + buf, aph, abort_flag)) break;
+            fence_after_sync();
+#pragma unroll 1
+            for (int c = 0; c < height; c += 32) {
+                uint32_t r[32];
+                tmem_load<32>(tmem_base + ((uint32_t)(quarter * 32) << 16) + (uint32_t)(buf * PAIR_BN + c), r);
+                tmem_wait_ld();
+                store_chunk<TC, GATED>(out, ld, lane, x0, y0 + c, N, y_end, r, sw, a_scale, turn);
+            }
+            fence_before_sync();
+            if (rank == 0) mbar_arrive(acc_empty + buf);
+            else mbar_arrive_cluster(map_to_rank(smem_u32(acc_empty + buf), 0));
+        }
+    }
+
+    fence_before_sync();
+    __syncthreads();
+    if (*abort_flag) {
+        if (threadIdx.x == 0) {
+            const unsigned long long t0 = global_timer();
+            while (global_timer() - t0 < 2000000ull) { }
+            report_status(status, SPY_STATUS_WAIT_TIMEOUT, (int)blockIdx.x);
+        }
+        __syncthreads();
+    }
+    cluster_sync();   // neither block leaves (and frees tensor memory the pair shares) while the other may still use it
+    if (warp == 1) {
+        fence_after_sync();
+        tmem_dealloc_pair(tmem_base, 2u * PAIR_BN);
+    }
+}
+
+// A [rows, K] matrix of codes with K contiguous; box = 128 codes x box_rows rows, 128-byte swizzle.
+static int make_map(CUtensorMap* map, const void* ptr, long long rows, long long K, long long ld, int box_rows)
+{
+    EncodeTiledFn fn = encode_tiled_fn();
+    if (!fn) SPY_FAIL("gemm_int8: cuTensorMapEncodeTiled is not available from the driver");
+    cuuint64_t dims[2] = {(cuuint64_t)K, (cuuint64_t)rows};
+    cuuint64_t strides[1] = {(cuuint64_t)ld};
+    cuuint32_t box[2] = {(cuuint32_t)BK, (cuuint32_t)box_rows};
+    cuuint32_t elem[2] = {1, 1};
+    CUresult r = fn(map, CU_TENSOR_MAP_DATA_TYPE_UINT8, 2, const_cast<void*>(ptr), dims, strides, box, elem, CU_TENSOR_MAP_INTERLEAVE_NONE,
+                    CU_TENSOR_MAP_SWIZZLE_128B, CU_TENSOR_MAP_L2_PROMOTION_L2_256B, CU_TENSOR_MAP_FLOAT_OOB_FILL_NONE);
+    if (r != CUDA_SUCCESS) SPY_FAIL("gemm_int8: cuTensorMapEncodeTiled failed with code %d (rows %lld, K %lld, ld %lld)", (int)r, rows, K, ld);
+    return 0;
+}
+
+// How a product is run.  pairs: `count` token tiles on pairs of blocks; else token tiles of `bn` on single blocks with tile_rows weight rows, K cut `splits` ways.
+struct Plan {
+    bool pairs;
+    int count, bn, splits, tile_rows;
+};
+
+static Plan choose(int M, int N, int K)
+{
+    const int k_blocks = (K + BK - 1) / BK, sms = spy_sm_count();
+    Plan p = {false, 0, M <= 16 ? 16 : (M <= 32 ? 32 : (M <= 64 ? 64 : 128)), 1, BM};
+    const long long w_tiles2 = (N + 2 * BM - 1) / (2 * BM);
+    if (M > 128 && w_tiles2 * ((M + 255) / 256) >= sms / 4) {
+        p.pairs = true;
+        p.count = (M + 255) / 256;
+        return p;
+    }
+    const long long tiles = (long long)((N + BM - 1) / BM) * ((M + p.bn - 1) / p.bn);
+    while (p.splits < 8 && tiles * p.splits * 2 <= 2 * sms && k_blocks >= 2 * 2 * p.splits) p.splits *= 2;
+    return p;
+}
+
+template <int BN, typename TC, bool GATED>
+static int launch_few(const Plan& p, const CUtensorMap& mw, const CUtensorMap& ma, const float* w_scale, const float* a_scale, void* C, long long ldc, int M,
+                      int N, int k_blocks, int* status, cudaStream_t stream)
+{
+    using T = Tile<BN>;
+    auto kernel = gemm_int8_few_kernel<BN, TC, GATED>;
+    SPY_ONCE_PER_DEVICE {
+        SPY_CUDA(cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)T::SMEM));
+    }
+    const dim3 grid((unsigned)((M + BN - 1) / BN * p.splits), (unsigned)((N + p.tile_rows - 1) / p.tile_rows));
+    if (grid.y > 65535) SPY_FAIL("gemm_int8: %u weight tiles exceed the launch limits", grid.y);
+    if (p.splits == 1)
+        spy_launch(kernel, grid, dim3(NUM_THREADS), T::SMEM, stream, mw, ma, w_scale, a_scale, (TC*)C, ldc, N, M, k_blocks, p.splits, p.tile_rows, status);
+    else
+        spy_launch_cluster(kernel, grid, dim3(NUM_THREADS), T::SMEM, stream, (unsigned)p.splits, mw, ma, w_scale, a_scale, (TC*)C, ldc, N, M, k_blocks,
+                           p.splits, p.tile_rows, status);
+    SPY_CHECK_LAUNCH("gemm_int8");
+    return 0;
+}
+
+template <typename TC, bool GATED>
+static int launch_pairs(const Plan& p, const CUtensorMap& mw, const CUtensorMap& ma, const float* w_scale, const float* a_scale, void* C, long long ldc, int M,
+                        int N, int k_blocks, const TokenTiles& tokens, int* status, cudaStream_t stream)
+{
+    auto kernel = gemm_int8_pair_kernel<TC, GATED>;
+    static int clusters_of_device[SPY_MAX_DEVICES] = {};
+    int& clusters_max = clusters_of_device[spy_device()];
+    if (clusters_max == 0) {
+        SPY_CUDA(cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)PAIR_SMEM));
+        const int sms = spy_sm_count();
+        cudaLaunchConfig_t cfg = {};
+        cfg.gridDim = dim3(sms / 2 * 2);
+        cfg.blockDim = dim3(NUM_THREADS);
+        cfg.dynamicSmemBytes = PAIR_SMEM;
+        cudaLaunchAttribute attr[1];
+        attr[0].id = cudaLaunchAttributeClusterDimension;
+        attr[0].val.clusterDim.x = 2;
+        attr[0].val.clusterDim.y = 1;
+        attr[0].val.clusterDim.z = 1;
+        cfg.attrs = attr;
+        cfg.numAttrs = 1;
+        int active = 0;
+        SPY_CUDA(cudaOccupancyMaxActiveClusters(&active, kernel, &cfg));
+        if (active <= 0) SPY_FAIL("gemm_int8: no cluster of two blocks fits the device");
+        clusters_max = active < sms / 2 ? active : sms / 2;
+    }
+    const long long num_tiles = (long long)((N + 2 * BM - 1) / (2 * BM)) * tokens.count;
+    if (num_tiles > 0x7fffffffLL) SPY_FAIL("gemm_int8: %lld tiles exceed the kernel's range", num_tiles);
+    const int clusters = (int)(num_tiles < clusters_max ? num_tiles : clusters_max);
+    spy_launch_cluster(kernel, dim3(2 * clusters), dim3(NUM_THREADS), PAIR_SMEM, stream, 2u, mw, ma, w_scale, a_scale, (TC*)C, ldc, N, M, k_blocks, tokens,
+                       (int)num_tiles, status);
+    SPY_CHECK_LAUNCH("gemm_int8 (pairs)");
+    return 0;
+}
+
+template <typename TC, bool GATED>
+static int run(const void* A, long long lda, const float* a_scale, const void* W, long long ldw, const float* w_scale, void* C, long long ldc, int M, int N,
+               int K, int* status, cudaStream_t stream)
+{
+    const Plan p = choose(M, N, K);
+    const int k_blocks = (K + BK - 1) / BK;
+    CUtensorMap mw, ma;
+    if (p.pairs) {
+        const TokenTiles tokens = token_tiles(M, p.count);
+        if (make_map(&mw, W, N, K, ldw, BM) || make_map(&ma, A, M, K, lda, tokens.rows / 2)) return 1;
+        return launch_pairs<TC, GATED>(p, mw, ma, w_scale, a_scale, C, ldc, M, N, k_blocks, tokens, status, stream);
+    }
+    if (make_map(&mw, W, N, K, ldw, p.tile_rows) || make_map(&ma, A, M, K, lda, p.bn)) return 1;
+    if (p.bn == 16) return launch_few<16, TC, GATED>(p, mw, ma, w_scale, a_scale, C, ldc, M, N, k_blocks, status, stream);
+    if (p.bn == 32) return launch_few<32, TC, GATED>(p, mw, ma, w_scale, a_scale, C, ldc, M, N, k_blocks, status, stream);
+    if (p.bn == 64) return launch_few<64, TC, GATED>(p, mw, ma, w_scale, a_scale, C, ldc, M, N, k_blocks, status, stream);
+    return launch_few<128, TC, GATED>(p, mw, ma, w_scale, a_scale, C, ldc, M, N, k_blocks, status, stream);
+}
+
+}  // namespace
+
+// A [M, K] and W [N, K] int8, rows lda / ldw bytes apart (multiples of 16); a_scale [M], w_scale [N]; C [M, N] of c_dtype, rows ldc elements apart.
+// gated: W's rows alternate gate and up rows, C is [M, N / 2] bfloat16.  status: null, or two ints that receive a code if a bounded wait runs out.
+extern "C" int spy_gemm_int8(const void* A, long long lda, const float* a_scale, const void* W, long long ldw, const float* w_scale, void* C, int c_dtype,
+                             long long ldc, int M, int N, int K, int gated, int* status, cudaStream_t stream)
+{
+    if (M <= 0 || N <= 0) return 0;
+    if (K <= 0 || K > MAX_K) SPY_FAIL("gemm_int8: K %d must lie in 1..%d (32-bit sums)", K, MAX_K);
+    if (lda % 16 != 0 || ldw % 16 != 0) SPY_FAIL("gemm_int8: row distances %lld/%lld must be multiples of 16 bytes", lda, ldw);
+    if ((reinterpret_cast<uintptr_t>(A) & 15) || (reinterpret_cast<uintptr_t>(W) & 15)) SPY_FAIL("gemm_int8: operands must be 16-byte aligned");
+    if (gated && (N % 2 != 0 || c_dtype != SPY_BF16)) SPY_FAIL("gemm_int8: the gated epilogue needs an even N and bfloat16 output");
+    if (gated) return run<bf16, true>(A, lda, a_scale, W, ldw, w_scale, C, ldc, M, N, K, status, stream);
+    if (c_dtype == SPY_BF16) return run<bf16, false>(A, lda, a_scale, W, ldw, w_scale, C, ldc, M, N, K, status, stream);
+    if (c_dtype == SPY_F32) return run<float, false>(A, lda, a_scale, W, ldw, w_scale, C, ldc, M, N, K, status, stream);
+    SPY_FAIL("gemm_int8: unknown output dtype code %d", c_dtype);
+}

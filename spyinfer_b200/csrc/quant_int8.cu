@@ -1,0 +1,363 @@
+// Rows of 8-bit codes with one 32-bit scale each, made in one pass over the row:
+//   quantize:  amax = max |x|,  code = the integer nearest 127 x / amax (ties to even),  scale = amax / 127
+//   rms norm:  v = x[row] (+ delta[row], itself possibly a sum of split-K partial products), 32-bit sums, stored into x when write_back;
+//              y = v * w rounded to 32 bits, quantised as above;  scale = amax / 127 / sqrt(mean(v^2) + eps)
+// so that code * scale is the normed row: the factor 1 / sqrt(..) cancels in the codes and goes into the scale alone.
+//
+// The codes are exact: 127 y / amax is compared with the half between two integers without being rounded first.  In 32 bits
+// t = y * (127 / amax) is off by at most |t| 2^-24 <= 7.6e-6 from the quotient (the fused multiply-add rounds t itself to the integer
+// directly), so only where t lies within 2e-5 of a half is the question left open; there 254 y and (2 n + 1) amax are compared without rounding
+// (one group of eight in 3,000).  The codes depend on no summation order and on no approximation, and a test can ask for equality.
+//
+// A row of zeros has codes 0 and scale 0.  A row with a NaN or an infinity has codes 0 and the scale NaN: what is made of it is NaN, and no
+// other row is touched.  |code| <= 127: -128 does not occur.
+//
+// Rows of codes lie a multiple of 16 bytes apart (the product fetches them by TMA); bytes between a row's end and the next row are not written.
+// The reference keeps no 8-bit values anywhere (its weights are half precision: spymaster2h/spyinfer src/utils/safetensors_reader.cpp:101-122).
+#include "common.cuh"
+
+SPY_MODULE(spy_quant_int8)
+
+namespace {
+
+constexpr float MAGIC = 12582912.0f;   // 1.5 * 2^23: added to a small number it leaves the nearest integer in the low bits
+
+__device__ __forceinline__ void load8(const float* p, float (&v)[8])
+{
+    const float4 a = reinterpret_cast<const float4*>(p)[0], b = reinterpret_cast<const float4*>(p)[1];
+    v[0] = a.x; v[1] = a.y; v[2] = a.z; v[3] = a.w;
+    v[4] = b.x; v[5] = b.y; v[6] = b.z; v[7] = b.w;
+}
+__device__ __forceinline__ void load8(const bf16* p, float (&v)[8])
+{
+    const uint4 x = *reinterpret_cast<const uint4*>(p);
+    const uint32_t w[4] = {x.x, x.y, x.z, x.w};
+#pragma unroll
+    for (int i = 0; i < 4; ++i) {
+        v[2 * i] = __uint_as_float(w[i] << 16);
+        v[2 * i + 1] = __uint_as_float(w[i] & 0xffff0000u);
+    }
+}
+__device__ __forceinline__ void store8(float* p, const float (&v)[8])
+{
+    reinterpret_cast<float4*>(p)[0] = make_float4(v[0], v[1], v[2], v[3]);
+    reinterpret_cast<float4*>(p)[1] = make_float4(v[4], v[5], v[6], v[7]);
+}
+__device__ __forceinline__ void store8(bf16* p, const float (&v)[8])
+{
+    uint32_t w[4];
+#pragma unroll
+    for (int i = 0; i < 4; ++i) {
+        const __nv_bfloat162 t = __floats2bfloat162_rn(v[2 * i], v[2 * i + 1]);
+        w[i] = *reinterpret_cast<const uint32_t*>(&t);
+    }
+    *reinterpret_cast<uint4*>(p) = make_uint4(w[0], w[1], w[2], w[3]);
+}
+
+// Threads that hold a row, `groups` times eight elements each.
+__host__ __device__ constexpr int block_most(int groups) { return groups <= 2 ? 1024 : 512; }
+
+// The eight elements of a row that group g of this thread holds; what lies behind the end is zero.  WHOLE: rows of a multiple of 8 elements on
+// 16-byte borders, a thread holds neighbours.  Else a warp's lanes hold neighbours, so that their plain loads and stores meet in few sectors.
+template <bool WHOLE> __device__ __forceinline__ int place(int g, int e) { return WHOLE ? (g * blockDim.x + threadIdx.x) * 8 + e : (g * 8 + e) * blockDim.x + threadIdx.x; }
+template <bool WHOLE, typename T> __device__ __forceinline__ void fetch(const T* row, int g, int len, float (&v)[8])
+{
+#pragma unroll
+    for (int e = 0; e < 8; ++e) v[e] = 0.f;
+    if constexpr (WHOLE) {
+        if (place<true>(g, 0) < len) load8(row + place<true>(g, 0), v);
+    } else {
+#pragma unroll
+        for (int e = 0; e < 8; ++e)
+            if (place<false>(g, e) < len) v[e] = to_f32(row[place<false>(g, e)]);
+    }
+}
+template <bool WHOLE, typename T> __device__ __forceinline__ void put(T* row, int g, int len, const float (&v)[8])
+{
+    if constexpr (WHOLE) {
+        if (place<true>(g, 0) < len) store8(row + place<true>(g, 0), v);
+    } else {
+#pragma unroll
+        for (int e = 0; e < 8; ++e)
+            if (place<false>(g, e) < len) row[place<false>(g, e)] = from_f32<T>(v[e]);
+    }
+}
+
+// The larger of m and |v|, NaN if either is: as bits, where a NaN is above the infinity and that above every number.
+__device__ __forceinline__ uint32_t size_max(uint32_t m, float v) { return max(m, __float_as_uint(v) & 0x7fffffffu); }
+
+// The whole number nearest to 127 y / amax, ties to even, by the sign of 254 y - (2 n + 1) amax with n the whole number below the quotient: hi + lo is
+// the second product exactly, and near the half the fused difference to hi is exact as well (a few of the 31 bits of 254 y are left); elsewhere
+// the sign is plain.
+__device__ __forceinline__ int nearest_exact(float y, float k, float amax)
+{
+    const float n = floorf(y * k), b = 2.0f * n + 1.0f;
+    const float hi = __fmul_rn(b, amax), lo = fmaf(b, amax, -hi), d = fmaf(254.0f, y, -hi);
+    const int low = (int)n;
+    return d > lo ? low + 1 : (d < lo ? low : low + (low & 1));
+}
+
+// The codes of eight numbers, four in a word.  k = 127 / amax.
+__device__ __forceinline__ uint2 encode8(const float (&y)[8], float k, float amax)
+{
+    uint32_t m[8];
+    float far = 0.f;
+#pragma unroll
+    for (int e = 0; e < 8; ++e) {
+        const float n = fmaf(y[e], k, MAGIC);
+        far = fmaxf(far, fabsf(fmaf(y[e], k, MAGIC - n)));
+        m[e] = __float_as_uint(n);
+    }
+    if (far > 0.49998f) {
+#pragma unroll
+        for (int e = 0; e < 8; ++e) m[e] = (uint32_t)nearest_exact(y[e], k, amax);
+    }
+    return make_uint2(__byte_perm(__byte_perm(m[0], m[1], 0x0040), __byte_perm(m[2], m[3], 0x0040), 0x5410),
+                      __byte_perm(__byte_perm(m[4], m[5], 0x0040), __byte_perm(m[6], m[7], 0x0040), 0x5410));
+}
+template <bool WHOLE> __device__ __forceinline__ void put_codes(int8_t* row, int g, int len, uint2 c)
+{
+    if constexpr (WHOLE) {
+        if (place<true>(g, 0) < len) *reinterpret_cast<uint2*>(row + place<true>(g, 0)) = c;
+    } else {
+#pragma unroll
+        for (int e = 0; e < 8; ++e)
+            if (place<false>(g, e) < len) row[place<false>(g, e)] = (int8_t)((e < 4 ? c.x >> (8 * e) : c.y >> (8 * (e - 4))) & 0xffu);
+    }
+}
+
+// What the codes of a row are formed with.  Rows below 2^-100 are lifted by 2^100 first, so that 127 / amax stays a number, and rows above 2^100
+// lowered by 2^-30, so that 255 amax does (exact but for numbers far below half a code); a row of zeros, or with a NaN or an infinity in it, is
+// replaced by zeros.
+struct RowScale {
+    float k, amax, lift;
+    bool plain, none;
+};
+__device__ __forceinline__ RowScale row_scale(uint32_t size)
+{
+    RowScale s;
+    s.none = size == 0 || size >= 0x7f800000u;
+    s.amax = s.none ? 1.f : __uint_as_float(size);
+    s.lift = s.amax < 0x1p-100f ? 0x1p100f : (s.amax > 0x1p100f ? 0x1p-30f : 1.f);
+    s.plain = !s.none && s.lift == 1.f;
+    s.amax *= s.lift;
+    s.k = 127.0f / s.amax;
+    return s;
+}
+__device__ __forceinline__ float scale_of(uint32_t size, float factor)
+{
+    return size >= 0x7f800000u ? __int_as_float(0x7fc00000) : __uint_as_float(size) / 127.0f * factor;
+}
+template <bool WHOLE, int GROUPS>
+__device__ __forceinline__ void encode_row(int8_t* row, int len, float (&y)[GROUPS][8], uint32_t size)
+{
+    const RowScale s = row_scale(size);
+    if (!s.plain) {
+#pragma unroll
+        for (int g = 0; g < GROUPS; ++g)
+#pragma unroll
+            for (int e = 0; e < 8; ++e) y[g][e] = s.none ? 0.f : y[g][e] * s.lift;
+    }
+#pragma unroll
+    for (int g = 0; g < GROUPS; ++g) put_codes<WHOLE>(row, g, len, encode8(y[g], s.k, s.amax));
+}
+
+// Sum and largest size over the block, one barrier; `part` holds 2 x 32 words and is used once a launch.
+template <bool WITH_SUM> __device__ __forceinline__ void block_reduce(float& sum, uint32_t& size, uint32_t* part)
+{
+    const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5, warps = blockDim.x >> 5;
+    size = __reduce_max_sync(0xffffffffu, size);
+    if (WITH_SUM) sum = warp_sum(sum);
+    if (lane == 0) {
+        part[warp] = size;
+        if (WITH_SUM) part[32 + warp] = __float_as_uint(sum);
+    }
+    __syncthreads();
+    size = __reduce_max_sync(0xffffffffu, lane < warps ? part[lane] : 0u);
+    if (WITH_SUM) sum = warp_sum(lane < warps ? __uint_as_float(part[32 + lane]) : 0.f);
+}
+
+template <typename T, bool WHOLE, int GROUPS>
+__global__ void __launch_bounds__(block_most(GROUPS)) quantize_kernel(const T* __restrict__ x, long long ldx, int8_t* __restrict__ codes, long long ldc,
+                                                        float* __restrict__ scales, int len)
+{
+    __shared__ uint32_t part[32];
+    pdl_enter();
+    const T* row = x + (size_t)blockIdx.x * ldx;
+    float v[GROUPS][8];
+#pragma unroll
+    for (int g = 0; g < GROUPS; ++g) fetch<WHOLE>(row, g, len, v[g]);
+    uint32_t size = 0;
+    float none = 0.f;
+#pragma unroll
+    for (int g = 0; g < GROUPS; ++g)
+#pragma unroll
+        for (int e = 0; e < 8; ++e) size = size_max(size, v[g][e]);
+    block_reduce<false>(none, size, part);
+    encode_row<WHOLE, GROUPS>(codes + (size_t)blockIdx.x * ldc, len, v, size);
+    if (threadIdx.x == 0) scales[blockIdx.x] = scale_of(size, 1.f);
+}
+
+// Rows longer than a block holds: read once for the largest size and once more, from L2, for the codes.
+template <typename T>
+__global__ void __launch_bounds__(1024) quantize_long_kernel(const T* __restrict__ x, long long ldx, int8_t* __restrict__ codes, long long ldc,
+                                                             float* __restrict__ scales, int len)
+{
+    __shared__ uint32_t part[32];
+    pdl_enter();
+    const T* row = x + (size_t)blockIdx.x * ldx;
+    uint32_t size = 0;
+    float none = 0.f;
+    const int piece = blockDim.x * 8;
+    for (int at = 0; len - at > 0; at += piece) {
+        float v[8];
+        fetch<false>(row + at, 0, len - at, v);
+#pragma unroll
+        for (int e = 0; e < 8; ++e) size = size_max(size, v[e]);
+        if (len - at <= piece) break;
+    }
+    block_reduce<false>(none, size, part);
+    int8_t* out = codes + (size_t)blockIdx.x * ldc;
+    for (int at = 0; len - at > 0; at += piece) {
+        float v[1][8];
+        fetch<false>(row + at, 0, len - at, v[0]);
+        encode_row<false, 1>(out + at, len - at, v, size);
+        if (len - at <= piece) break;
+    }
+    if (threadIdx.x == 0) scales[blockIdx.x] = scale_of(size, 1.f);
+}
+
+template <typename TX, typename TD, typename TW, bool WHOLE, int GROUPS>
+__global__ void __launch_bounds__(block_most(GROUPS)) rmsnorm_int8_kernel(TX* x, const TD* __restrict__ delta, int splits, long long split_stride, const int* __restrict__ rows,
+                                                            const TW* __restrict__ w, int8_t* __restrict__ codes, long long ldc,
+                                                            float* __restrict__ scales, int len, float eps, int write_back)
+{
+    __shared__ uint32_t part[64];
+    pdl_launch_dependents();
+    // few rows: the weight, which depends on no kernel ahead in the stream, is loaded before the wait for them
+    float w_first[8];
+    if constexpr (GROUPS == 1) fetch<WHOLE>(w, 0, len, w_first);
+    pdl_wait();
+    const int src = rows ? rows[blockIdx.x] : blockIdx.x;
+    TX* xr = x + (size_t)src * len;
+    const TD* dr = delta ? delta + (size_t)src * len : nullptr;
+    float v[GROUPS][8];
+#pragma unroll
+    for (int g = 0; g < GROUPS; ++g) fetch<WHOLE>(xr, g, len, v[g]);
+    for (int s = 0; s < splits; ++s) {       // the partial products are added in their order
+#pragma unroll
+        for (int g = 0; g < GROUPS; ++g) {
+            float d[8];
+            fetch<WHOLE>(dr + (size_t)s * split_stride, g, len, d);
+#pragma unroll
+            for (int e = 0; e < 8; ++e) v[g][e] = __fadd_rn(v[g][e], d[e]);
+        }
+    }
+    float ss = 0.f;
+    uint32_t size = 0;
+#pragma unroll
+    for (int g = 0; g < GROUPS; ++g) {
+        if (write_back) put<WHOLE>(xr, g, len, v[g]);
+        float wv[8];
+        if constexpr (GROUPS > 1) fetch<WHOLE>(w, g, len, wv);
+#pragma unroll
+        for (int e = 0; e < 8; ++e) {
+            ss += v[g][e] * v[g][e];
+            v[g][e] = __fmul_rn(v[g][e], GROUPS > 1 ? wv[e] : w_first[e]);
+            size = size_max(size, v[g][e]);
+        }
+    }
+    block_reduce<true>(ss, size, part);
+    encode_row<WHOLE, GROUPS>(codes + (size_t)blockIdx.x * ldc, len, v, size);
+    if (threadIdx.x == 0) scales[blockIdx.x] = scale_of(size, 1.0f / sqrtf(ss / (float)len + eps));
+}
+
+constexpr int ROW_MOST = 8 * 8 * block_most(8);    // elements that a block holds
+
+// How a row is shared out: few rows (decoding) as wide as it goes, many rows 32 elements a thread, all their loads in flight together and
+// several blocks an SM.
+static inline int row_groups(bool whole, int n, int len)
+{
+    if (len > 8 * 4 * block_most(4)) return 8;
+    if (!whole || n >= 512) return 4;
+    return len > 8 * block_most(1) ? 2 : 1;
+}
+static inline int row_threads(int len, int groups)
+{
+    const int t = ((len + 8 * groups - 1) / (8 * groups) + 31) / 32 * 32;
+    return t < 64 ? 64 : t;
+}
+static inline bool aligned16(const void* p) { return (reinterpret_cast<uintptr_t>(p) & 15) == 0; }
+
+template <typename T>
+static int quantize(const T* x, long long ldx, int8_t* codes, long long ldc, float* scales, int n, int len, cudaStream_t stream)
+{
+    const bool whole = len % 8 == 0 && aligned16(x) && ldx * (long long)sizeof(T) % 16 == 0;
+    if (len > ROW_MOST) {
+        spy_launch(quantize_long_kernel<T>, dim3(n), dim3(1024), 0, stream, x, ldx, codes, ldc, scales, len);
+        SPY_CHECK_LAUNCH("quantize_int8 (long rows)");
+        return 0;
+    }
+    const int groups = row_groups(whole, n, len);
+    auto kernel = groups == 8 ? (whole ? quantize_kernel<T, true, 8> : quantize_kernel<T, false, 8>)
+                : groups == 4 ? (whole ? quantize_kernel<T, true, 4> : quantize_kernel<T, false, 4>)
+                : groups == 2 ? quantize_kernel<T, true, 2> : quantize_kernel<T, true, 1>;
+    spy_launch(kernel, dim3(n), dim3(row_threads(len, groups)), 0, stream, x, ldx, codes, ldc, scales, len);
+    SPY_CHECK_LAUNCH("quantize_int8");
+    return 0;
+}
+
+template <typename TX, typename TD, typename TW>
+static int norm(TX* x, const TD* delta, int splits, long long split_stride, const int* rows, const TW* w, int8_t* codes, long long ldc, float* scales,
+                int n, int len, float eps, int write_back, cudaStream_t stream)
+{
+    const bool whole = len % 8 == 0 && aligned16(x) && aligned16(delta) && aligned16(w) && split_stride * (long long)sizeof(TD) % 16 == 0;
+    const int groups = row_groups(whole, n, len);
+    auto kernel = groups == 8 ? (whole ? rmsnorm_int8_kernel<TX, TD, TW, true, 8> : rmsnorm_int8_kernel<TX, TD, TW, false, 8>)
+                : groups == 4 ? (whole ? rmsnorm_int8_kernel<TX, TD, TW, true, 4> : rmsnorm_int8_kernel<TX, TD, TW, false, 4>)
+                : groups == 2 ? rmsnorm_int8_kernel<TX, TD, TW, true, 2> : rmsnorm_int8_kernel<TX, TD, TW, true, 1>;
+    spy_launch(kernel, dim3(n), dim3(row_threads(len, groups)), 0, stream, x, delta, splits, split_stride, rows, w, codes, ldc, scales, len, eps,
+               write_back);
+    SPY_CHECK_LAUNCH("rmsnorm_int8");
+    return 0;
+}
+
+static int check_codes(const char* what, const void* codes, long long ldc, int len)
+{
+    if (len <= 0) SPY_FAIL("%s: row length %d must be positive", what, len);
+    if (!aligned16(codes) || ldc % 16 != 0) SPY_FAIL("%s: rows of codes must start on 16-byte borders (row distance %lld)", what, ldc);
+    return 0;
+}
+
+}  // namespace
+
+// x: [n, len] of dtype, rows ldx elements apart; codes: [n, len], rows ldc bytes apart (a multiple of 16); scales: [n].
+extern "C" int spy_quantize_int8(const void* x, int dtype, long long ldx, int8_t* codes, long long ldc, float* scales, int n, int len, cudaStream_t stream)
+{
+    if (n <= 0) return 0;
+    if (int rc = check_codes("quantize_int8", codes, ldc, len)) return rc;
+    SPY_DISPATCH_DTYPE(dtype, T, { return quantize<T>((const T*)x, ldx, codes, ldc, scales, n, len, stream); })
+    return 0;
+}
+
+// x: [*, len] of x_dtype; delta: null or `splits` stacked [*, len] arrays of delta_dtype, split_stride elements apart, added to x in order;
+// rows: null or n row indices (gather); w: [len] of w_dtype; codes and scales as above.  write_back stores the sum into x and needs rows == null.
+extern "C" int spy_rmsnorm_int8(void* x, int x_dtype, const void* delta, int delta_dtype, int splits, long long split_stride, const int* rows,
+                                const void* w, int w_dtype, int8_t* codes, long long ldc, float* scales, int n, int len, float eps, int write_back,
+                                cudaStream_t stream)
+{
+    if (n <= 0) return 0;
+    if (int rc = check_codes("rmsnorm_int8", codes, ldc, len)) return rc;
+    if (len > ROW_MOST) SPY_FAIL("rmsnorm_int8: a row of %d elements is longer than %d", len, ROW_MOST);
+    if (write_back && rows) SPY_FAIL("rmsnorm_int8: write_back with a row gather is not defined");
+    if (delta && splits <= 0) SPY_FAIL("rmsnorm_int8: splits %d must be positive", splits);
+    if (!delta) { delta_dtype = x_dtype; splits = 0; split_stride = 0; write_back = 0; }
+    SPY_DISPATCH_DTYPE(x_dtype, TX, {
+        SPY_DISPATCH_DTYPE(delta_dtype, TD, {
+            SPY_DISPATCH_DTYPE(w_dtype, TW, {
+                return norm<TX, TD, TW>((TX*)x, (const TD*)delta, splits, split_stride, rows, (const TW*)w, codes, ldc, scales, n, len, eps, write_back, stream);
+            })
+        })
+    })
+    return 0;
+}

@@ -8,7 +8,7 @@ from __future__ import annotations
 
 import ctypes
 import functools
-from typing import Optional
+from typing import NamedTuple, Optional
 
 import torch
 
@@ -2075,3 +2075,135 @@ def moe_combine(rows: torch.Tensor, slot: torch.Tensor, shared: Optional[torch.T
     _call("moe", "spy_moe_combine", _ptr(rows), _code(rows, "expert results"), _ptr(slot), top, _ptr(shared), _ptr(out), T, rows.shape[1], _stream())
     return out
 
+
+# ---- rows of 8-bit codes -------------------------------------------------------------------------------------------------------
+class Int8Rows(NamedTuple):
+    """A matrix held in 8 bits: ``codes [rows, len]`` int8, whose rows start on 16-byte borders (``empty_int8``), and one float32 scale a row;
+    the values are ``codes * scales[:, None]``.  Activations have a scale for every token, weights ``[out, in]`` one for every output channel."""
+
+    codes: torch.Tensor
+    scales: torch.Tensor
+
+    @property
+    def shape(self):
+        return self.codes.shape
+
+    @property
+    def device(self):
+        return self.codes.device
+
+
+def empty_int8(rows: int, length: int, device) -> Int8Rows:
+    """Room for ``rows`` rows of ``length`` codes, a multiple of 16 bytes apart, and their scales."""
+    pitch = (length + 15) // 16 * 16
+    codes = torch.empty((rows, pitch), dtype=torch.int8, device=device)
+    return Int8Rows(codes if pitch == length else codes[:, :length], torch.empty((rows,), dtype=torch.float32, device=device))
+
+
+def _on_current_device(t: torch.Tensor, what: str) -> None:
+    if t.device.index != torch.cuda.current_device():
+        raise KernelError(f"{what}: lies on {t.device}, the current device is cuda:{torch.cuda.current_device()}")
+
+
+def _check_int8(m: Int8Rows, what: str) -> int:
+    """Returns the distance between the rows of codes in bytes."""
+    if not isinstance(m, Int8Rows):
+        raise KernelError(f"{what}: expected Int8Rows (codes and scales), found {type(m).__name__}")
+    codes, scales = m
+    if not isinstance(codes, torch.Tensor) or not codes.is_cuda or codes.dtype != torch.int8 or codes.dim() != 2:
+        raise KernelError(f"{what}: expected a CUDA matrix of int8 codes")
+    if not isinstance(scales, torch.Tensor) or scales.dtype != torch.float32 or scales.dim() != 1 or scales.shape[0] != codes.shape[0] \
+            or scales.device != codes.device or not scales.is_contiguous():
+        raise KernelError(f"{what}: expected one float32 scale a row, contiguous and on the codes' device")
+    _on_current_device(codes, what)
+    rows, length = codes.shape
+    pitch = codes.stride(0)
+    if rows <= 1 or length == 0:
+        pitch = (length + 15) // 16 * 16
+    if (length > 1 and codes.stride(1) != 1) or pitch < length or pitch % 16 != 0 or codes.data_ptr() % 16 != 0:
+        raise KernelError(f"{what}: rows of codes must be contiguous and start on 16-byte borders, found strides {codes.stride()} at address "
+                          f"{codes.data_ptr():#x} (empty_int8 makes such rows)")
+    return pitch
+
+
+def quantize_int8(x: torch.Tensor, out: Optional[Int8Rows] = None) -> Int8Rows:
+    """Every row of ``x [rows, len]`` (float32 or bfloat16; the rows contiguous, possibly apart) in 8 bits: ``scale = max |x| / 127`` and ``code`` the
+    integer nearest to ``127 x / max |x|``, ties to even, without a rounding of the quotient.  A row of zeros has codes and scale 0; a row with a NaN
+    or an infinity has codes 0 and the scale NaN."""
+    code = _code(x, "quantize_int8 input")
+    ldx = _check_weight(x, "quantize_int8 input")
+    _on_current_device(x, "quantize_int8 input")
+    n, length = x.shape
+    if out is None:
+        out = empty_int8(n, length, x.device)
+    pitch = _check_int8(out, "quantize_int8 output")
+    if tuple(out.codes.shape) != (n, length) or out.device != x.device:
+        raise KernelError(f"quantize_int8 output: {tuple(out.codes.shape)} on {out.device} does not fit the input {tuple(x.shape)} on {x.device}")
+    if n > 1 and ldx < length:
+        raise KernelError(f"quantize_int8 input: rows overlap (strides {x.stride()} for shape {tuple(x.shape)})")
+    _call("quant_int8", "spy_quantize_int8", _ptr(x), code, ctypes.c_longlong(ldx), _ptr(out.codes), ctypes.c_longlong(pitch), _ptr(out.scales), n, length, _stream())
+    return out
+
+
+def rmsnorm_int8(x: torch.Tensor, weight: torch.Tensor, eps: float, out: Optional[Int8Rows] = None, delta: Optional[torch.Tensor] = None,
+                 rows: Optional[torch.Tensor] = None, write_back: bool = False) -> Int8Rows:
+    """``rmsnorm(x [+ delta]) * weight`` row by row as ``rmsnorm`` has it, the result in 8 bits for ``gemm_int8``.  The row that is quantised is ``y = (x + delta)
+    * weight`` in 32 bits: ``code`` is the integer nearest to ``127 y / max |y|`` (as ``quantize_int8``), and the scale ``max |y| / 127 / sqrt(mean((x + delta)^2)
+    + eps)``.  ``delta``: x's shape, or a stack ``[splits, rows, len]`` of partial sums that are added in order; ``write_back`` stores the sum into ``x``; ``rows``
+    gathers rows of x (and delta).  Rows of up to 32,768 elements."""
+    _check(x, "rmsnorm_int8 input", ndim=2)
+    _on_current_device(x, "rmsnorm_int8 input")
+    _check(weight, "rmsnorm_int8 weight", ndim=1)
+    H = x.shape[1]
+    if weight.shape[0] != H:
+        raise KernelError(f"rmsnorm_int8: row lengths differ: input {H}, weight {weight.shape[0]}")
+    d, splits, split_stride = _stack_of(delta, x, "rmsnorm_int8 delta")
+    if d is not None and splits == 0:
+        raise KernelError("rmsnorm_int8 delta: an empty stack")
+    n = x.shape[0]
+    if rows is not None:
+        _check(rows, "rmsnorm_int8 rows", torch.int32, 1)
+        n = rows.shape[0]
+        if write_back:
+            raise KernelError("rmsnorm_int8: write_back with a row gather is not defined")
+    for t, what in ((weight, "weight"), (d, "delta"), (rows, "rows")):
+        if t is not None and t.device != x.device:
+            raise KernelError(f"rmsnorm_int8 {what}: lies on {t.device}, the input on {x.device}")
+    if out is None:
+        out = empty_int8(n, H, x.device)
+    pitch = _check_int8(out, "rmsnorm_int8 output")
+    if tuple(out.codes.shape) != (n, H) or out.device != x.device:
+        raise KernelError(f"rmsnorm_int8 output: expected {(n, H)} on {x.device}, found {tuple(out.codes.shape)} on {out.device}")
+    _call("quant_int8", "spy_rmsnorm_int8", _ptr(x), _code(x, "rmsnorm_int8 input"), _ptr(d), _code(d, "rmsnorm_int8 delta") if d is not None else 0, splits,
+          ctypes.c_longlong(split_stride), _ptr(rows), _ptr(weight), _code(weight, "rmsnorm_int8 weight"), _ptr(out.codes), ctypes.c_longlong(pitch),
+          _ptr(out.scales), n, H, ctypes.c_float(eps), int(bool(write_back)), _stream())
+    return out
+
+
+def gemm_int8(a: Int8Rows, w: Int8Rows, out: Optional[torch.Tensor] = None, status: Optional[torch.Tensor] = None, out_dtype: Optional[torch.dtype] = None,
+              epilogue: Optional[str] = None) -> torch.Tensor:
+    """``a [M, K] @ w [N, K]^T`` of 8-bit rows on the tensor cores, ``(sum_k a w) * a.scales[m] * w.scales[n]`` with the sum in 32-bit integers (exact; K below
+    131,072), in bfloat16 (default) or float32.  ``epilogue="swiglu"``: ``w``'s rows alternate gate and up rows and the result is ``silu(gate) * up``,
+    ``[M, N / 2]`` bfloat16.  A row whose scale is NaN gives a row of NaN.  A token's result does not depend on the rest of the batch."""
+    lda, ldw = _check_int8(a, "gemm_int8 input"), _check_int8(w, "gemm_int8 weight")
+    M, K = a.codes.shape
+    N = w.codes.shape[0]
+    if w.codes.shape[1] != K:
+        raise KernelError(f"gemm_int8: shapes do not fit: input {tuple(a.codes.shape)}, weight {tuple(w.codes.shape)}")
+    if epilogue not in (None, "swiglu"):
+        raise KernelError(f"gemm_int8: unknown epilogue {epilogue!r}")
+    n_out = N // 2 if epilogue else N
+    if out is None:
+        out = torch.empty((M, n_out), dtype=out_dtype or torch.bfloat16, device=a.codes.device)
+    else:
+        _check(out, "gemm_int8 output", out_dtype, 2)
+        if tuple(out.shape) != (M, n_out) or out.device != a.codes.device:
+            raise KernelError(f"gemm_int8: output {tuple(out.shape)} on {out.device} does not fit [{M}, {n_out}] on {a.codes.device}")
+    if status is None:
+        if str(a.codes.device) not in _status_words and torch.cuda.is_current_stream_capturing():
+            raise KernelError("gemm_int8: the device's status word does not exist yet and must not come from a graph's memory: make one call (or "
+                              "status_word()) before the capture, or give a status")
+        status = status_word(a.codes.device)
+    _call("gemm_int8", "spy_gemm_int8", _ptr(a.codes), ctypes.c_longlong(lda), _ptr(a.scales), _ptr(w.codes), ctypes.c_longlong(ldw), _ptr(w.scales), _ptr(out),
+          _code(out, "gemm_int8 output"), ctypes.c_longlong(n_out), M, N, K, int(epilogue is not None), _ptr(status), _stream())
+    return out

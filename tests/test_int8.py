@@ -1,0 +1,353 @@
+"""Rows of 8-bit codes: the quantisation, the norm that ends in it and the matrix product, each against a statement of its formula in 64 bits.
+
+The codes are whole numbers defined without a rounding, so they are compared for equality: in float64 the quotient ``127 y / max |y|`` of two float32
+numbers is formed to 2^-53, and a quotient that is not a half is at least 2^-34 of itself away from one (``254 y`` and ``(2 n + 1) max |y|`` have at most 32
+significant bits).  Sums of products are compared through what was made of them: integers below 2^53 are exact in float64."""
+import pytest
+import torch
+
+from spyinfer_b200 import kernels
+from spyinfer_b200.kernels import Int8Rows, KernelError
+
+DEV = "cuda:0"
+gpu = pytest.mark.gpu
+STEP = {torch.bfloat16: 2.0 ** -8, torch.float32: 2.0 ** -24}      # a rounding is off by at most this, relative to the value
+
+
+@pytest.fixture(autouse=True)
+def guard_zones(guarded_allocations):
+    yield guarded_allocations
+
+
+def codes_of(y):
+    """(codes, largest size, usable) of float32 rows, in 64 bits."""
+    y = y.double()
+    top = y.abs().amax(1) if y.shape[1] else y.new_zeros(y.shape[0])
+    fine = torch.isfinite(y).all(1)
+    safe = torch.where(fine & (top > 0), top, torch.ones_like(top))
+    q = torch.round(torch.where(fine[:, None], y, torch.zeros_like(y)) * 127.0 / safe[:, None])
+    return q.to(torch.int64), top, fine
+
+
+def check_rows(got, y, factor=None, factor_err=0.0):
+    """The codes of float32 rows ``y`` exactly; the scales to their roundings (one division, one product) and what ``factor`` is off by."""
+    q, top, fine = codes_of(y)
+    assert torch.equal(got.codes.to(torch.int64), q)
+    want = top / 127.0 * (1.0 if factor is None else factor)
+    err = (got.scales.double() - want).abs()
+    assert bool((err[fine] <= (2.1 * 2.0 ** -24 + factor_err) * want[fine] + 2.0 ** -149).all())
+    assert bool(torch.isnan(got.scales[~fine]).all())
+
+
+def wild_rows(rows, length, seed=0):
+    g = torch.Generator(device=DEV).manual_seed(seed)
+    return torch.randn(rows, length, generator=g, device=DEV) * torch.exp(2.0 * torch.randn(rows, length, generator=g, device=DEV))
+
+
+@gpu
+@pytest.mark.parametrize("dtype", [torch.float32, torch.bfloat16])
+@pytest.mark.parametrize("length", [1, 2, 7, 8, 15, 16, 33, 100, 513, 1000, 4096, 4999, 8200, 12288, 16392, 20001, 32768, 32769, 40008])
+@pytest.mark.parametrize("rows", [1, 5, 530])
+def test_quantize(rows, length, dtype):
+    x = wild_rows(rows, length).to(dtype)
+    check_rows(kernels.quantize_int8(x), x.float())
+
+
+@gpu
+@pytest.mark.parametrize("dtype", [torch.float32, torch.bfloat16])
+@pytest.mark.parametrize("length", [40, 257, 4096, 16400, 33000])
+def test_quantize_rows_at_the_edges(length, dtype):
+    """Halves between two codes in both directions, the smallest and largest numbers, zeros of both signs, and rows that are not finite beside
+    rows that are."""
+    top = torch.finfo(dtype).max
+    tiny = 2.0 ** -149 if dtype == torch.float32 else 2.0 ** -133
+    x = wild_rows(12, length, 3)
+    x[0] = (torch.arange(length, device=DEV) % 254 - 127).float() + 0.5      # halves, with the largest size 127
+    x[0, 0] = 127.0
+    x[1] = 0.0
+    x[2] = -0.0
+    x[3] = x[0] * 2.0 ** -120
+    x[4] = torch.where(x[4] > 0, tiny, -3 * tiny)
+    x[5] = 0.0
+    x[5, length // 2] = tiny
+    x[6] = torch.where(x[6] > 1.0, top, x[6].clamp(-1.0, 1.0) * 1e36)
+    x[6, 3] = -top
+    x[7, length - 1] = float("nan")
+    x[8, 0] = float("inf")
+    x[9, length // 3], x[9, length // 2] = float("-inf"), float("nan")
+    x[10] = x[0] * 2.0 ** 117
+    x = x.to(dtype)
+    got = kernels.quantize_int8(x)
+    check_rows(got, x.float())
+    assert float(got.scales[1]) == 0.0 and int(got.codes[7:10].abs().max()) == 0
+    assert int(got.codes.min()) >= -127
+
+
+@gpu
+@pytest.mark.parametrize("dtype", [torch.float32, torch.bfloat16])
+def test_quantize_views(dtype):
+    """Rows that lie apart or start off a 16-byte border, and codes into a part of a wider matrix, whose other bytes stay."""
+    wide = wild_rows(40, 300, 5).to(dtype)
+    for first, end in ((0, 128), (8, 264), (1, 258), (3, 4)):
+        check_rows(kernels.quantize_int8(wide[:, first:end]), wide[:, first:end].float())
+    held = torch.full((42, 320), 77, dtype=torch.int8, device=DEV)
+    scales = torch.full((42,), 9.0, device=DEV)
+    out = Int8Rows(held[1:41, 16:16 + 250], scales[1:41])
+    kernels.quantize_int8(wide[:, :250], out)
+    check_rows(out, wide[:, :250].float())
+    held[1:41, 16:16 + 250] = 77
+    assert bool((held == 77).all()) and float(scales[0]) == float(scales[41]) == 9.0
+
+
+@gpu
+@pytest.mark.parametrize("xd,dd,wd", [(torch.float32, torch.bfloat16, torch.bfloat16), (torch.float32, torch.float32, torch.bfloat16),
+                                      (torch.float32, torch.float32, torch.float32), (torch.bfloat16, torch.bfloat16, torch.float32),
+                                      (torch.bfloat16, torch.float32, torch.bfloat16)])
+@pytest.mark.parametrize("rows,length", [(1, 1), (3, 8), (2, 100), (4, 1001), (1, 4096), (520, 64), (515, 4096), (3, 5120), (2, 8200), (513, 8200), (2, 16392),
+                                         (2, 32768), (3, 20003)])
+def test_norm(rows, length, xd, dd, wd):
+    """The stream after the sum, the codes and the scales: alone, with a delta, with a stack of partial sums, and gathered.  The mean square is a
+    sum of positive terms: any order of summation is off by at most (terms + 2) roundings, the inverse root by half of that and two more."""
+    x, w = wild_rows(rows, length, 1).to(xd), (1 + 0.2 * torch.randn(length, device=DEV)).to(wd)
+    delta, stack, eps = wild_rows(rows, length, 2).to(dd), wild_rows(3 * rows, length, 4).view(3, rows, length), 1e-5
+
+    def check(got, v):
+        factor = 1.0 / torch.sqrt(v.double().square().mean(1) + eps)
+        check_rows(got, v * w.float(), factor, (length / 2 + 4) * 2.0 ** -24)
+
+    check(kernels.rmsnorm_int8(x, w, eps), x.float())
+    total = x.float() + delta.float()
+    kept = x.clone()
+    check(kernels.rmsnorm_int8(x, w, eps, delta=delta), total)
+    assert torch.equal(x, kept)
+    check(kernels.rmsnorm_int8(x, w, eps, delta=delta, write_back=True), total)
+    assert torch.equal(x, total.to(xd))
+    x = kept.clone()
+    total = ((x.float() + stack[0]) + stack[1]) + stack[2]
+    check(kernels.rmsnorm_int8(x, w, eps, delta=stack, write_back=True), total)
+    assert torch.equal(x, total.to(xd))
+    picked = torch.tensor([rows - 1, 0, rows // 2, 0], dtype=torch.int32, device=DEV)
+    check(kernels.rmsnorm_int8(kept, w, eps, delta=delta, rows=picked), (kept.float() + delta.float())[picked.long()])
+
+
+@gpu
+def test_norm_rows_at_the_edges():
+    length, eps = 72, 1e-6
+    x = wild_rows(6, length, 7)
+    w = 1 + 0.2 * torch.randn(length, device=DEV)
+    x[0] = 0.0
+    x[1, 5] = float("nan")
+    x[2, 71] = float("inf")
+    x[3] *= 2.0 ** -126
+    x[4] *= 2.0 ** -30
+    got = kernels.rmsnorm_int8(x, w, eps)
+    check_rows(got, x * w, 1.0 / torch.sqrt(x.double().square().mean(1) + eps), (length / 2 + 4) * 2.0 ** -24)
+    assert float(got.scales[0]) == 0.0 and bool(torch.isnan(got.scales[1:3]).all()) and bool(torch.isfinite(got.scales[3:]).all())
+
+
+def rows_of_codes(rows, length, seed, pitch=None, full=False):
+    g = torch.Generator(device=DEV).manual_seed(seed)
+    pitch = pitch or (length + 15) // 16 * 16
+    held = torch.full((rows, pitch), -99, dtype=torch.int8, device=DEV)       # what lies between the rows must not count
+    held[:, :length] = torch.randint(-128, 128, (rows, length), generator=g, device=DEV, dtype=torch.int64).to(torch.int8) if not full else full
+    return Int8Rows(held[:, :length], 0.01 * torch.rand(rows, generator=g, device=DEV) + 1e-4)
+
+
+def product_of(a, w):
+    """The product in 64 bits: the sums are whole numbers below 2^53."""
+    return (a.codes.double() @ w.codes.double().t()) * a.scales.double()[:, None] * w.scales.double()
+
+
+def check_product(got, ref, dtype):
+    assert got.dtype == dtype
+    err = (got.double() - ref).abs()
+    # the sum to 32 bits, two products, and the result's own rounding
+    assert bool((err <= (STEP[dtype] + 3.1 * 2.0 ** -24) * ref.abs()).all()), float((err / ref.abs().clamp_min(1e-300)).max())
+
+
+def check_gated(got, ref, ref_err=0.0):
+    g, u = ref[:, 0::2], ref[:, 1::2]
+    want = g * torch.sigmoid(g) * u
+    # beside the result's rounding: gate and up to 3 roundings each (the gate's also through the exponential), an exponential to 2 + |g| steps of
+    # 2^-22, a division and a product
+    tol = (2.0 ** -8 + (8 + 2 * g.abs()) * 2.0 ** -22) * want.abs() + 1e-37 * u.abs()
+    err = (got.double() - want).abs()
+    assert got.dtype == torch.bfloat16 and bool((err <= tol).all()), float((err / tol).max())
+
+
+SHAPES = [(1, 1, 1), (1, 33, 16), (2, 130, 15), (3, 64, 127), (7, 4, 128), (16, 200, 129), (17, 256, 700), (32, 129, 144), (33, 1000, 300), (64, 132, 2055),
+          (65, 300, 4100), (100, 4100, 512), (128, 514, 1024), (129, 5003, 257), (200, 260, 640), (256, 9600, 130), (257, 1187, 384), (301, 5003, 96),
+          (520, 4864, 320), (1031, 2570, 160), (2050, 1030, 64), (700, 70, 1000)]
+
+
+@gpu
+@pytest.mark.parametrize("M,N,K", SHAPES)
+def test_product(M, N, K):
+    a, w = rows_of_codes(M, K, 1), rows_of_codes(N, K, 2)
+    ref = product_of(a, w)
+    for dtype in (torch.bfloat16, torch.float32):
+        got = kernels.gemm_int8(a, w, out_dtype=dtype)
+        check_product(got, ref, dtype)
+        again = torch.empty(M, N, dtype=dtype, device=DEV)
+        assert kernels.gemm_int8(a, w, out=again) is again and torch.equal(again, got)
+    # a token's result is the same in every company
+    for t in {0, M // 2, M - 1}:
+        alone = kernels.gemm_int8(Int8Rows(a.codes[t:t + 1], a.scales[t:t + 1]), w, out_dtype=torch.float32)
+        assert torch.equal(alone[0], got[t])
+
+
+@gpu
+@pytest.mark.parametrize("M,N,K", [(m, n + n % 2, k) for m, n, k in SHAPES])
+def test_product_gated(M, N, K):
+    a, w = rows_of_codes(M, K, 3), rows_of_codes(N, K, 4)
+    w = Int8Rows(w.codes, w.scales * (8.0 / K ** 0.5))      # gates between about -30 and 30
+    got = kernels.gemm_int8(a, w, epilogue="swiglu")
+    check_gated(got, product_of(a, w))
+    alone = kernels.gemm_int8(Int8Rows(a.codes[M - 1:], a.scales[M - 1:]), w, epilogue="swiglu")
+    assert torch.equal(alone[0], got[M - 1])
+
+
+@gpu
+@pytest.mark.parametrize("M", [3, 140])
+def test_product_of_the_largest_sums(M):
+    """K at its limit with every code -128: 2^31 - 16,384, the largest sum there is, and its negative."""
+    K, N = 131071, 20000 if M > 128 else 40
+    a, w = rows_of_codes(M, K, 1, full=-128), rows_of_codes(40, K, 2, full=-128)
+    w.codes[5] = 127
+    w = Int8Rows(w.codes[torch.arange(N, device=DEV) % 40] if N > 40 else w.codes, w.scales[torch.arange(N, device=DEV) % 40].contiguous())
+    if N > 40:
+        held = torch.zeros(N, (K + 15) // 16 * 16, dtype=torch.int8, device=DEV)
+        held[:, :K] = w.codes
+        w = Int8Rows(held[:, :K], w.scales)
+    check_product(kernels.gemm_int8(a, w, out_dtype=torch.float32), product_of(a, Int8Rows(w.codes[:40], w.scales[:40])).repeat(1, N // 40), torch.float32)
+
+
+@gpu
+@pytest.mark.parametrize("M", [5, 150])
+def test_product_scales_and_views(M):
+    """Parts of wider matrices, scales of zero, and a row that is not a number: it alone gives NaN."""
+    K, N = 208, 19000 if M > 128 else 131
+    a, w = rows_of_codes(M, 400, 1), rows_of_codes(N, 400, 2)
+    a, w = Int8Rows(a.codes[:, 32:32 + K], a.scales), Int8Rows(w.codes[:, 176:176 + K], w.scales)
+    check_product(kernels.gemm_int8(a, w), product_of(a, w), torch.bfloat16)
+    a.scales[1], a.scales[2], w.scales[7] = float("nan"), 0.0, 0.0
+    got = kernels.gemm_int8(a, w, out_dtype=torch.float32)
+    ref = product_of(a, w)
+    assert bool(torch.isnan(got[1]).all()) and not bool(torch.isnan(got[torch.arange(M, device=DEV) != 1]).any())
+    keep = torch.arange(M, device=DEV) != 1
+    check_product(got[keep], ref[keep], torch.float32)
+
+
+@gpu
+@pytest.mark.parametrize("M", [1, 9, 70, 300])
+def test_a_feed_forward(M):
+    """Norm, gate and up with the activation, quantisation, down: each step against its formula on what the step before gave; and the whole once
+    more from a captured graph, on another stream, with new inputs."""
+    H, inter, eps = 320, 4736, 1e-6
+    x, delta = wild_rows(M, H, 1), wild_rows(M, H, 2).to(torch.bfloat16)
+    norm = (1 + 0.1 * torch.randn(H, device=DEV)).to(torch.bfloat16)
+    gate_up = kernels.quantize_int8((torch.randn(2 * inter, H, device=DEV) / H ** 0.5).to(torch.bfloat16))
+    down = kernels.quantize_int8((torch.randn(H, inter, device=DEV) / inter ** 0.5).to(torch.bfloat16))
+
+    def run(stream):
+        rows = kernels.rmsnorm_int8(stream, norm, eps, delta=delta, write_back=True)
+        z = kernels.gemm_int8(rows, gate_up, epilogue="swiglu")
+        mid = kernels.quantize_int8(z)
+        return rows, z, mid, kernels.gemm_int8(mid, down)
+
+    stream = x.clone()
+    rows, z, mid, y = run(stream)
+    total = x + delta.float()
+    assert torch.equal(stream, total)
+    check_rows(rows, total * norm.float(), 1.0 / torch.sqrt(total.double().square().mean(1) + eps), (H / 2 + 4) * 2.0 ** -24)
+    check_gated(z, product_of(rows, gate_up))
+    check_rows(mid, z.float())
+    check_product(y, product_of(mid, down), torch.bfloat16)
+
+    side = torch.cuda.Stream()
+    side.wait_stream(torch.cuda.current_stream())
+    with torch.cuda.stream(side):
+        stream.copy_(x)
+        graph = torch.cuda.CUDAGraph()
+        with torch.cuda.graph(graph, stream=side):
+            held = run(stream)
+        for seed in (5, 6):
+            stream.copy_(wild_rows(M, H, seed))
+            fresh = stream.clone()
+            graph.replay()
+            eager = run(fresh)
+            for p, q in zip(held, eager):
+                for s, t in zip(p if isinstance(p, Int8Rows) else (p,), q if isinstance(q, Int8Rows) else (q,)):
+                    assert torch.equal(s, t)
+            assert torch.equal(stream, fresh)
+    torch.cuda.current_stream().wait_stream(side)
+    assert kernels.status_word(torch.device(DEV)).tolist() == [0, 0]
+
+
+@gpu
+def test_no_rows_and_no_outputs():
+    a, w = kernels.empty_int8(0, 48, DEV), rows_of_codes(20, 48, 1)
+    assert tuple(kernels.gemm_int8(a, w).shape) == (0, 20)
+    assert tuple(kernels.gemm_int8(w, a).shape) == (20, 0)
+    assert tuple(kernels.quantize_int8(torch.empty(0, 48, device=DEV)).codes.shape) == (0, 48)
+    got = kernels.rmsnorm_int8(torch.empty(0, 48, device=DEV), torch.ones(48, device=DEV), 1e-6)
+    assert tuple(got.codes.shape) == (0, 48) and tuple(got.scales.shape) == (0,)
+
+
+@gpu
+def test_refusals():
+    """What the kernels cannot index is refused on the host, with a message that says what is wrong."""
+    a, w = rows_of_codes(4, 48, 1), rows_of_codes(6, 48, 2)
+    x = torch.randn(4, 48, device=DEV)
+    ones = torch.ones(48, device=DEV)
+    odd = torch.zeros(4, 50, dtype=torch.int8, device=DEV)
+    for call, message in (
+            (lambda: kernels.gemm_int8(a, rows_of_codes(6, 32, 2)), "do not fit"),
+            (lambda: kernels.gemm_int8(a.codes, w), "Int8Rows"),
+            (lambda: kernels.gemm_int8(Int8Rows(a.codes.cpu(), a.scales.cpu()), w), "CUDA"),
+            (lambda: kernels.gemm_int8(Int8Rows(a.codes.float(), a.scales), w), "int8"),
+            (lambda: kernels.gemm_int8(Int8Rows(a.codes, a.scales[:3]), w), "one float32 scale"),
+            (lambda: kernels.gemm_int8(Int8Rows(a.codes, a.scales.double()), w), "one float32 scale"),
+            (lambda: kernels.gemm_int8(Int8Rows(a.codes, torch.ones(8, device=DEV)[::2]), w), "one float32 scale"),
+            (lambda: kernels.gemm_int8(Int8Rows(odd, a.scales), rows_of_codes(6, 50, 1)), "16-byte borders"),
+            (lambda: kernels.gemm_int8(Int8Rows(a.codes[:, 1:33], a.scales), rows_of_codes(6, 32, 1)), "16-byte borders"),
+            (lambda: kernels.gemm_int8(Int8Rows(a.codes[:1].expand(4, 48), a.scales), w), "16-byte borders"),
+            (lambda: kernels.gemm_int8(a, w, epilogue="relu"), "unknown epilogue"),
+            (lambda: kernels.gemm_int8(a, rows_of_codes(5, 48, 2), epilogue="swiglu"), "even N"),
+            (lambda: kernels.gemm_int8(a, w, epilogue="swiglu", out_dtype=torch.float32), "bfloat16 output"),
+            (lambda: kernels.gemm_int8(a, w, out=torch.empty(4, 5, device=DEV)), "does not fit"),
+            (lambda: kernels.gemm_int8(a, w, out_dtype=torch.float16), "float32 or bfloat16"),
+            (lambda: kernels.gemm_int8(kernels.empty_int8(1, 131072, DEV), kernels.empty_int8(1, 131072, DEV)), "131071"),
+            (lambda: kernels.gemm_int8(kernels.empty_int8(2, 0, DEV), kernels.empty_int8(2, 0, DEV)), "must lie in"),
+            (lambda: kernels.quantize_int8(x.half()), "float32 or bfloat16"),
+            (lambda: kernels.quantize_int8(x.cpu()), "CUDA"),
+            (lambda: kernels.quantize_int8(x.t()), "rows must be contiguous"),
+            (lambda: kernels.quantize_int8(x[:1].expand(4, 48)), "overlap"),
+            (lambda: kernels.quantize_int8(x, kernels.empty_int8(4, 64, DEV)), "does not fit"),
+            (lambda: kernels.quantize_int8(torch.empty(3, 0, device=DEV)), "must be positive"),
+            (lambda: kernels.rmsnorm_int8(x, ones[:40], 1e-6), "lengths differ"),
+            (lambda: kernels.rmsnorm_int8(x, ones, 1e-6, delta=x[:3]), "differs"),
+            (lambda: kernels.rmsnorm_int8(x, ones, 1e-6, delta=torch.empty(0, 4, 48, device=DEV)), "empty stack"),
+            (lambda: kernels.rmsnorm_int8(x, ones, 1e-6, delta=x, rows=torch.zeros(2, dtype=torch.int32, device=DEV), write_back=True), "row gather"),
+            (lambda: kernels.rmsnorm_int8(x, ones, 1e-6, rows=torch.zeros(2, dtype=torch.int64, device=DEV)), "int32"),
+            (lambda: kernels.rmsnorm_int8(x, ones, 1e-6, out=kernels.empty_int8(3, 48, DEV)), "expected"),
+            (lambda: kernels.rmsnorm_int8(torch.empty(1, 32769, device=DEV), torch.empty(32769, device=DEV), 1e-6), "longer than 32768")):
+        with pytest.raises(KernelError, match=message):
+            call()
+
+
+def test_rows_of_codes_start_on_borders():
+    """On the CPU: the room that is made for codes, and what is refused before a device is needed."""
+    for rows, length in ((1, 1), (3, 16), (4, 17), (0, 5), (5, 4096)):
+        room = kernels.empty_int8(rows, length, "cpu")
+        assert tuple(room.shape) == (rows, length) and room.codes.dtype == torch.int8 and room.scales.dtype == torch.float32
+        assert room.codes.stride(0) % 16 == 0 and tuple(room.scales.shape) == (rows,) and room.device == torch.device("cpu")
+    room = kernels.empty_int8(4, 32, "cpu")
+    with pytest.raises(KernelError, match="CUDA"):
+        kernels.gemm_int8(room, room)
+    with pytest.raises(KernelError, match="Int8Rows"):
+        kernels.gemm_int8((room.codes, room.scales), room)
+    with pytest.raises(KernelError, match="CUDA"):
+        kernels.quantize_int8(torch.zeros(4, 32))
+    with pytest.raises(KernelError, match="CUDA"):
+        kernels.rmsnorm_int8(torch.zeros(4, 32), torch.ones(32), 1e-6)
