@@ -64,32 +64,153 @@ __device__ __forceinline__ void umma_s8_pair(uint32_t tmem_d, uint64_t desc_a, u
 // below -87 gives g / inf = -0, the limit.
 __device__ __forceinline__ float silu_mul(float g, float u) { return __fdividef(g, 1.0f + __expf(-g)) * u; }
 
-__device__ __forceinline__ int4 load_shared_of(uint32_t cluster_addr)
+__device__ __forceinline__ void epilogue_barrier() { asm volatile("bar.sync 1, 128;" ::: "memory"); }   // the four epilogue warps
+__device__ __forceinline__ void cluster_arrive() { asm volatile("barrier.cluster.arrive.release.aligned;" ::: "memory"); }
+__device__ __forceinline__ void cluster_wait() { asm volatile("barrier.cluster.wait.acquire.aligned;" ::: "memory"); }
+__device__ __forceinline__ void store_shared_of(uint32_t cluster_addr, uint32_t a, uint32_t b, uint32_t c, uint32_t d)
 {
-    int4 v;
-    asm volatile("ld.shared::cluster.v4.s32 {%0, %1, %2, %3}, [%4];" : "=r"(v.x), "=r"(v.y), "=r"(v.z), "=r"(v.w) : "r"(cluster_addr) : "memory");
-    return v;
+    asm volatile("st.shared::cluster.v4.u32 [%0], {%1, %2, %3, %4};" ::"r"(cluster_addr), "r"(a), "r"(b), "r"(c), "r"(d) : "memory");
+}
+
+constexpr int TURN_LD = 36;                                  // floats between the tokens of a warp's chunk of 32 tokens x 32 weight rows
+constexpr int TURN_BYTES = 32 * TURN_LD * 4 + 32 * 4;        // and the tokens' scales
+
+// Finishes COLS tokens of 32 weight rows: this lane holds weight row x0 + lane of the tokens from y on.  `turn` is the warp's own place in shared
+// memory, where the numbers are turned so that the results leave in rows of 16 bytes a lane.
+template <int COLS, typename TC, bool GATED>
+__device__ __forceinline__ void store_chunk(TC* __restrict__ out, long long ld, int lane, int x0, int y, int x_end, int y_end, const uint32_t (&r)[COLS], float sw,
+                                            float sa_lane, float* turn)
+{
+    const int count = min(COLS, y_end - y), outs = min(32, x_end - x0);
+    if (outs <= 0 || count <= 0) return;      // the same for the whole warp
+    float* sa = turn + 32 * TURN_LD;
+    sa[lane] = sa_lane;
+    __syncwarp();
+#pragma unroll
+    for (int j = 0; j < COLS; j += 4) {
+        const float4 s = *reinterpret_cast<const float4*>(sa + j);
+        turn[j * TURN_LD + lane] = (float)(int)r[j] * s.x * sw;
+        turn[(j + 1) * TURN_LD + lane] = (float)(int)r[j + 1] * s.y * sw;
+        turn[(j + 2) * TURN_LD + lane] = (float)(int)r[j + 2] * s.z * sw;
+        turn[(j + 3) * TURN_LD + lane] = (float)(int)r[j + 3] * s.w * sw;
+    }
+    __syncwarp();
+    constexpr int PER = GATED ? 16 : 32;      // results of a token
+    TC* dst = out + (size_t)y * ld + (GATED ? x0 / 2 : x0);
+    if (outs == 32 && ld * (long long)sizeof(TC) % 16 == 0 && (reinterpret_cast<uintptr_t>(dst) & 15) == 0) {
+        if constexpr (GATED) {
+            // two lanes a token, eight results each
+            const int part = lane & 1;
+#pragma unroll
+            for (int i = 0; i < COLS / 16; ++i) {
+                const int t = i * 16 + (lane >> 1);
+                uint32_t w[4];
+#pragma unroll
+                for (int e = 0; e < 4; ++e) {
+                    const float4 v = *reinterpret_cast<const float4*>(turn + t * TURN_LD + part * 16 + 4 * e);
+                    w[e] = pack_bf16(silu_mul(v.x, v.y), silu_mul(v.z, v.w));
+                }
+                if (t < count) *reinterpret_cast<uint4*>(dst + (size_t)t * ld + part * 8) = make_uint4(w[0], w[1], w[2], w[3]);
+            }
+        } else if constexpr (sizeof(TC) == 2) {
+            // four lanes a token, eight results each
+            const int part = lane & 3;
+#pragma unroll
+            for (int i = 0; i < COLS / 8; ++i) {
+                const int t = i * 8 + (lane >> 2);
+                const float4 v = *reinterpret_cast<const float4*>(turn + t * TURN_LD + part * 8);
+                const float4 w = *reinterpret_cast<const float4*>(turn + t * TURN_LD + part * 8 + 4);
+                if (t < count)
+                    *reinterpret_cast<uint4*>(dst + (size_t)t * ld + part * 8) =
+                        make_uint4(pack_bf16(v.x, v.y), pack_bf16(v.z, v.w), pack_bf16(w.x, w.y), pack_bf16(w.z, w.w));
+            }
+        } else {
+            const int part = lane & 7;
+#pragma unroll
+            for (int i = 0; i < COLS / 4; ++i) {
+                const int t = i * 4 + (lane >> 3);
+                if (t < count) *reinterpret_cast<float4*>(dst + (size_t)t * ld + part * 4) = *reinterpret_cast<const float4*>(turn + t * TURN_LD + part * 4);
+            }
+        }
+    } else {
+        const int results = GATED ? outs / 2 : outs;
+        for (int i = lane; i < count * PER; i += 32) {
+            const int t = i / PER, c = i % PER;
+            if (c < results) {
+                if constexpr (GATED) dst[(size_t)t * ld + c] = from_f32<TC>(silu_mul(turn[t * TURN_LD + 2 * c], turn[t * TURN_LD + 2 * c + 1]));
+                else dst[(size_t)t * ld + c] = from_f32<TC>(turn[t * TURN_LD + c]);
+            }
+        }
+    }
+    __syncwarp();   // the next chunk's numbers may come
 }
 
 // ---- few tokens ------------------------------------------------------------------------------------------------------------------
 // Two blocks share an SM, each with AREA bytes of stages.  A tile of fewer than 128 weight rows takes only its own bytes (rounded up to the
 // swizzle's 1 KB); the tensor core still reads 128 rows: the spare ones come from whatever lies behind (the area ends with room for that) and feed
-// accumulator rows that are never stored.  When the sums are complete the ring is free and holds the integer tile, [token][TILE_LD].
-constexpr int TILE_LD = BM + 4;
+// accumulator rows that are never stored.
+// What follows the last load is as short as it can be (at first it took 3 us of 8): the scales are fetched while the tiles stream in; with K whole, each
+// warp turns its rows in the ring, which is free by then, and stores them.  With K cut, block r of the cluster finishes the r-th part of the weight
+// rows: every block writes its integer sums of these rows straight into block r's shared memory (`mail`, [source][group of four tokens][row]), one cluster barrier, and
+// block r adds them up.  Up to 32 tokens the mail has a place of its own; beyond, it takes the ring's, and the blocks first tell one another that theirs is free.
 template <int BN> struct Tile {
     static constexpr int Y_BYTES = BN * BK;
     static constexpr int TMEM_COLS = BN < 32 ? 32 : BN;
-    static constexpr int AREA = 110 * 1024;
+    static constexpr int MAIL = BN * BM * 4;
+    static constexpr bool MAIL_IN_RING = BN > 32;
+    static constexpr int AREA = 110 * 1024 - (MAIL_IN_RING ? 0 : MAIL);
     static constexpr int MAX_STAGES = 12;
-    static constexpr size_t SMEM = (size_t)AREA + 1024 /* alignment slack */ + 256 /* barriers */;
+    static constexpr size_t SMEM = 110 * 1024 + 1024 /* alignment slack */ + 256 /* barriers */ + BN * 4 /* the tokens' scales */;
     __host__ __device__ static constexpr int x_bytes(int tile_rows) { return (tile_rows * BK + 1023) & ~1023; }
     __host__ __device__ static constexpr int stages(int tile_rows)
     {
         const int n = (AREA - (BM * BK - x_bytes(tile_rows))) / (x_bytes(tile_rows) + Y_BYTES);
         return n < MAX_STAGES ? n : MAX_STAGES;
     }
-    static_assert(BN * TILE_LD * 4 <= AREA, "the integer tile fits the ring");
+    static_assert(MAIL <= AREA && 4 * TURN_BYTES <= AREA, "what follows the main loop fits the ring");
 };
+
+// The end of a tile whose K is cut: this thread adds up weight row x of every SPLITS-th group of four tokens.  Gated: lanes 2i and 2i + 1 hold gate and
+// up; of four tokens the even lane finishes the first two and the odd lane the others.
+template <int SPLITS, int BN, typename TC, bool GATED>
+__device__ __forceinline__ void finish_cut(TC* __restrict__ out, long long ld, const int4* mail, const float* sa, float sw, int x, int x_end, int y0, int tokens,
+                                           int tid, int lane)
+{
+    constexpr int SHARE = BM / SPLITS;
+    const int4* got = mail + tid % SHARE;
+    const bool inside = x < x_end, odd = (lane & 1) != 0;
+    TC* dst = out + (size_t)y0 * ld + (GATED ? x / 2 : x);
+#pragma unroll 2
+    for (int q0 = 0; q0 < BN / 4; q0 += SPLITS) {
+        const int q = q0 + tid / SHARE;
+        if (4 * q0 >= tokens) break;                  // the same for the whole block
+        int4 sum = make_int4(0, 0, 0, 0);
+        float4 s4 = make_float4(0.f, 0.f, 0.f, 0.f);
+        if (4 * q < tokens) {
+            s4 = *reinterpret_cast<const float4*>(sa + 4 * q);
+#pragma unroll
+            for (int s = 0; s < SPLITS; ++s) {
+                const int4 v = got[(s * (BN / 4) + q) * SHARE];
+                sum.x += v.x;
+                sum.y += v.y;
+                sum.z += v.z;
+                sum.w += v.w;
+            }
+        }
+        const float v[4] = {(float)sum.x * s4.x * sw, (float)sum.y * s4.y * sw, (float)sum.z * s4.z * sw, (float)sum.w * s4.w * sw};
+        if constexpr (GATED) {
+            const float p = __shfl_xor_sync(0xffffffffu, odd ? v[0] : v[2], 1), r = __shfl_xor_sync(0xffffffffu, odd ? v[1] : v[3], 1);
+            const float first = odd ? silu_mul(p, v[2]) : silu_mul(v[0], p), second = odd ? silu_mul(r, v[3]) : silu_mul(v[1], r);
+            const int t = 4 * q + (odd ? 2 : 0);
+            if (inside && t < tokens) dst[(size_t)t * ld] = from_f32<TC>(first);
+            if (inside && t + 1 < tokens) dst[(size_t)(t + 1) * ld] = from_f32<TC>(second);
+        } else {
+#pragma unroll
+            for (int e = 0; e < 4; ++e)
+                if (inside && 4 * q + e < tokens) dst[(size_t)(4 * q + e) * ld] = from_f32<TC>(v[e]);
+        }
+    }
+}
 
 // Block (token tile, K range) = (blockIdx.x / splits, blockIdx.x % splits) of weight tile blockIdx.y; the K ranges of a tile are a cluster.
 template <int BN, typename TC, bool GATED>
@@ -100,11 +221,13 @@ gemm_int8_few_kernel(const __grid_constant__ CUtensorMap map_w, const __grid_con
     using T = Tile<BN>;
     extern __shared__ uint8_t smem_raw[];
     uint8_t* tiles = reinterpret_cast<uint8_t*>((reinterpret_cast<uintptr_t>(smem_raw) + 1023) & ~(uintptr_t)1023);
-    uint64_t* full_bar = reinterpret_cast<uint64_t*>(tiles + T::AREA);
+    int4* mail = reinterpret_cast<int4*>(T::MAIL_IN_RING ? tiles : tiles + T::AREA);
+    uint64_t* full_bar = reinterpret_cast<uint64_t*>(tiles + 110 * 1024);
     uint64_t* empty_bar = full_bar + T::MAX_STAGES;
     uint64_t* accum_bar = empty_bar + T::MAX_STAGES;
     uint32_t* tmem_slot = reinterpret_cast<uint32_t*>(accum_bar + 1);
     volatile int* abort_flag = reinterpret_cast<volatile int*>(tmem_slot + 1);
+    float* sa = reinterpret_cast<float*>(tiles + 110 * 1024 + 256);
 
     const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
     const int rank = blockIdx.x % splits;                       // the block's place in its cluster
@@ -130,6 +253,8 @@ gemm_int8_few_kernel(const __grid_constant__ CUtensorMap map_w, const __grid_con
     const uint32_t tmem_base = *tmem_slot;
 
     pdl_launch_dependents();
+    // the cluster's first barrier: a block's mail may be written.  All but the warps that free the ring arrive here.
+    if (splits > 1 && (!T::MAIL_IN_RING || warp < 2)) cluster_arrive();
     if (warp == 0) {
         if (lane == 0) {
             // the weights depend on no earlier kernel: their tiles for the first stages are requested before the wait for the kernels ahead in the stream
@@ -182,77 +307,58 @@ gemm_int8_few_kernel(const __grid_constant__ CUtensorMap map_w, const __grid_con
             umma_commit(accum_bar);           // the accumulator is complete when every MMA has finished
         }
     } else {
-        // warp w reads tensor-memory lanes 32 (w % 4) .. + 31, i.e. weight rows of the tile; the tile goes to the ring, which every MMA has read
-        const int row = (warp & 3) * 32 + lane;
+        // warp w reads tensor-memory lanes 32 (w % 4) .. + 31, i.e. weight rows of the tile
+        const int quarter = warp & 3, row = quarter * 32 + lane, tid = threadIdx.x - 64;
+        const int tokens = min(BN, M - y0), x_end = min(N, x0 + tile_rows);
+        const int share = BM / splits, part = rank * share + (tid & (share - 1));        // K cut: the weight row that this thread finishes
+        const int x = x0 + (splits > 1 ? part : row);
+        const float sw = x < x_end ? w_scale[x] : 0.f;
+        pdl_wait();                           // the tokens' scales and the output belong to kernels ahead in the stream until here
+        if (tid < BN) sa[tid] = tid < tokens ? a_scale[y0 + tid] : 0.f;
+        epilogue_barrier();
         const bool ok = mbar_wait(accum_bar, 0, abort_flag);
         fence_after_sync();
-        if (ok) {
-            int* staged = reinterpret_cast<int*>(tiles);
-            constexpr int COLS = BN < 32 ? BN : 32;
+        const uint32_t acc = tmem_base + ((uint32_t)(quarter * 32) << 16);
+        constexpr int COLS = BN < 32 ? BN : 32;
+        if (splits == 1) {
+            float* turn = reinterpret_cast<float*>(tiles + quarter * TURN_BYTES);
 #pragma unroll 1
-            for (int c = 0; c < BN; c += COLS) {
+            for (int c = 0; c < tokens && ok; c += COLS) {
                 uint32_t r[COLS];
-                tmem_load<COLS>(tmem_base + ((uint32_t)((warp & 3) * 32) << 16) + (uint32_t)c, r);
+                tmem_load<COLS>(acc + (uint32_t)c, r);
+                tmem_wait_ld();
+                store_chunk<COLS, TC, GATED>(out, ld, lane, x0 + quarter * 32, y0 + c, x_end, M, r, sw, lane < COLS ? sa[c + lane] : 0.f, turn);
+            }
+        } else {
+            __syncwarp();
+            if constexpr (T::MAIL_IN_RING) cluster_arrive();
+            cluster_wait();
+            const uint32_t to = map_to_rank(smem_u32(mail + (size_t)rank * (BN / 4) * share + (row & (share - 1))), row / share);
+#pragma unroll 1
+            for (int c = 0; c < tokens && ok; c += COLS) {
+                uint32_t r[COLS];
+                tmem_load<COLS>(acc + (uint32_t)c, r);
                 tmem_wait_ld();
 #pragma unroll
-                for (int j = 0; j < COLS; ++j) staged[(c + j) * TILE_LD + row] = (int)r[j];
+                for (int j = 0; j < COLS; j += 4)
+                    if (c + j < tokens) store_shared_of(to + (uint32_t)((c + j) / 4 * share) * 16, r[j], r[j + 1], r[j + 2], r[j + 3]);
+            }
+            __syncwarp();
+            cluster_arrive();
+            cluster_wait();
+            if (ok) {
+                if (splits == 2) finish_cut<2, BN, TC, GATED>(out, ld, mail, sa, sw, x0 + part, x_end, y0, tokens, tid, lane);
+                else if (splits == 4) finish_cut<4, BN, TC, GATED>(out, ld, mail, sa, sw, x0 + part, x_end, y0, tokens, tid, lane);
+                else finish_cut<8, BN, TC, GATED>(out, ld, mail, sa, sw, x0 + part, x_end, y0, tokens, tid, lane);
             }
         }
     }
     fence_before_sync();
-    __syncthreads();
-    if (splits > 1) cluster_sync();           // every block's part of the sums lies in its shared memory
-    pdl_wait();                               // the scales and the output belong to kernels ahead in the stream until here
-
-    // the cluster's blocks finish the tile together, four outputs of one token at a time, each a part of them
-    {
-        const int tokens = min(BN, M - y0), outs = min(tile_rows, N - x0), quads = (outs + 3) >> 2;
-        const int total = tokens * quads, first = (int)((long long)rank * total / splits), end = (int)((long long)(rank + 1) * total / splits);
-        const uint32_t own = smem_u32(tiles);
-        constexpr int WIDTH = GATED ? 2 : 4;  // results of a quad
-        TC* base = out + (size_t)y0 * ld + (GATED ? x0 / 2 : x0);
-        const bool whole_rows = ld % WIDTH == 0 && (reinterpret_cast<uintptr_t>(base) & (WIDTH * sizeof(TC) - 1)) == 0;
-#pragma unroll 1
-        for (int i = first + (int)threadIdx.x; i < end; i += NUM_THREADS) {
-            const int t = i / quads, q = i - t * quads, left = outs - 4 * q;
-            const uint32_t at = own + (uint32_t)(t * TILE_LD + 4 * q) * 4;
-            int4 sum = make_int4(0, 0, 0, 0);
-            if (splits == 1) {
-                sum = *reinterpret_cast<const int4*>(tiles + (size_t)(t * TILE_LD + 4 * q) * 4);
-            } else {
-#pragma unroll 2
-                for (int r = 0; r < splits; ++r) {
-                    const int4 v = load_shared_of(map_to_rank(at, r));
-                    sum.x += v.x;
-                    sum.y += v.y;
-                    sum.z += v.z;
-                    sum.w += v.w;
-                }
-            }
-            const float sa = a_scale[y0 + t];
-            const float* sw = w_scale + x0 + 4 * q;
-            float v[4] = {(float)sum.x * sa, (float)sum.y * sa, (float)sum.z * sa, (float)sum.w * sa};
-#pragma unroll
-            for (int e = 0; e < 4; ++e) v[e] = e < left ? v[e] * sw[e] : 0.f;
-            TC* dst = base + (size_t)t * ld + WIDTH * q;
-            if constexpr (GATED) {
-                v[0] = silu_mul(v[0], v[1]);
-                v[1] = silu_mul(v[2], v[3]);
-            }
-            if (left >= 4 && whole_rows) {
-                if constexpr (sizeof(TC) == 4) {
-                    *reinterpret_cast<float4*>(dst) = make_float4(v[0], v[1], v[2], v[3]);
-                } else if constexpr (GATED) {
-                    *reinterpret_cast<uint32_t*>(dst) = pack_bf16(v[0], v[1]);
-                } else {
-                    *reinterpret_cast<uint2*>(dst) = make_uint2(pack_bf16(v[0], v[1]), pack_bf16(v[2], v[3]));
-                }
-            } else {
-#pragma unroll
-                for (int e = 0; e < WIDTH; ++e)
-                    if (e < (GATED ? left / 2 : left)) dst[e] = from_f32<TC>(v[e]);
-            }
-        }
+    if (splits > 1 && warp < 2) {
+        __syncwarp();
+        cluster_wait();
+        cluster_arrive();
+        cluster_wait();
     }
 
     __syncthreads();
@@ -265,7 +371,6 @@ gemm_int8_few_kernel(const __grid_constant__ CUtensorMap map_w, const __grid_con
         }
         __syncthreads();
     }
-    if (splits > 1) cluster_sync();           // no block leaves while another may still read its shared memory
     if (warp == 1) {
         fence_after_sync();
         tmem_dealloc(tmem_base, T::TMEM_COLS);
@@ -300,84 +405,12 @@ constexpr int PAIR_BN = 256;                                 // tensor-memory co
 constexpr int PAIR_MAX_STAGES = 10;
 constexpr int PAIR_X_BYTES = BM * BK;
 constexpr int PAIR_AREA = 6 * 2 * PAIR_X_BYTES;              // the ring: six stages at 256 tokens a tile, more at fewer
-constexpr int TURN_LD = 36;                                  // floats between the tokens of a warp's chunk of 32 tokens x 32 weight rows
-constexpr int TURN_BYTES = 32 * TURN_LD * 4 + 32 * 4;        // and the tokens' scales
 constexpr size_t PAIR_SMEM = (size_t)PAIR_AREA + 4 * TURN_BYTES + 1024 /* alignment slack */ + 256 /* barriers */;
 __host__ __device__ constexpr int pair_stage_bytes(int token_rows) { return PAIR_X_BYTES + token_rows / 2 * BK; }
 __host__ __device__ constexpr int pair_stages(int token_rows)
 {
     const int n = PAIR_AREA / pair_stage_bytes(token_rows);
     return n < PAIR_MAX_STAGES ? n : PAIR_MAX_STAGES;
-}
-
-// Finishes one chunk: this lane holds weight row x0 + lane of the 32 tokens from y on.  `turn` is the warp's own place in shared memory, where the
-// chunk is turned so that the results leave in rows.
-template <typename TC, bool GATED>
-__device__ __forceinline__ void store_chunk(TC* __restrict__ out, long long ld, int lane, int x0, int y, int N, int y_end, const uint32_t (&r)[32], float sw,
-                                            const float* __restrict__ a_scale, float* turn)
-{
-    const int count = min(32, y_end - y), outs = min(32, N - x0);
-    if (outs <= 0 || count <= 0) return;      // the same for the whole warp
-    float* sa = turn + 32 * TURN_LD;
-    sa[lane] = lane < count ? a_scale[y + lane] : 0.f;
-    __syncwarp();
-#pragma unroll
-    for (int j = 0; j < 32; j += 4) {
-        const float4 s = *reinterpret_cast<const float4*>(sa + j);
-        turn[j * TURN_LD + lane] = (float)(int)r[j] * s.x * sw;
-        turn[(j + 1) * TURN_LD + lane] = (float)(int)r[j + 1] * s.y * sw;
-        turn[(j + 2) * TURN_LD + lane] = (float)(int)r[j + 2] * s.z * sw;
-        turn[(j + 3) * TURN_LD + lane] = (float)(int)r[j + 3] * s.w * sw;
-    }
-    __syncwarp();
-    constexpr int PER = GATED ? 16 : 32;      // results of a token
-    TC* dst = out + (size_t)y * ld + (GATED ? x0 / 2 : x0);
-    if (outs == 32 && ld * (long long)sizeof(TC) % 16 == 0 && (reinterpret_cast<uintptr_t>(dst) & 15) == 0) {
-        if constexpr (GATED) {
-            // two lanes a token, eight results each
-            const int part = lane & 1;
-#pragma unroll
-            for (int i = 0; i < 2; ++i) {
-                const int t = i * 16 + (lane >> 1);
-                uint32_t w[4];
-#pragma unroll
-                for (int e = 0; e < 4; ++e) {
-                    const float4 v = *reinterpret_cast<const float4*>(turn + t * TURN_LD + part * 16 + 4 * e);
-                    w[e] = pack_bf16(silu_mul(v.x, v.y), silu_mul(v.z, v.w));
-                }
-                if (t < count) *reinterpret_cast<uint4*>(dst + (size_t)t * ld + part * 8) = make_uint4(w[0], w[1], w[2], w[3]);
-            }
-        } else if constexpr (sizeof(TC) == 2) {
-            // four lanes a token, eight results each
-            const int part = lane & 3;
-#pragma unroll
-            for (int i = 0; i < 4; ++i) {
-                const int t = i * 8 + (lane >> 2);
-                const float4 v = *reinterpret_cast<const float4*>(turn + t * TURN_LD + part * 8);
-                const float4 w = *reinterpret_cast<const float4*>(turn + t * TURN_LD + part * 8 + 4);
-                if (t < count)
-                    *reinterpret_cast<uint4*>(dst + (size_t)t * ld + part * 8) =
-                        make_uint4(pack_bf16(v.x, v.y), pack_bf16(v.z, v.w), pack_bf16(w.x, w.y), pack_bf16(w.z, w.w));
-            }
-        } else {
-            const int part = lane & 7;
-#pragma unroll
-            for (int i = 0; i < 8; ++i) {
-                const int t = i * 4 + (lane >> 3);
-                if (t < count) *reinterpret_cast<float4*>(dst + (size_t)t * ld + part * 4) = *reinterpret_cast<const float4*>(turn + t * TURN_LD + part * 4);
-            }
-        }
-    } else {
-        const int results = GATED ? outs / 2 : outs;
-        for (int i = lane; i < count * PER; i += 32) {
-            const int t = i / PER, c = i % PER;
-            if (c < results) {
-                if constexpr (GATED) dst[(size_t)t * ld + c] = from_f32<TC>(silu_mul(turn[t * TURN_LD + 2 * c], turn[t * TURN_LD + 2 * c + 1]));
-                else dst[(size_t)t * ld + c] = from_f32<TC>(turn[t * TURN_LD + c]);
-            }
-        }
-    }
-    __syncwarp();   // the next chunk's numbers may come
 }
 
 template <typename TC, bool GATED>
@@ -509,7 +542,7 @@ gemm_int8_pair_kernel(const __grid_constant__ CUtensorMap map_w, const __grid_co
                 uint32_t r[32];
                 tmem_load<32>(tmem_base + ((uint32_t)(quarter * 32) << 16) + (uint32_t)(buf * PAIR_BN + c), r);
                 tmem_wait_ld();
-                store_chunk<TC, GATED>(out, ld, lane, x0, y0 + c, N, y_end, r, sw, a_scale, turn);
+                store_chunk<32, TC, GATED>(out, ld, lane, x0, y0 + c, N, y_end, r, sw, y0 + c + lane < y_end ? a_scale[y0 + c + lane] : 0.f, turn);
             }
             fence_before_sync();
             if (rank == 0) mbar_arrive(acc_empty + buf);

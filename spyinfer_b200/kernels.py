@@ -2100,30 +2100,66 @@ def empty_int8(rows: int, length: int, device) -> Int8Rows:
     return Int8Rows(codes if pitch == length else codes[:, :length], torch.empty((rows,), dtype=torch.float32, device=device))
 
 
-def _on_current_device(t: torch.Tensor, what: str) -> None:
-    if t.device.index != torch.cuda.current_device():
-        raise KernelError(f"{what}: lies on {t.device}, the current device is cuda:{torch.cuda.current_device()}")
+class _Kernel:
+    """A C entry with its argument types declared once, for calls that are short beside what wrapping every argument takes: numbers and addresses go in as
+    they are.  Counted and timed as ``_call`` does it."""
+
+    def __init__(self, module: str, fn: str, *types):
+        self.module, self.fn, self.types, self.entry = module, fn, types, None
+
+    def __call__(self, *args) -> None:
+        global _launches
+        if self.entry is None:
+            entry = getattr(build.load(self.module), self.fn)
+            entry.restype, entry.argtypes = ctypes.c_int, self.types
+            self.entry = entry
+        if _timed_calls is not None:
+            return _call(self.module, self.fn, *args)
+        _launches += 1
+        if self.entry(*args) != 0:
+            raise KernelError(build.last_error(self.module))
 
 
-def _check_int8(m: Int8Rows, what: str) -> int:
-    """Returns the distance between the rows of codes in bytes."""
+_P, _L, _I, _F = ctypes.c_void_p, ctypes.c_longlong, ctypes.c_int, ctypes.c_float
+_quantize_int8 = _Kernel("quant_int8", "spy_quantize_int8", _P, _I, _L, _P, _L, _P, _I, _I, _P)
+_rmsnorm_int8 = _Kernel("quant_int8", "spy_rmsnorm_int8", _P, _I, _P, _I, _I, _L, _P, _P, _I, _P, _L, _P, _I, _I, _F, _I, _P)
+_gemm_int8 = _Kernel("gemm_int8", "spy_gemm_int8", _P, _L, _P, _P, _L, _P, _P, _I, _L, _I, _I, _I, _I, _P, _P)
+
+
+def _on_current_device(t: torch.Tensor, what: str) -> int:
+    """The current device's index, which has to be the tensor's."""
+    device = torch.cuda.current_device()
+    if t.get_device() != device:
+        raise KernelError(f"{what}: lies on {t.device}, the current device is cuda:{device}")
+    return device
+
+
+def _int8_layout(m: Int8Rows, what: str, device: Optional[int] = None):
+    """(rows, length, bytes between rows, address of the codes, address of the scales) of a matrix that the kernels can index."""
     if not isinstance(m, Int8Rows):
         raise KernelError(f"{what}: expected Int8Rows (codes and scales), found {type(m).__name__}")
     codes, scales = m
-    if not isinstance(codes, torch.Tensor) or not codes.is_cuda or codes.dtype != torch.int8 or codes.dim() != 2:
+    if not isinstance(codes, torch.Tensor) or codes.dtype is not torch.int8 or codes.dim() != 2 or not codes.is_cuda:
         raise KernelError(f"{what}: expected a CUDA matrix of int8 codes")
-    if not isinstance(scales, torch.Tensor) or scales.dtype != torch.float32 or scales.dim() != 1 or scales.shape[0] != codes.shape[0] \
-            or scales.device != codes.device or not scales.is_contiguous():
-        raise KernelError(f"{what}: expected one float32 scale a row, contiguous and on the codes' device")
-    _on_current_device(codes, what)
     rows, length = codes.shape
-    pitch = codes.stride(0)
+    at = codes.get_device()
+    if not isinstance(scales, torch.Tensor) or scales.dtype is not torch.float32 or scales.shape != (rows,) or scales.get_device() != at \
+            or not scales.is_contiguous():
+        raise KernelError(f"{what}: expected one float32 scale a row, contiguous and on the codes' device")
+    if at != device:
+        _on_current_device(codes, what)
+    pitch, step = codes.stride()
     if rows <= 1 or length == 0:
         pitch = (length + 15) // 16 * 16
-    if (length > 1 and codes.stride(1) != 1) or pitch < length or pitch % 16 != 0 or codes.data_ptr() % 16 != 0:
+    address = codes.data_ptr()
+    if (step != 1 and length > 1) or pitch < length or pitch & 15 or address & 15:
         raise KernelError(f"{what}: rows of codes must be contiguous and start on 16-byte borders, found strides {codes.stride()} at address "
-                          f"{codes.data_ptr():#x} (empty_int8 makes such rows)")
-    return pitch
+                          f"{address:#x} (empty_int8 makes such rows)")
+    return rows, length, pitch, address, scales.data_ptr()
+
+
+def _raw_stream(device: int) -> int:
+    return torch._C._cuda_getCurrentRawStream(device)
 
 
 def quantize_int8(x: torch.Tensor, out: Optional[Int8Rows] = None) -> Int8Rows:
@@ -2132,16 +2168,16 @@ def quantize_int8(x: torch.Tensor, out: Optional[Int8Rows] = None) -> Int8Rows:
     or an infinity has codes 0 and the scale NaN."""
     code = _code(x, "quantize_int8 input")
     ldx = _check_weight(x, "quantize_int8 input")
-    _on_current_device(x, "quantize_int8 input")
+    device = _on_current_device(x, "quantize_int8 input")
     n, length = x.shape
-    if out is None:
-        out = empty_int8(n, length, x.device)
-    pitch = _check_int8(out, "quantize_int8 output")
-    if tuple(out.codes.shape) != (n, length) or out.device != x.device:
-        raise KernelError(f"quantize_int8 output: {tuple(out.codes.shape)} on {out.device} does not fit the input {tuple(x.shape)} on {x.device}")
     if n > 1 and ldx < length:
         raise KernelError(f"quantize_int8 input: rows overlap (strides {x.stride()} for shape {tuple(x.shape)})")
-    _call("quant_int8", "spy_quantize_int8", _ptr(x), code, ctypes.c_longlong(ldx), _ptr(out.codes), ctypes.c_longlong(pitch), _ptr(out.scales), n, length, _stream())
+    if out is None:
+        out = empty_int8(n, length, x.device)
+    rows, width, pitch, codes, scales = _int8_layout(out, "quantize_int8 output", device)
+    if (rows, width) != (n, length):
+        raise KernelError(f"quantize_int8 output: {(rows, width)} does not fit the input {(n, length)}")
+    _quantize_int8(x.data_ptr(), code, ldx, codes, pitch, scales, n, length, _raw_stream(device))
     return out
 
 
@@ -2152,31 +2188,30 @@ def rmsnorm_int8(x: torch.Tensor, weight: torch.Tensor, eps: float, out: Optiona
     + eps)``.  ``delta``: x's shape, or a stack ``[splits, rows, len]`` of partial sums that are added in order; ``write_back`` stores the sum into ``x``; ``rows``
     gathers rows of x (and delta).  Rows of up to 32,768 elements."""
     _check(x, "rmsnorm_int8 input", ndim=2)
-    _on_current_device(x, "rmsnorm_int8 input")
+    device = _on_current_device(x, "rmsnorm_int8 input")
     _check(weight, "rmsnorm_int8 weight", ndim=1)
-    H = x.shape[1]
+    n, H = x.shape
     if weight.shape[0] != H:
         raise KernelError(f"rmsnorm_int8: row lengths differ: input {H}, weight {weight.shape[0]}")
-    d, splits, split_stride = _stack_of(delta, x, "rmsnorm_int8 delta")
-    if d is not None and splits == 0:
+    delta, splits, split_stride = _stack_of(delta, x, "rmsnorm_int8 delta")
+    if delta is not None and splits == 0:
         raise KernelError("rmsnorm_int8 delta: an empty stack")
-    n = x.shape[0]
     if rows is not None:
         _check(rows, "rmsnorm_int8 rows", torch.int32, 1)
         n = rows.shape[0]
         if write_back:
             raise KernelError("rmsnorm_int8: write_back with a row gather is not defined")
-    for t, what in ((weight, "weight"), (d, "delta"), (rows, "rows")):
-        if t is not None and t.device != x.device:
+    for t, what in ((weight, "weight"), (delta, "delta"), (rows, "rows")):
+        if t is not None and t.get_device() != device:
             raise KernelError(f"rmsnorm_int8 {what}: lies on {t.device}, the input on {x.device}")
     if out is None:
         out = empty_int8(n, H, x.device)
-    pitch = _check_int8(out, "rmsnorm_int8 output")
-    if tuple(out.codes.shape) != (n, H) or out.device != x.device:
-        raise KernelError(f"rmsnorm_int8 output: expected {(n, H)} on {x.device}, found {tuple(out.codes.shape)} on {out.device}")
-    _call("quant_int8", "spy_rmsnorm_int8", _ptr(x), _code(x, "rmsnorm_int8 input"), _ptr(d), _code(d, "rmsnorm_int8 delta") if d is not None else 0, splits,
-          ctypes.c_longlong(split_stride), _ptr(rows), _ptr(weight), _code(weight, "rmsnorm_int8 weight"), _ptr(out.codes), ctypes.c_longlong(pitch),
-          _ptr(out.scales), n, H, ctypes.c_float(eps), int(bool(write_back)), _stream())
+    got, width, pitch, codes, scales = _int8_layout(out, "rmsnorm_int8 output", device)
+    if (got, width) != (n, H):
+        raise KernelError(f"rmsnorm_int8 output: expected {(n, H)}, found {(got, width)}")
+    _rmsnorm_int8(x.data_ptr(), _code(x, "rmsnorm_int8 input"), delta.data_ptr() if delta is not None else 0,
+                  _code(delta, "rmsnorm_int8 delta") if delta is not None else 0, splits, split_stride, rows.data_ptr() if rows is not None else 0,
+                  weight.data_ptr(), _code(weight, "rmsnorm_int8 weight"), codes, pitch, scales, n, H, eps, 1 if write_back else 0, _raw_stream(device))
     return out
 
 
@@ -2185,25 +2220,30 @@ def gemm_int8(a: Int8Rows, w: Int8Rows, out: Optional[torch.Tensor] = None, stat
     """``a [M, K] @ w [N, K]^T`` of 8-bit rows on the tensor cores, ``(sum_k a w) * a.scales[m] * w.scales[n]`` with the sum in 32-bit integers (exact; K below
     131,072), in bfloat16 (default) or float32.  ``epilogue="swiglu"``: ``w``'s rows alternate gate and up rows and the result is ``silu(gate) * up``,
     ``[M, N / 2]`` bfloat16.  A row whose scale is NaN gives a row of NaN.  A token's result does not depend on the rest of the batch."""
-    lda, ldw = _check_int8(a, "gemm_int8 input"), _check_int8(w, "gemm_int8 weight")
-    M, K = a.codes.shape
-    N = w.codes.shape[0]
-    if w.codes.shape[1] != K:
-        raise KernelError(f"gemm_int8: shapes do not fit: input {tuple(a.codes.shape)}, weight {tuple(w.codes.shape)}")
-    if epilogue not in (None, "swiglu"):
+    M, K, lda, a_codes, a_scales = _int8_layout(a, "gemm_int8 input")
+    device = a.codes.get_device()
+    N, k_of_w, ldw, w_codes, w_scales = _int8_layout(w, "gemm_int8 weight", device)
+    if k_of_w != K:
+        raise KernelError(f"gemm_int8: shapes do not fit: input {(M, K)}, weight {(N, k_of_w)}")
+    if epilogue is not None and epilogue != "swiglu":
         raise KernelError(f"gemm_int8: unknown epilogue {epilogue!r}")
     n_out = N // 2 if epilogue else N
     if out is None:
         out = torch.empty((M, n_out), dtype=out_dtype or torch.bfloat16, device=a.codes.device)
     else:
         _check(out, "gemm_int8 output", out_dtype, 2)
-        if tuple(out.shape) != (M, n_out) or out.device != a.codes.device:
-            raise KernelError(f"gemm_int8: output {tuple(out.shape)} on {out.device} does not fit [{M}, {n_out}] on {a.codes.device}")
+        if out.shape != (M, n_out) or out.get_device() != device:
+            raise KernelError(f"gemm_int8: output {tuple(out.shape)} on {out.device} does not fit [{M}, {n_out}] on cuda:{device}")
     if status is None:
-        if str(a.codes.device) not in _status_words and torch.cuda.is_current_stream_capturing():
-            raise KernelError("gemm_int8: the device's status word does not exist yet and must not come from a graph's memory: make one call (or "
-                              "status_word()) before the capture, or give a status")
-        status = status_word(a.codes.device)
-    _call("gemm_int8", "spy_gemm_int8", _ptr(a.codes), ctypes.c_longlong(lda), _ptr(a.scales), _ptr(w.codes), ctypes.c_longlong(ldw), _ptr(w.scales), _ptr(out),
-          _code(out, "gemm_int8 output"), ctypes.c_longlong(n_out), M, N, K, int(epilogue is not None), _ptr(status), _stream())
+        status = _int8_status.get(device)
+        if status is None:
+            # the word must not come from a captured graph's memory
+            if torch.cuda.is_current_stream_capturing() and str(a.codes.device) not in _status_words:
+                raise KernelError("gemm_int8: the device's status word does not exist yet: make one call (or status_word()) before the capture, or give a status")
+            status = _int8_status[device] = status_word(a.codes.device)
+    _gemm_int8(a_codes, lda, a_scales, w_codes, ldw, w_scales, out.data_ptr(), _code(out, "gemm_int8 output"), n_out, M, N, K, 1 if epilogue else 0,
+               status.data_ptr(), _raw_stream(device))
     return out
+
+
+_int8_status = {}        # device index -> its status word
