@@ -29,6 +29,7 @@ class EngineConfig:
     device: str = "cuda:0"
     use_cuda_graphs: bool = True
     graph_step_tokens: int = 384      # steps of other shapes than decode steps are replayed from CUDA graphs up to this many tokens (0: never)
+    quantization: Optional[str] = None   # "int8": the layers' products in 8-bit integers (weights and activations), bfloat16 elsewhere
     lookahead_decode: bool = True     # launch the next decode step before the last one's tokens are read (see LLMEngine.step)
 
     def __post_init__(self):
@@ -45,6 +46,10 @@ class EngineConfig:
             raise ValueError(f"num_kvcache_blocks must be positive, found {self.num_kvcache_blocks!r}")
         if not isinstance(self.graph_step_tokens, int) or self.graph_step_tokens < 0:
             raise ValueError(f"graph_step_tokens must be a non-negative integer, found {self.graph_step_tokens!r}")
+        if self.quantization not in (None, "int8"):
+            raise ValueError(f"quantization {self.quantization!r}: choose \"int8\" or None")
+        if self.quantization is not None and self.dtype != "bfloat16":
+            raise ValueError(f"quantization {self.quantization!r} goes with dtype bfloat16, found {self.dtype}")
         if not 0.0 < self.gpu_memory_utilization <= 1.0:
             raise ValueError("gpu_memory_utilization must lie in (0, 1]")
 

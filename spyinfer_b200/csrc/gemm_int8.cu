@@ -216,7 +216,8 @@ __device__ __forceinline__ void finish_cut(TC* __restrict__ out, long long ld, c
 template <int BN, typename TC, bool GATED>
 __global__ void __launch_bounds__(NUM_THREADS, 2)
 gemm_int8_few_kernel(const __grid_constant__ CUtensorMap map_w, const __grid_constant__ CUtensorMap map_a, const float* __restrict__ w_scale,
-                     const float* __restrict__ a_scale, TC* __restrict__ out, long long ld, int N, int M, int k_blocks, int splits, int tile_rows, int* status)
+                     const float* __restrict__ a_scale, TC* __restrict__ out, long long ld, int N, int M, int k_blocks, int splits, int tile_rows, int* status,
+                     const uint8_t* __restrict__ next_weights, long long next_bytes)
 {
     using T = Tile<BN>;
     extern __shared__ uint8_t smem_raw[];
@@ -280,6 +281,15 @@ gemm_int8_few_kernel(const __grid_constant__ CUtensorMap map_w, const __grid_con
                     s = 0;
                     phase ^= 1;
                 }
+            }
+            // Every load of this block has been requested: what follows in a decode step are short kernels that leave the memory idle, and then a product
+            // whose weights are known now.  This block asks for its share of them to be brought into L2 meanwhile.  A hint only: nothing waits for it.
+            if (next_bytes > 0) {
+                const long long blocks = (long long)gridDim.x * gridDim.y, me = blockIdx.x + (long long)gridDim.x * blockIdx.y;
+                const long long piece = ((next_bytes + blocks - 1) / blocks + 127) / 128 * 128;
+                const long long stop = min(next_bytes, (me + 1) * piece);
+#pragma unroll 1
+                for (long long at = me * piece; at < stop; at += 16384) l2_prefetch(next_weights + at, (uint32_t)(min(stop - at, 16384LL) & ~15LL));
             }
         }
     } else if (warp == 1) {
@@ -605,7 +615,7 @@ static Plan choose(int M, int N, int K)
 
 template <int BN, typename TC, bool GATED>
 static int launch_few(const Plan& p, const CUtensorMap& mw, const CUtensorMap& ma, const float* w_scale, const float* a_scale, void* C, long long ldc, int M,
-                      int N, int k_blocks, int* status, cudaStream_t stream)
+                      int N, int k_blocks, int* status, cudaStream_t stream, const void* next_weights, long long next_bytes)
 {
     using T = Tile<BN>;
     auto kernel = gemm_int8_few_kernel<BN, TC, GATED>;
@@ -615,10 +625,11 @@ static int launch_few(const Plan& p, const CUtensorMap& mw, const CUtensorMap& m
     const dim3 grid((unsigned)((M + BN - 1) / BN * p.splits), (unsigned)((N + p.tile_rows - 1) / p.tile_rows));
     if (grid.y > 65535) SPY_FAIL("gemm_int8: %u weight tiles exceed the launch limits", grid.y);
     if (p.splits == 1)
-        spy_launch(kernel, grid, dim3(NUM_THREADS), T::SMEM, stream, mw, ma, w_scale, a_scale, (TC*)C, ldc, N, M, k_blocks, p.splits, p.tile_rows, status);
+        spy_launch(kernel, grid, dim3(NUM_THREADS), T::SMEM, stream, mw, ma, w_scale, a_scale, (TC*)C, ldc, N, M, k_blocks, p.splits, p.tile_rows, status,
+                   (const uint8_t*)next_weights, next_bytes);
     else
         spy_launch_cluster(kernel, grid, dim3(NUM_THREADS), T::SMEM, stream, (unsigned)p.splits, mw, ma, w_scale, a_scale, (TC*)C, ldc, N, M, k_blocks,
-                           p.splits, p.tile_rows, status);
+                           p.splits, p.tile_rows, status, (const uint8_t*)next_weights, next_bytes);
     SPY_CHECK_LAUNCH("gemm_int8");
     return 0;
 }
@@ -660,7 +671,7 @@ static int launch_pairs(const Plan& p, const CUtensorMap& mw, const CUtensorMap&
 
 template <typename TC, bool GATED>
 static int run(const void* A, long long lda, const float* a_scale, const void* W, long long ldw, const float* w_scale, void* C, long long ldc, int M, int N,
-               int K, int* status, cudaStream_t stream)
+               int K, int* status, cudaStream_t stream, const void* next_weights, long long next_bytes)
 {
     const Plan p = choose(M, N, K);
     const int k_blocks = (K + BK - 1) / BK;
@@ -671,26 +682,32 @@ static int run(const void* A, long long lda, const float* a_scale, const void* W
         return launch_pairs<TC, GATED>(p, mw, ma, w_scale, a_scale, C, ldc, M, N, k_blocks, tokens, status, stream);
     }
     if (make_map(&mw, W, N, K, ldw, p.tile_rows) || make_map(&ma, A, M, K, lda, p.bn)) return 1;
-    if (p.bn == 16) return launch_few<16, TC, GATED>(p, mw, ma, w_scale, a_scale, C, ldc, M, N, k_blocks, status, stream);
-    if (p.bn == 32) return launch_few<32, TC, GATED>(p, mw, ma, w_scale, a_scale, C, ldc, M, N, k_blocks, status, stream);
-    if (p.bn == 64) return launch_few<64, TC, GATED>(p, mw, ma, w_scale, a_scale, C, ldc, M, N, k_blocks, status, stream);
-    return launch_few<128, TC, GATED>(p, mw, ma, w_scale, a_scale, C, ldc, M, N, k_blocks, status, stream);
+    if (p.bn == 16) return launch_few<16, TC, GATED>(p, mw, ma, w_scale, a_scale, C, ldc, M, N, k_blocks, status, stream, next_weights, next_bytes);
+    if (p.bn == 32) return launch_few<32, TC, GATED>(p, mw, ma, w_scale, a_scale, C, ldc, M, N, k_blocks, status, stream, next_weights, next_bytes);
+    if (p.bn == 64) return launch_few<64, TC, GATED>(p, mw, ma, w_scale, a_scale, C, ldc, M, N, k_blocks, status, stream, next_weights, next_bytes);
+    return launch_few<128, TC, GATED>(p, mw, ma, w_scale, a_scale, C, ldc, M, N, k_blocks, status, stream, next_weights, next_bytes);
 }
 
 }  // namespace
 
 // A [M, K] and W [N, K] int8, rows lda / ldw bytes apart (multiples of 16); a_scale [M], w_scale [N]; C [M, N] of c_dtype, rows ldc elements apart.
 // gated: W's rows alternate gate and up rows, C is [M, N / 2] bfloat16.  status: null, or two ints that receive a code if a bounded wait runs out.
+// next_weights / next_bytes (may be null / 0): memory that a later kernel of the stream will read, which the kernel for few tokens asks to be brought into L2.
 extern "C" int spy_gemm_int8(const void* A, long long lda, const float* a_scale, const void* W, long long ldw, const float* w_scale, void* C, int c_dtype,
-                             long long ldc, int M, int N, int K, int gated, int* status, cudaStream_t stream)
+                             long long ldc, int M, int N, int K, int gated, int* status, cudaStream_t stream, const void* next_weights,
+                             long long next_bytes)
 {
+    if (next_weights == nullptr || next_bytes <= 0 || (reinterpret_cast<uintptr_t>(next_weights) & 15)) {
+        next_weights = nullptr;
+        next_bytes = 0;
+    }
     if (M <= 0 || N <= 0) return 0;
     if (K <= 0 || K > MAX_K) SPY_FAIL("gemm_int8: K %d must lie in 1..%d (32-bit sums)", K, MAX_K);
     if (lda % 16 != 0 || ldw % 16 != 0) SPY_FAIL("gemm_int8: row distances %lld/%lld must be multiples of 16 bytes", lda, ldw);
     if ((reinterpret_cast<uintptr_t>(A) & 15) || (reinterpret_cast<uintptr_t>(W) & 15)) SPY_FAIL("gemm_int8: operands must be 16-byte aligned");
     if (gated && (N % 2 != 0 || c_dtype != SPY_BF16)) SPY_FAIL("gemm_int8: the gated epilogue needs an even N and bfloat16 output");
-    if (gated) return run<bf16, true>(A, lda, a_scale, W, ldw, w_scale, C, ldc, M, N, K, status, stream);
-    if (c_dtype == SPY_BF16) return run<bf16, false>(A, lda, a_scale, W, ldw, w_scale, C, ldc, M, N, K, status, stream);
-    if (c_dtype == SPY_F32) return run<float, false>(A, lda, a_scale, W, ldw, w_scale, C, ldc, M, N, K, status, stream);
+    if (gated) return run<bf16, true>(A, lda, a_scale, W, ldw, w_scale, C, ldc, M, N, K, status, stream, next_weights, next_bytes);
+    if (c_dtype == SPY_BF16) return run<bf16, false>(A, lda, a_scale, W, ldw, w_scale, C, ldc, M, N, K, status, stream, next_weights, next_bytes);
+    if (c_dtype == SPY_F32) return run<float, false>(A, lda, a_scale, W, ldw, w_scale, C, ldc, M, N, K, status, stream, next_weights, next_bytes);
     SPY_FAIL("gemm_int8: unknown output dtype code %d", c_dtype);
 }

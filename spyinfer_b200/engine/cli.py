@@ -7,7 +7,7 @@ ids, streamed as they are generated.  Lines of one conversation are appended to 
 ``/new`` starts a fresh one.
 
     spyinfer -m /path/to/model [-b cuda] [--dtype bfloat16|float32] [--max-new-tokens N]
-             [--temperature X] [--top-k K] [--seed N] [--prompt-tokens 1,2,3 | --prompt-len N] [--stats]
+             [--quantization int8] [--temperature X] [--top-k K] [--seed N] [--prompt-tokens 1,2,3 | --prompt-len N] [--stats]
     spyinfer --random CONFIG.json --seed 7 ...        (random weights instead of a checkpoint)
 """
 from __future__ import annotations
@@ -30,6 +30,7 @@ def build_parser() -> argparse.ArgumentParser:
     ap.add_argument("--random", metavar="CONFIG_JSON", help="a config.json; the model gets seeded random weights")
     ap.add_argument("--seed", type=int, default=0, help="seed of random weights and of temperature sampling")
     ap.add_argument("--dtype", default="bfloat16", choices=["bfloat16", "bf16", "float32", "fp32"])
+    ap.add_argument("--quantization", default=None, choices=["int8"], help="run the layers' products in 8-bit integers (with --dtype bfloat16)")
     ap.add_argument("--prompt-tokens", help="run this one prompt (comma-separated ids) and exit")
     ap.add_argument("--prompt-len", type=int, default=None, help="run one prompt of this many seeded random token ids and exit")
     ap.add_argument("--max-new-tokens", type=int, default=64)
@@ -64,7 +65,7 @@ def main(argv=None) -> int:
     from .llm_engine import LLMEngine
 
     params = {"dtype": args.dtype}
-    for key in ("max_num_batched_tokens", "max_num_seqs", "chunk_size", "max_model_len", "kvcache_block_size", "num_kvcache_blocks"):
+    for key in ("quantization", "max_num_batched_tokens", "max_num_seqs", "chunk_size", "max_model_len", "kvcache_block_size", "num_kvcache_blocks"):
         if getattr(args, key) is not None:
             params[key] = getattr(args, key)
     print("Using CUDA backend", flush=True)

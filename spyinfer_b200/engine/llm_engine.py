@@ -5,7 +5,8 @@
 this engine.  Engine options are keyword arguments with the names of the reference's
 parameter map (src/engine/llm_engine.cpp:11-16): ``max_num_batched_tokens``,
 ``max_num_seqs``, ``max_model_len``, ``kvcache_block_size``, ``num_kvcache_blocks``,
-``backend_type`` (only "cuda" exists here), plus ``dtype``.
+``backend_type`` (only "cuda" exists here), plus ``dtype`` and ``quantization`` (``"int8"``: the layers' weights are quantised as they
+are loaded and their products run in 8-bit integers; Qwen3, bfloat16).
 
     engine = LLMEngine("/path/to/model", dtype="bfloat16", max_num_seqs=64)
     rid = engine.add_request([1, 2, 3], SamplingParams(max_new_tokens=16))
@@ -67,7 +68,7 @@ class LLMEngine:
         spec = self.model_config.to_spec()
         self.config.clamp_to_model(spec.max_position)
         dtype = torch.bfloat16 if self.config.dtype == "bfloat16" else torch.float32
-        self.model = Model(spec, dtype, self.config.device, self.config.max_model_len)
+        self.model = Model(spec, dtype, self.config.device, self.config.max_model_len, quantization=self.config.quantization)
         if model_path is not None:
             self.model.load(model_path)
         else:

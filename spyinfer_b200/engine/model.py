@@ -8,6 +8,7 @@ src/models/qwen3.hpp:283-301; only the wanted rows are computed here).
 from __future__ import annotations
 
 import warnings
+from dataclasses import replace
 from typing import Dict, List, Optional
 
 import torch
@@ -39,13 +40,24 @@ def _prefixed(part, prefix: str) -> List[WeightDecl]:
 
 
 class Model:
-    def __init__(self, spec: ModelSpec, dtype: torch.dtype, device, max_model_len: int):
+    def __init__(self, spec: ModelSpec, dtype: torch.dtype, device, max_model_len: int, quantization: Optional[str] = None):
+        """``quantization="int8"``: the layers' products run on 8-bit weights and activations (``Int8Linear``); embedding, attention, stream, final norm
+        and head stay as they are.  Every part of every layer has to take it."""
         spec.validate()
         self.spec = spec
         self.ctx = BuildContext(dtype=dtype, device=torch.device(device) if device is not None else None,
                                 max_model_len=min(max_model_len, spec.max_position))
+        layer_ctx = replace(self.ctx, quantization=quantization)
         self.embedding = build_part(spec.embedding, self.ctx)
-        self.layers = [_Layer(ls, self.ctx) for ls in spec.layers]
+        self.layers = [_Layer(ls, layer_ctx) for ls in spec.layers]
+        if quantization is not None:
+            if quantization != "int8" or dtype != torch.bfloat16:
+                raise ValueError(f"quantization {quantization!r} with {dtype}: only \"int8\" with bfloat16 exists")
+            refused = sorted({p.kind for layer in self.layers for p in layer.parts() if not p.takes_int8()}
+                             | {layer.block.kind for layer in self.layers if not layer.block.takes_int8()})
+            if refused or any(e.before is not None for e in spec.run_order):
+                raise ValueError(f"quantization \"int8\" does not cover this architecture ({spec.architecture}): no 8-bit form of "
+                                 + (", ".join(refused) if refused else "what its run order adds to the stream"))
         self.final_norm = build_part(spec.final_norm, self.ctx)
         self.head = build_part(spec.head, self.ctx)
         # tensors that the run order adds to the stream between layers (name -> rows), and the bound tensors

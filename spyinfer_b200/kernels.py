@@ -2123,7 +2123,7 @@ class _Kernel:
 _P, _L, _I, _F = ctypes.c_void_p, ctypes.c_longlong, ctypes.c_int, ctypes.c_float
 _quantize_int8 = _Kernel("quant_int8", "spy_quantize_int8", _P, _I, _L, _P, _L, _P, _I, _I, _P)
 _rmsnorm_int8 = _Kernel("quant_int8", "spy_rmsnorm_int8", _P, _I, _P, _I, _I, _L, _P, _P, _I, _P, _L, _P, _I, _I, _F, _I, _P)
-_gemm_int8 = _Kernel("gemm_int8", "spy_gemm_int8", _P, _L, _P, _P, _L, _P, _P, _I, _L, _I, _I, _I, _I, _P, _P)
+_gemm_int8 = _Kernel("gemm_int8", "spy_gemm_int8", _P, _L, _P, _P, _L, _P, _P, _I, _L, _I, _I, _I, _I, _P, _P, _P, _L)
 
 
 def _on_current_device(t: torch.Tensor, what: str) -> int:
@@ -2216,10 +2216,11 @@ def rmsnorm_int8(x: torch.Tensor, weight: torch.Tensor, eps: float, out: Optiona
 
 
 def gemm_int8(a: Int8Rows, w: Int8Rows, out: Optional[torch.Tensor] = None, status: Optional[torch.Tensor] = None, out_dtype: Optional[torch.dtype] = None,
-              epilogue: Optional[str] = None) -> torch.Tensor:
+              epilogue: Optional[str] = None, prefetch: Optional[torch.Tensor] = None, prefetch_bytes: int = 0) -> torch.Tensor:
     """``a [M, K] @ w [N, K]^T`` of 8-bit rows on the tensor cores, ``(sum_k a w) * a.scales[m] * w.scales[n]`` with the sum in 32-bit integers (exact; K below
     131,072), in bfloat16 (default) or float32.  ``epilogue="swiglu"``: ``w``'s rows alternate gate and up rows and the result is ``silu(gate) * up``,
-    ``[M, N / 2]`` bfloat16.  A row whose scale is NaN gives a row of NaN.  A token's result does not depend on the rest of the batch."""
+    ``[M, N / 2]`` bfloat16.  A row whose scale is NaN gives a row of NaN.  A token's result does not depend on the rest of the batch.
+    ``prefetch``, ``prefetch_bytes``: as ``gemm_tcgen05`` has them."""
     M, K, lda, a_codes, a_scales = _int8_layout(a, "gemm_int8 input")
     device = a.codes.get_device()
     N, k_of_w, ldw, w_codes, w_scales = _int8_layout(w, "gemm_int8 weight", device)
@@ -2241,8 +2242,15 @@ def gemm_int8(a: Int8Rows, w: Int8Rows, out: Optional[torch.Tensor] = None, stat
             if torch.cuda.is_current_stream_capturing() and str(a.codes.device) not in _status_words:
                 raise KernelError("gemm_int8: the device's status word does not exist yet: make one call (or status_word()) before the capture, or give a status")
             status = _int8_status[device] = status_word(a.codes.device)
+    next_at = next_bytes = 0
+    if prefetch is not None and M <= 256:
+        if prefetch.get_device() != device:
+            raise KernelError(f"gemm_int8: the tensor to prefetch lies on {prefetch.device}, the operands on cuda:{device}")
+        next_at, next_bytes = prefetch.data_ptr(), prefetch.numel() * prefetch.element_size()
+        if prefetch_bytes > 0:
+            next_bytes = min(next_bytes, prefetch_bytes)
     _gemm_int8(a_codes, lda, a_scales, w_codes, ldw, w_scales, out.data_ptr(), _code(out, "gemm_int8 output"), n_out, M, N, K, 1 if epilogue else 0,
-               status.data_ptr(), _raw_stream(device))
+               status.data_ptr(), _raw_stream(device), next_at, next_bytes)
     return out
 
 

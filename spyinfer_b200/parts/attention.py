@@ -18,7 +18,7 @@ from .. import kernels
 from ..config.spec import CompositeCacheNeed, PagedCacheNeed, StateCacheNeed
 from ..weights.loader import WeightDecl
 from .base import Mixer
-from .linear import Linear
+from .linear import Linear, linear_for
 from .registry import build_part, register_part
 
 
@@ -91,8 +91,8 @@ class Attention(Mixer):
         bias = None
         if self.qkv_bias:
             bias = torch.cat([tensors[p + n].float() for n in ("q_proj.bias", "k_proj.bias", "v_proj.bias")]).contiguous()
-        self.qkv = Linear(torch.cat(qkv, dim=0).contiguous(), self.ctx.dtype, bias=bias)
-        self.o = Linear(tensors[p + "o_proj.weight"], self.ctx.dtype, bias=tensors[p + "o_proj.bias"] if self.o_bias else None)
+        self.qkv = linear_for(self.ctx, torch.cat(qkv, dim=0).contiguous(), bias=bias)
+        self.o = linear_for(self.ctx, tensors[p + "o_proj.weight"], bias=tensors[p + "o_proj.bias"] if self.o_bias else None)
         if self.qk_norm_eps is not None:
             self.q_norm, self.k_norm = tensors[p + "q_norm.weight"], tensors[p + "k_norm.weight"]
             if self.q_norm.dtype != self.k_norm.dtype:
@@ -107,6 +107,9 @@ class Attention(Mixer):
 
     def linears(self):
         return [self.qkv, self.o]
+
+    def takes_int8(self):
+        return type(self) is Attention      # not the kinds that are made from it
 
     def cache_need(self):
         return PagedCacheNeed(self.nkv, self.hd, int(self.window) if self.window is not None else None)
@@ -161,12 +164,12 @@ class Attention(Mixer):
         qkv = self.qkv(x, defer=True)
         q = None
         if qkv.dim() == 3:   # split-K partial products: summed inside the next kernel, q gets a buffer of its own
-            q = torch.empty((x.shape[0], self.nh * self.hd), dtype=x.dtype, device=x.device)
+            q = torch.empty((x.shape[0], self.nh * self.hd), dtype=self.ctx.dtype, device=x.device)
         q = kernels.qk_rope_store(qkv, self.nh, self.nkv, self.hd, self.q_norm, self.k_norm, float(self.qk_norm_eps or 0.0),
                                   self.rope_table, batch.positions, batch.seq_of_token, cache.block_table, cache.pages,
                                   store=cache.writes, status=batch.status, q_out=q,
                                   pairing=self.position.pairing if self.position is not None else "half")
-        out = torch.empty((x.shape[0], self.nh * self.hd), dtype=x.dtype, device=x.device)
+        out = torch.empty((x.shape[0], self.nh * self.hd), dtype=self.ctx.dtype, device=x.device)
         self.attend(q, out, batch, cache)
         return self.o(out, defer=self.defer_output)
 

@@ -27,11 +27,13 @@ from ..weights.loader import WeightDecl
 @dataclass
 class BuildContext:
     """What every part is built with.  ``dtype`` is the storage type of activations and of
-    the cache: bfloat16 (the serving path) or float32 (everything in true 32-bit)."""
+    the cache: bfloat16 (the serving path) or float32 (everything in true 32-bit).  ``quantization`` ``"int8"``: the parts
+    that ``takes_int8`` hold their weights in 8 bits and read their input as ``kernels.Int8Rows``."""
 
     dtype: torch.dtype
     device: torch.device
     max_model_len: int
+    quantization: Optional[str] = None
 
 
 @dataclass
@@ -111,6 +113,11 @@ class Part:
     def modules(self) -> List[str]:
         return list(self.kernel_modules)
 
+    def takes_int8(self) -> bool:
+        """Whether the part can be built with ``BuildContext.quantization`` ``"int8"``: a mixer or feed-forward whose products all run on 8-bit rows and
+        whose input may be ``Int8Rows``, a norm that can hand such rows over (``emits_int8``)."""
+        return False
+
     def choosing(self) -> List["Part"]:
         """The parts (this one, or those it is made of) that launch other kernels, or with other arguments, for batches of the same padded
         sizes: a graph of such a step is captured for every answer of their ``choice``.  Parts of equal ``choice_sizes`` answer alike."""
@@ -140,6 +147,8 @@ class Norm(Part):
     takes_channel_scale: bool = False
     #: True: ``forward_add`` also takes a ``NormedDelta`` as ``delta`` (of its own size, groups and eps)
     takes_normed_delta: bool = False
+    #: set by a block arrangement whose sublayer behind the norm reads 8-bit rows: ``forward_add`` then returns ``kernels.Int8Rows``
+    emits_int8: bool = False
 
     def forward(self, x: torch.Tensor, out_dtype: Optional[torch.dtype] = None) -> torch.Tensor:
         raise NotImplementedError
@@ -230,6 +239,10 @@ class Block:
         """``hidden`` is the 32-bit residual stream; ``delta`` the previous block's output
         that is still to be added to it (None for the first).  Returns the same pair."""
         raise NotImplementedError
+
+    def takes_int8(self) -> bool:
+        """Whether the arrangement can hand 8-bit rows from its norms to its sublayers (``BuildContext.quantization``)."""
+        return False
 
     def run_feed_forward(self, x: torch.Tensor, batch) -> torch.Tensor:
         return self.feed_forward.forward(x, batch) if self.feed_forward.takes_batch else self.feed_forward.forward(x)

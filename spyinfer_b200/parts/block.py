@@ -37,6 +37,16 @@ def build_block(kind: str, parts, params=None) -> Block:
 class PreNormBlock(Block):
     graph_safe = True
 
+    def __init__(self, parts, params=None):
+        super().__init__(parts, params)
+        # with 8-bit weights the norms hand 8-bit rows over: the stream's sum, the norm and the quantisation are one launch
+        for norm, sublayer in ((self.mixer_norm, self.mixer), (self.ffn_norm, self.feed_forward)):
+            if norm.ctx.quantization == "int8" and sublayer.takes_int8() and norm.takes_int8():
+                norm.emits_int8 = True
+
+    def takes_int8(self):
+        return True
+
     def forward(self, hidden, delta, batch, cache):
         x = self.mixer_norm.forward_add(hidden, delta)
         a = self.mixer.forward(x, batch, cache)

@@ -13,7 +13,7 @@ import torch
 from .. import kernels
 from ..weights.loader import WeightDecl
 from .base import FeedForward
-from .linear import Linear
+from .linear import Linear, linear_for
 from .registry import register_part
 
 
@@ -105,10 +105,11 @@ class GatedMLP(FeedForward):
             gate, up = gate.float(), up.float()
         # silu and gelu_tanh without biases, and the clamped activation with or without them, run in the tensor-core product's epilogue
         self.fused = (self.ctx.dtype == torch.bfloat16 and gate.dtype == torch.bfloat16 and kernels.tensor_core_gemm_takes(2 * self.inter, self.hidden)
-                      and (self.activation == "clamped_swish" or (self.activation in ("silu", "gelu_tanh") and not self.has_bias)))
+                      and (self.activation == "clamped_swish" or (self.activation in ("silu", "gelu_tanh") and not self.has_bias))) \
+            or self.ctx.quantization == "int8"
         if self.fused:
             # rows alternate gate_i, up_i: the tensor-core product applies act(gate) * up in its epilogue
-            self.gate_up = Linear(torch.stack([gate, up], dim=1).reshape(2 * self.inter, self.hidden).contiguous(), self.ctx.dtype)
+            self.gate_up = linear_for(self.ctx, torch.stack([gate, up], dim=1).reshape(2 * self.inter, self.hidden).contiguous())
         else:
             self.gate_up = Linear(torch.cat([gate, up], dim=0).contiguous(), self.ctx.dtype)
         if self.has_bias:
@@ -119,11 +120,14 @@ class GatedMLP(FeedForward):
         down_bias = tensors[p + n["down"] + ".b"].float().contiguous() if self.has_bias else None
         if self.leave_output_bias:           # the consumer adds it (and may then take the down product's split-K parts unsummed)
             self.output_bias, down_bias = down_bias, None
-        self.down = Linear(tensors[p + n["down"]], self.ctx.dtype, bias=down_bias)
+        self.down = linear_for(self.ctx, tensors[p + n["down"]], bias=down_bias)
         self.gate_up.hint_next = not self.fused       # fused: the down product follows at once
 
     def linears(self):
         return [self.gate_up, self.down]
+
+    def takes_int8(self):
+        return self.activation == "silu" and not self.has_bias
 
     def modules(self):
         return ([] if self.fused else ["swiglu"]) + self.gate_up.modules() + self.down.modules()

@@ -97,3 +97,39 @@ class Linear:
             return kernels.gemm_simt(x, w, out)
         return self._plain(x, w, out)
 
+
+class Int8Linear:
+    """The same with the weight in 8 bits, one scale for every output, made here from the stored weight.  The input is 8-bit rows already (a norm that
+    ``emits_int8``) or is quantised row by row first.  The sums are integers: a token's result does not depend on the batch it is in."""
+
+    next_weight: Optional[torch.Tensor] = None      # as ``Linear``'s
+    hint_next: bool = True
+    fast = True                                     # it has the gated epilogue
+
+    def __init__(self, weight: torch.Tensor, bias: Optional[torch.Tensor] = None):
+        if weight.dim() != 2:
+            raise ValueError(f"a linear weight is [out, in], found shape {tuple(weight.shape)}")
+        if bias is not None and tuple(bias.shape) != (weight.shape[0],):
+            raise ValueError(f"a bias of shape {tuple(bias.shape)} does not fit a weight of shape {tuple(weight.shape)}")
+        self.rows, self.bias = kernels.quantize_int8(weight), bias
+        self.weight = self.rows.codes               # what the product ahead asks for ahead of time
+        self.out_features, self.in_features = weight.shape
+        self.prefetch_bytes = _prefetch_cap()
+
+    def modules(self) -> List[str]:
+        return ["quant_int8", "gemm_int8"] + (["swiglu"] if self.bias is not None else [])
+
+    def __call__(self, x, out_dtype: Optional[torch.dtype] = None, epilogue: Optional[str] = None, defer: bool = False) -> torch.Tensor:
+        """``x``: ``Int8Rows`` or a matrix.  ``epilogue="swiglu"`` as ``Linear``; ``defer`` is taken and not used: the result is always summed."""
+        if self.bias is not None and epilogue is not None:
+            raise ValueError("a product with a bias takes no fused epilogue")
+        if not isinstance(x, kernels.Int8Rows):
+            x = kernels.quantize_int8(x)
+        hint = self.next_weight if self.hint_next and x.codes.shape[0] <= 256 and self.prefetch_bytes > 0 else None
+        y = kernels.gemm_int8(x, self.rows, out_dtype=out_dtype, epilogue=epilogue, prefetch=hint, prefetch_bytes=self.prefetch_bytes)
+        return kernels.add_bias(y, self.bias) if self.bias is not None else y
+
+
+def linear_for(ctx, weight: torch.Tensor, bias: Optional[torch.Tensor] = None):
+    """The product that a part built with ``ctx`` runs: in 8 bits when the model is, else by the storage types."""
+    return Int8Linear(weight, bias) if ctx.quantization == "int8" else Linear(weight, ctx.dtype, bias=bias)

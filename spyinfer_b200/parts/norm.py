@@ -40,7 +40,10 @@ class RMSNorm(Norm):
             self.weight = (self.weight.float() + self.weight_offset).contiguous()     # the gain itself, in 32-bit
 
     def modules(self):
-        return ["residual_norm"] if self.adds_to_stream else ["rmsnorm"]
+        return ["residual_norm"] if self.adds_to_stream else (["quant_int8"] if self.emits_int8 else ["rmsnorm"])
+
+    def takes_int8(self):
+        return True
 
     def add_normed(self, residual, y):
         """``residual += norm(y)`` (32-bit, in place) for a block whose norm sits on a sublayer's output; ``y`` may be a
@@ -55,6 +58,8 @@ class RMSNorm(Norm):
         return kernels.rmsnorm(x, self.weight, self.eps, out)
 
     def forward_add(self, residual, delta, rows=None, out_dtype=None):
+        if self.emits_int8:
+            return kernels.rmsnorm_int8(residual, self.weight, self.eps, delta=delta, rows=rows, write_back=delta is not None and rows is None)
         n = residual.shape[0] if rows is None else rows.shape[0]
         out = torch.empty((n, self.size), dtype=out_dtype or self.ctx.dtype, device=residual.device)
         return kernels.rmsnorm(residual, self.weight, self.eps, out, delta=delta, rows=rows, write_back=delta is not None and rows is None)

@@ -351,3 +351,111 @@ def test_rows_of_codes_start_on_borders():
         kernels.quantize_int8(torch.zeros(4, 32))
     with pytest.raises(KernelError, match="CUDA"):
         kernels.rmsnorm_int8(torch.zeros(4, 32), torch.ones(32), 1e-6)
+
+
+# ---- the engine on 8-bit weights ----------------------------------------------------------------------------------------------
+def plain_int8_logits(monkeypatch, weights, cfg, tokens):
+    """The plain implementation with every product of the layers on quantised rows and quantised weights, in 32 bits (the sums in 64)."""
+    import plain_model
+
+    def quantised(m):
+        m = m.double()
+        top = m.abs().amax(1, keepdim=True).clamp_min(1e-300)
+        return torch.round(m * 127.0 / top), top / 127.0
+
+    head = weights["model.embed_tokens.weight"] if cfg.get("tie_word_embeddings", False) else weights["lm_head.weight"]
+    plain = plain_model.linear
+
+    def linear(x, w):
+        if w is head:
+            return plain(x, w)
+        (qx, sx), (qw, sw) = quantised(x), quantised(w)
+        return ((qx @ qw.t()) * sx * sw.t()).to(x.dtype)
+
+    monkeypatch.setattr(plain_model, "linear", linear)
+    try:
+        return plain_model.forward_logits(weights, cfg, tokens)
+    finally:
+        monkeypatch.setattr(plain_model, "linear", plain)
+
+
+def int8_engine(folder, **kw):
+    from spyinfer_b200 import LLMEngine
+    opts = dict(dtype="bfloat16", quantization="int8", max_num_seqs=4, max_model_len=256, kvcache_block_size=16, num_kvcache_blocks=64, max_num_batched_tokens=256)
+    opts.update(kw)
+    return LLMEngine(folder, **opts)
+
+
+@gpu
+@pytest.mark.parametrize("name", ["a", "b", "c", "d", "e"])
+def test_engine_logits(name, tiny_models, monkeypatch):
+    """A prompt whole, in portions, and its last tokens one by one, against the plain implementation on quantised weights and rows.  The engine's
+    numbers between two products are rounded to bfloat16, so a few codes of a row differ by one: at most what two independent quantisations
+    differ by, 0.41 of a code (rms) with the largest of a row near 2.5 times its rms, 1 % of the row; four such rows a layer in up to four
+    layers add up to 4 % of the logits in the mean square if nothing damped them, and the largest of some thousand differences is to its rms
+    what the largest logit is to the logits', within a factor of two."""
+    from spyinfer_b200.engine.batch import StepEntry
+    folder, cfg, weights = tiny_models[name]
+    g = torch.Generator().manual_seed(7)
+    tokens = torch.randint(0, cfg["vocab_size"], (150,), generator=g).tolist()
+    want = plain_int8_logits(monkeypatch, weights, cfg, tokens).double()
+    engine = int8_engine(folder)
+
+    def check(rows, first):
+        got = torch.as_tensor(rows).double()
+        ref = want[first:first + got.shape[0]]
+        err = (got - ref).abs()
+        assert bool(torch.isfinite(got).all())
+        assert float(err.max()) <= 8e-2 * float(ref.abs().max()) and float(err.square().mean().sqrt()) <= 4e-2 * float(ref.square().mean().sqrt())
+
+    check(engine.step_raw([StepEntry("whole", tokens, list(range(150)))]), 0)
+    at = 0
+    for n in (7, 1, 64, 33, 40):
+        check(engine.step_raw([StepEntry("parts", tokens[at:at + n], list(range(n)))]), at)
+        at += n
+    for at in range(145, 150):
+        check(engine.step_raw([StepEntry("parts", tokens[at:at + 1], [0])]), at)
+    used = {m for layer in engine.model.layers for p in layer.parts() for m in p.modules()}
+    assert {"gemm_int8", "quant_int8"} <= used and not {"gemm_tcgen05", "gemm_simt", "rmsnorm"} & used
+
+
+@gpu
+def test_engine_generates_the_same_with_and_without_graphs(tiny_models):
+    """Decode steps and small mixed steps replayed from graphs (with their hints of the next weights) against launches one by one."""
+    from spyinfer_b200 import SamplingParams
+    folder, cfg, _ = tiny_models["d"]
+    g = torch.Generator().manual_seed(3)
+    prompts = [torch.randint(0, cfg["vocab_size"], (n,), generator=g).tolist() for n in (1, 9, 40, 130, 17, 3)]
+    outs = []
+    for graphs in (True, False):
+        engine = int8_engine(folder, use_cuda_graphs=graphs)
+        outs.append(engine.generate(prompts, SamplingParams(max_new_tokens=20, ignore_eos=True)))
+        assert (engine.runner.graph_steps > 0) == graphs
+        engine.runner.check_status()
+    assert outs[0] == outs[1] and all(len(o) == 20 for o in outs[0])
+
+
+def test_engine_options():
+    from spyinfer_b200 import EngineConfig, config_from_json
+    from spyinfer_b200.engine.model import Model
+    from conftest import TINY
+    assert EngineConfig(quantization="int8").quantization == "int8" and EngineConfig().quantization is None
+    for bad in (dict(quantization="int4"), dict(quantization="int8", dtype="float32")):
+        with pytest.raises(ValueError, match="quantization"):
+            EngineConfig(**bad)
+    spec = config_from_json(TINY["a"]["config"]).to_spec()
+    model = Model(spec, torch.bfloat16, None, 256, quantization="int8")
+    assert all(l.block.mixer_norm.emits_int8 and l.block.ffn_norm.emits_int8 for l in model.layers) and not model.final_norm.emits_int8
+    assert not Model(spec, torch.bfloat16, None, 256).layers[0].block.mixer_norm.emits_int8
+    with pytest.raises(ValueError, match="quantization"):
+        Model(spec, torch.float32, None, 256, quantization="int8")
+
+
+def test_other_architectures_are_refused():
+    from spyinfer_b200 import config_from_json
+    from spyinfer_b200.engine.model import Model
+    from test_bubalix import BX
+    from test_dogilorn import DG
+    for config in (BX["a"]["config"], DG["a"]["config"]):
+        with pytest.raises(ValueError, match="does not cover"):
+            Model(config_from_json(config).to_spec(), torch.bfloat16, None, 256, quantization="int8")
