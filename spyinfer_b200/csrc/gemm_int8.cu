@@ -326,7 +326,9 @@ gemm_int8_few_kernel(const __grid_constant__ CUtensorMap map_w, const __grid_con
         pdl_wait();                           // the tokens' scales and the output belong to kernels ahead in the stream until here
         if (tid < BN) sa[tid] = tid < tokens ? a_scale[y0 + tid] : 0.f;
         epilogue_barrier();
-        const bool ok = mbar_wait(accum_bar, 0, abort_flag);
+        // one lane asks for the warp: lanes that left the wait one by one would meet the warp-wide loads and barriers behind it apart
+        const bool ok = mbar_wait_warp(accum_bar, 0, abort_flag);
+        __syncwarp();
         fence_after_sync();
         const uint32_t acc = tmem_base + ((uint32_t)(quarter * 32) << 16);
         constexpr int COLS = BN < 32 ? BN : 32;
@@ -340,7 +342,6 @@ gemm_int8_few_kernel(const __grid_constant__ CUtensorMap map_w, const __grid_con
                 store_chunk<COLS, TC, GATED>(out, ld, lane, x0 + quarter * 32, y0 + c, x_end, M, r, sw, lane < COLS ? sa[c + lane] : 0.f, turn);
             }
         } else {
-            __syncwarp();
             if constexpr (T::MAIL_IN_RING) cluster_arrive();
             cluster_wait();
             const uint32_t to = map_to_rank(smem_u32(mail + (size_t)rank * (BN / 4) * share + (row & (share - 1))), row / share);
@@ -363,9 +364,9 @@ gemm_int8_few_kernel(const __grid_constant__ CUtensorMap map_w, const __grid_con
             }
         }
     }
+    __syncwarp();                             // the lanes that had no part in a role wait for the one that had
     fence_before_sync();
     if (splits > 1 && warp < 2) {
-        __syncwarp();
         cluster_wait();
         cluster_arrive();
         cluster_wait();
@@ -454,6 +455,10 @@ gemm_int8_pair_kernel(const __grid_constant__ CUtensorMap map_w, const __grid_co
         *abort_flag = 0;
         asm volatile("fence.mbarrier_init.release.cluster;" ::: "memory");
     }
+    __syncwarp();
+    // The allocation is one for the pair.  Asked for before the other block runs it never comes back: without this barrier prompts of 640 tokens
+    // through 36 layers, where a block's start can be held up by the many small blocks of a quantisation on its SM, stopped within some hundred steps.
+    cluster_sync();
     if (warp == 1) tmem_alloc_pair(tmem_slot, 2u * PAIR_BN);
     fence_before_sync();
     __syncthreads();
@@ -545,7 +550,9 @@ gemm_int8_pair_kernel(const __grid_constant__ CUtensorMap map_w, const __grid_co
             const int x0 = (tile / tokens.count) * (2 * BM) + (int)rank * BM + quarter * 32, ty = tile % tokens.count;   // the warp's first weight row
             const int y0 = tokens.first(ty), height = tokens.height(ty), y_end = min(M, y0 + height);
             const float sw = x0 + lane < N ? w_scale[x0 + lane] : 0.f;
-            if (!mbar_wait(acc_full + buf, aph, abort_flag)) break;
+            const bool ok = mbar_wait_warp(acc_full + buf, aph, abort_flag);     // one lane asks: the warp goes on together
+            __syncwarp();
+            if (!ok) break;
             fence_after_sync();
 #pragma unroll 1
             for (int c = 0; c < height; c += 32) {
@@ -560,6 +567,7 @@ gemm_int8_pair_kernel(const __grid_constant__ CUtensorMap map_w, const __grid_co
         }
     }
 
+    __syncwarp();     // the lanes that had no part in a role wait for the one that had
     fence_before_sync();
     __syncthreads();
     if (*abort_flag) {
