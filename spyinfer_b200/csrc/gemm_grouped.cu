@@ -103,6 +103,8 @@ gemm_grouped_kernel(const __grid_constant__ CUtensorMap map_a, const __grid_cons
         *abort_flag = 0;
         asm volatile("fence.mbarrier_init.release.cluster;" ::: "memory");
     }
+    __syncwarp();
+    cluster_sync();   // the allocation is one for the pair: asked for before the other block runs, it may never come back
     if (warp == 1) tmem_alloc_pair(tmem_slot, 2u * BN);
     fence_before_sync();
     __syncthreads();
