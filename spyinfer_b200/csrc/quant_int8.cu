@@ -7,7 +7,7 @@
 // The codes are exact: 127 y / amax is compared with the half between two integers without being rounded first.  In 32 bits
 // t = y * (127 / amax) is off by at most |t| 2^-24 <= 7.6e-6 from the quotient (the fused multiply-add rounds t itself to the integer
 // directly), so only where t lies within 2e-5 of a half is the question left open; there 254 y and (2 n + 1) amax are compared without rounding
-// (one group of eight in 3,000).  The codes depend on no summation order and on no approximation, and a test can ask for equality.
+// (one group of eight in 3,000 of float32 numbers; bfloat16 rows have exact halves, and one in sixty).  The codes depend on no summation order and on no approximation, and a test can ask for equality.
 //
 // A row of zeros has codes 0 and scale 0.  A row with a NaN or an infinity has codes 0 and the scale NaN: what is made of it is NaN, and no
 // other row is touched.  |code| <= 127: -128 does not occur.
@@ -53,9 +53,6 @@ __device__ __forceinline__ void store8(bf16* p, const float (&v)[8])
     }
     *reinterpret_cast<uint4*>(p) = make_uint4(w[0], w[1], w[2], w[3]);
 }
-
-// Threads that hold a row, `groups` times eight elements each.
-__host__ __device__ constexpr int block_most(int groups) { return groups <= 2 ? 1024 : 512; }
 
 // The eight elements of a row that group g of this thread holds; what lies behind the end is zero.  WHOLE: rows of a multiple of 8 elements on
 // 16-byte borders, a thread holds neighbours.  Else a warp's lanes hold neighbours, so that their plain loads and stores meet in few sectors.
@@ -148,18 +145,20 @@ __device__ __forceinline__ float scale_of(uint32_t size, float factor)
 {
     return size >= 0x7f800000u ? __int_as_float(0x7fc00000) : __uint_as_float(size) / 127.0f * factor;
 }
+__device__ __forceinline__ uint2 encode_group(float (&y)[8], const RowScale& s)
+{
+    if (!s.plain) {
+#pragma unroll
+        for (int e = 0; e < 8; ++e) y[e] = s.none ? 0.f : y[e] * s.lift;
+    }
+    return encode8(y, s.k, s.amax);
+}
 template <bool WHOLE, int GROUPS>
 __device__ __forceinline__ void encode_row(int8_t* row, int len, float (&y)[GROUPS][8], uint32_t size)
 {
     const RowScale s = row_scale(size);
-    if (!s.plain) {
 #pragma unroll
-        for (int g = 0; g < GROUPS; ++g)
-#pragma unroll
-            for (int e = 0; e < 8; ++e) y[g][e] = s.none ? 0.f : y[g][e] * s.lift;
-    }
-#pragma unroll
-    for (int g = 0; g < GROUPS; ++g) put_codes<WHOLE>(row, g, len, encode8(y[g], s.k, s.amax));
+    for (int g = 0; g < GROUPS; ++g) put_codes<WHOLE>(row, g, len, encode_group(y[g], s));
 }
 
 // Sum and largest size over the block, one barrier; `part` holds 2 x 32 words and is used once a launch.
@@ -178,7 +177,7 @@ template <bool WITH_SUM> __device__ __forceinline__ void block_reduce(float& sum
 }
 
 template <typename T, bool WHOLE, int GROUPS>
-__global__ void __launch_bounds__(block_most(GROUPS)) quantize_kernel(const T* __restrict__ x, long long ldx, int8_t* __restrict__ codes, long long ldc,
+__global__ void __launch_bounds__(1024) quantize_kernel(const T* __restrict__ x, long long ldx, int8_t* __restrict__ codes, long long ldc,
                                                         float* __restrict__ scales, int len)
 {
     __shared__ uint32_t part[32];
@@ -195,6 +194,38 @@ __global__ void __launch_bounds__(block_most(GROUPS)) quantize_kernel(const T* _
         for (int e = 0; e < 8; ++e) size = size_max(size, v[g][e]);
     block_reduce<false>(none, size, part);
     encode_row<WHOLE, GROUPS>(codes + (size_t)blockIdx.x * ldc, len, v, size);
+    if (threadIdx.x == 0) scales[blockIdx.x] = scale_of(size, 1.f);
+}
+
+// bfloat16 rows of whole groups: the row is kept as it was read, two elements in a register, and the largest size is taken of two at once.
+template <int GROUPS>
+__global__ void __launch_bounds__(1024) quantize_packed_kernel(const bf16* __restrict__ x, long long ldx, int8_t* __restrict__ codes, long long ldc,
+                                                               float* __restrict__ scales, int len)
+{
+    __shared__ uint32_t part[32];
+    pdl_enter();
+    const bf16* row = x + (size_t)blockIdx.x * ldx;
+    uint4 v[GROUPS];
+#pragma unroll
+    for (int g = 0; g < GROUPS; ++g) {
+        v[g] = make_uint4(0, 0, 0, 0);
+        if (place<true>(g, 0) < len) v[g] = *reinterpret_cast<const uint4*>(row + place<true>(g, 0));
+    }
+    uint32_t two = 0;       // of bfloat16 bits without their signs the larger number is the larger size, a NaN the largest
+#pragma unroll
+    for (int g = 0; g < GROUPS; ++g)
+        two = __vmaxu2(__vmaxu2(two, __vmaxu2(v[g].x & 0x7fff7fffu, v[g].y & 0x7fff7fffu)), __vmaxu2(v[g].z & 0x7fff7fffu, v[g].w & 0x7fff7fffu));
+    uint32_t size = max(two << 16, two & 0xffff0000u);
+    float none = 0.f;
+    block_reduce<false>(none, size, part);
+    const RowScale s = row_scale(size);
+    int8_t* out = codes + (size_t)blockIdx.x * ldc;
+#pragma unroll
+    for (int g = 0; g < GROUPS; ++g) {
+        float y[8] = {__uint_as_float(v[g].x << 16), __uint_as_float(v[g].x & 0xffff0000u), __uint_as_float(v[g].y << 16), __uint_as_float(v[g].y & 0xffff0000u),
+                      __uint_as_float(v[g].z << 16), __uint_as_float(v[g].z & 0xffff0000u), __uint_as_float(v[g].w << 16), __uint_as_float(v[g].w & 0xffff0000u)};
+        put_codes<true>(out, g, len, encode_group(y, s));
+    }
     if (threadIdx.x == 0) scales[blockIdx.x] = scale_of(size, 1.f);
 }
 
@@ -228,7 +259,7 @@ __global__ void __launch_bounds__(1024) quantize_long_kernel(const T* __restrict
 }
 
 template <typename TX, typename TD, typename TW, bool WHOLE, int GROUPS>
-__global__ void __launch_bounds__(block_most(GROUPS)) rmsnorm_int8_kernel(TX* x, const TD* __restrict__ delta, int splits, long long split_stride, const int* __restrict__ rows,
+__global__ void __launch_bounds__(1024) rmsnorm_int8_kernel(TX* x, const TD* __restrict__ delta, int splits, long long split_stride, const int* __restrict__ rows,
                                                             const TW* __restrict__ w, int8_t* __restrict__ codes, long long ldc,
                                                             float* __restrict__ scales, int len, float eps, int write_back)
 {
@@ -272,16 +303,10 @@ __global__ void __launch_bounds__(block_most(GROUPS)) rmsnorm_int8_kernel(TX* x,
     if (threadIdx.x == 0) scales[blockIdx.x] = scale_of(size, 1.0f / sqrtf(ss / (float)len + eps));
 }
 
-constexpr int ROW_MOST = 8 * 8 * block_most(8);    // elements that a block holds
+constexpr int ROW_MOST = 1024 * 8 * 4;    // elements that a block holds, up to four groups of eight a thread
 
-// How a row is shared out: few rows (decoding) as wide as it goes, many rows 32 elements a thread, all their loads in flight together and
-// several blocks an SM.
-static inline int row_groups(bool whole, int n, int len)
-{
-    if (len > 8 * 4 * block_most(4)) return 8;
-    if (!whole || n >= 512) return 4;
-    return len > 8 * block_most(1) ? 2 : 1;
-}
+// Groups of eight elements a thread holds: `least`, or as many as a block of 1,024 threads needs.
+static inline int row_groups(int len, int least) { return len > 16384 && least < 4 ? 4 : (len > 8192 && least < 2 ? 2 : least); }
 static inline int row_threads(int len, int groups)
 {
     const int t = ((len + 8 * groups - 1) / (8 * groups) + 31) / 32 * 32;
@@ -298,11 +323,23 @@ static int quantize(const T* x, long long ldx, int8_t* codes, long long ldc, flo
         SPY_CHECK_LAUNCH("quantize_int8 (long rows)");
         return 0;
     }
-    const int groups = row_groups(whole, n, len);
-    auto kernel = groups == 8 ? (whole ? quantize_kernel<T, true, 8> : quantize_kernel<T, false, 8>)
-                : groups == 4 ? (whole ? quantize_kernel<T, true, 4> : quantize_kernel<T, false, 4>)
-                : groups == 2 ? quantize_kernel<T, true, 2> : quantize_kernel<T, true, 1>;
-    spy_launch(kernel, dim3(n), dim3(row_threads(len, groups)), 0, stream, x, ldx, codes, ldc, scales, len);
+    // Few rows: the row spread as wide as it goes.  Many: more groups a thread, as what a warp does once a row (reduction, barrier, division) is bought
+    // once for more elements.  us with 1 / 2 / 4 / 8 groups, whole rows of bfloat16: 64 x 4,096 1.9 / 1.9 / 2.1 / 2.9, 2,048 x 4,096 8.4 / 7.3 / 7.2 / 7.4,
+    // 2,048 x 12,288 - / 20.5 / 17.4 / 16.2, 24,576 x 4,096 81 / 63.7 / 59.3 / 52.9 (0.87 of the copy rate; two thirds of the issue slots are taken); of float32 2,048 x
+    // 4,096 8.3 / 7.4 / 6.5 (0.98).  Others, float32: 1,531 x 4,999 20.8 / 12.6 / 14.6, 64 x 4,999 2.6 / 3.7 / 5.4.
+    const bool packed = whole && sizeof(T) == 2;
+    const int groups = row_groups(len, n < 1024 ? 1 : (!whole ? 2 : (packed && (long long)n * len >= (1 << 24) ? 8 : 4))), threads = row_threads(len, groups);
+    if constexpr (sizeof(T) == 2) {
+        if (whole) {
+            auto kernel = groups == 8 ? quantize_packed_kernel<8> : groups == 4 ? quantize_packed_kernel<4> : groups == 2 ? quantize_packed_kernel<2> : quantize_packed_kernel<1>;
+            spy_launch(kernel, dim3(n), dim3(threads), 0, stream, x, ldx, codes, ldc, scales, len);
+            SPY_CHECK_LAUNCH("quantize_int8 (bfloat16)");
+            return 0;
+        }
+    }
+    auto kernel = whole ? (groups == 4 ? quantize_kernel<T, true, 4> : groups == 2 ? quantize_kernel<T, true, 2> : quantize_kernel<T, true, 1>)
+                        : (groups == 4 ? quantize_kernel<T, false, 4> : groups == 2 ? quantize_kernel<T, false, 2> : quantize_kernel<T, false, 1>);
+    spy_launch(kernel, dim3(n), dim3(threads), 0, stream, x, ldx, codes, ldc, scales, len);
     SPY_CHECK_LAUNCH("quantize_int8");
     return 0;
 }
@@ -312,10 +349,11 @@ static int norm(TX* x, const TD* delta, int splits, long long split_stride, cons
                 int n, int len, float eps, int write_back, cudaStream_t stream)
 {
     const bool whole = len % 8 == 0 && aligned16(x) && aligned16(delta) && aligned16(w) && split_stride * (long long)sizeof(TD) % 16 == 0;
-    const int groups = row_groups(whole, n, len);
-    auto kernel = groups == 8 ? (whole ? rmsnorm_int8_kernel<TX, TD, TW, true, 8> : rmsnorm_int8_kernel<TX, TD, TW, false, 8>)
-                : groups == 4 ? (whole ? rmsnorm_int8_kernel<TX, TD, TW, true, 4> : rmsnorm_int8_kernel<TX, TD, TW, false, 4>)
-                : groups == 2 ? rmsnorm_int8_kernel<TX, TD, TW, true, 2> : rmsnorm_int8_kernel<TX, TD, TW, true, 1>;
+    // us with 1 / 2 / 4 groups a thread.  Whole rows: 64 x 5,120 3.0 / 3.1 / 3.3, 512 x 4,096 5.7 / 5.7 / 8.4, 4,096 x 5,120 36.5 / 38.1 / 42.1 (a norm with a
+    // bfloat16 result 41.8).  Others: 64 x 4,999 3.7 / 4.4 / 26.9, 1,000 x 4,999 23.7 / 17.9 / 71.0.
+    const int groups = row_groups(len, whole || n < 512 ? 1 : 2);
+    auto kernel = whole ? (groups == 4 ? rmsnorm_int8_kernel<TX, TD, TW, true, 4> : groups == 2 ? rmsnorm_int8_kernel<TX, TD, TW, true, 2> : rmsnorm_int8_kernel<TX, TD, TW, true, 1>)
+                        : (groups == 4 ? rmsnorm_int8_kernel<TX, TD, TW, false, 4> : groups == 2 ? rmsnorm_int8_kernel<TX, TD, TW, false, 2> : rmsnorm_int8_kernel<TX, TD, TW, false, 1>);
     spy_launch(kernel, dim3(n), dim3(row_threads(len, groups)), 0, stream, x, delta, splits, split_stride, rows, w, codes, ldc, scales, len, eps,
                write_back);
     SPY_CHECK_LAUNCH("rmsnorm_int8");

@@ -84,6 +84,17 @@ def test_quantize_rows_at_the_edges(length, dtype):
 
 
 @gpu
+@pytest.mark.parametrize("rows,length", [(1024, 64), (1100, 8208), (4200, 4096), (16500, 1024), (1030, 16392), (1025, 32768), (1300, 1003)])
+def test_quantize_many_rows(rows, length):
+    """The shares of a row that many rows are given, at their limits."""
+    for dtype in (torch.bfloat16, torch.float32):
+        x = wild_rows(rows, length, 9).to(dtype)
+        x[rows - 1, length - 1] = float("inf")
+        x[rows - 2] = 0.0
+        check_rows(kernels.quantize_int8(x), x.float())
+
+
+@gpu
 @pytest.mark.parametrize("dtype", [torch.float32, torch.bfloat16])
 def test_quantize_views(dtype):
     """Rows that lie apart or start off a 16-byte border, and codes into a part of a wider matrix, whose other bytes stay."""
