@@ -27,7 +27,10 @@ using namespace tc;
 constexpr int BM = 128;            // weight rows of a block = the instruction's M (half of it on pairs)
 constexpr int BK = 128;            // codes of K a stage = bytes of a swizzled row
 constexpr int UMMA_K = 32;
-constexpr int NUM_THREADS = 192;   // warp 0: TMA, warp 1: MMA and tensor memory, warps 2 to 5: epilogue
+// warp 0: TMA, warp 1: MMA and tensor memory, warps 2 and on: epilogue, in fours (each of four reads its own quarter of the tensor-memory lanes), the fours
+// taking the tokens in turns.  Four warps alone read a tile of 128 tokens out in 3.1 us, eight in 1.6, and nothing runs beside that behind a block's last tile.
+__host__ __device__ constexpr int epilogue_warps(int tokens) { return tokens >= 64 ? 8 : 4; }
+__host__ __device__ constexpr int block_threads(int tokens) { return 64 + 32 * epilogue_warps(tokens); }
 constexpr int MAX_K = 131071;
 
 // Instruction descriptor of kind::i8: signed 8-bit operands, both K-major, a 32-bit integer accumulator.
@@ -64,7 +67,7 @@ __device__ __forceinline__ void umma_s8_pair(uint32_t tmem_d, uint64_t desc_a, u
 // below -87 gives g / inf = -0, the limit.
 __device__ __forceinline__ float silu_mul(float g, float u) { return __fdividef(g, 1.0f + __expf(-g)) * u; }
 
-__device__ __forceinline__ void epilogue_barrier() { asm volatile("bar.sync 1, 128;" ::: "memory"); }   // the four epilogue warps
+template <int WARPS> __device__ __forceinline__ void epilogue_barrier() { asm volatile("bar.sync 1, %0;" ::"n"(32 * WARPS) : "memory"); }
 __device__ __forceinline__ void cluster_arrive() { asm volatile("barrier.cluster.arrive.release.aligned;" ::: "memory"); }
 __device__ __forceinline__ void cluster_wait() { asm volatile("barrier.cluster.wait.acquire.aligned;" ::: "memory"); }
 __device__ __forceinline__ void store_shared_of(uint32_t cluster_addr, uint32_t a, uint32_t b, uint32_t c, uint32_t d)
@@ -72,8 +75,8 @@ __device__ __forceinline__ void store_shared_of(uint32_t cluster_addr, uint32_t 
     asm volatile("st.shared::cluster.v4.u32 [%0], {%1, %2, %3, %4};" ::"r"(cluster_addr), "r"(a), "r"(b), "r"(c), "r"(d) : "memory");
 }
 
-constexpr int TURN_LD = 36;                                  // floats between the tokens of a warp's chunk of 32 tokens x 32 weight rows
-constexpr int TURN_BYTES = 32 * TURN_LD * 4 + 32 * 4;        // and the tokens' scales
+constexpr int TURN_LD = 36;                                  // floats between the tokens of a warp's chunk of some tokens x 32 weight rows
+__host__ __device__ constexpr int turn_bytes(int cols) { return (cols * TURN_LD + 32) * 4; }   // and the tokens' scales
 
 // Finishes COLS tokens of 32 weight rows: this lane holds weight row x0 + lane of the tokens from y on.  `turn` is the warp's own place in shared
 // memory, where the numbers are turned so that the results leave in rows of 16 bytes a lane.
@@ -83,7 +86,7 @@ __device__ __forceinline__ void store_chunk(TC* __restrict__ out, long long ld, 
 {
     const int count = min(COLS, y_end - y), outs = min(32, x_end - x0);
     if (outs <= 0 || count <= 0) return;      // the same for the whole warp
-    float* sa = turn + 32 * TURN_LD;
+    float* sa = turn + COLS * TURN_LD;
     sa[lane] = sa_lane;
     __syncwarp();
 #pragma unroll
@@ -156,6 +159,9 @@ __device__ __forceinline__ void store_chunk(TC* __restrict__ out, long long ld, 
 template <int BN> struct Tile {
     static constexpr int Y_BYTES = BN * BK;
     static constexpr int TMEM_COLS = BN < 32 ? 32 : BN;
+    static constexpr int COLS = BN < 32 ? BN : 32;              // tokens of a chunk that a warp reads out at a time
+    static constexpr int WARPS = epilogue_warps(BN);
+    static constexpr int THREADS = block_threads(BN);
     static constexpr int MAIL = BN * BM * 4;
     static constexpr bool MAIL_IN_RING = BN > 32;
     static constexpr int AREA = 110 * 1024 - (MAIL_IN_RING ? 0 : MAIL);
@@ -167,21 +173,21 @@ template <int BN> struct Tile {
         const int n = (AREA - (BM * BK - x_bytes(tile_rows))) / (x_bytes(tile_rows) + Y_BYTES);
         return n < MAX_STAGES ? n : MAX_STAGES;
     }
-    static_assert(MAIL <= AREA && 4 * TURN_BYTES <= AREA, "what follows the main loop fits the ring");
+    static_assert(MAIL <= AREA && WARPS * turn_bytes(COLS) <= AREA, "what follows the main loop fits the ring");
 };
 
-// The end of a tile whose K is cut: this thread adds up weight row x of every SPLITS-th group of four tokens.  Gated: lanes 2i and 2i + 1 hold gate and
+// The end of a tile whose K is cut: this thread adds up weight row x of every STEP-th group of four tokens.  Gated: lanes 2i and 2i + 1 hold gate and
 // up; of four tokens the even lane finishes the first two and the odd lane the others.
 template <int SPLITS, int BN, typename TC, bool GATED>
 __device__ __forceinline__ void finish_cut(TC* __restrict__ out, long long ld, const int4* mail, const float* sa, float sw, int x, int x_end, int y0, int tokens,
                                            int tid, int lane)
 {
-    constexpr int SHARE = BM / SPLITS;
+    constexpr int SHARE = BM / SPLITS, STEP = 32 * epilogue_warps(BN) / SHARE;      // groups of four tokens that the block finishes at a time
     const int4* got = mail + tid % SHARE;
     const bool inside = x < x_end, odd = (lane & 1) != 0;
     TC* dst = out + (size_t)y0 * ld + (GATED ? x / 2 : x);
 #pragma unroll 2
-    for (int q0 = 0; q0 < BN / 4; q0 += SPLITS) {
+    for (int q0 = 0; q0 < BN / 4; q0 += STEP) {
         const int q = q0 + tid / SHARE;
         if (4 * q0 >= tokens) break;                  // the same for the whole block
         int4 sum = make_int4(0, 0, 0, 0);
@@ -214,7 +220,7 @@ __device__ __forceinline__ void finish_cut(TC* __restrict__ out, long long ld, c
 
 // Block (token tile, K range) = (blockIdx.x / splits, blockIdx.x % splits) of weight tile blockIdx.y; the K ranges of a tile are a cluster.
 template <int BN, typename TC, bool GATED>
-__global__ void __launch_bounds__(NUM_THREADS, 2)
+__global__ void __launch_bounds__(block_threads(BN), 2)
 gemm_int8_few_kernel(const __grid_constant__ CUtensorMap map_w, const __grid_constant__ CUtensorMap map_a, const float* __restrict__ w_scale,
                      const float* __restrict__ a_scale, TC* __restrict__ out, long long ld, int N, int M, int k_blocks, int splits, int tile_rows, int* status,
                      const uint8_t* __restrict__ next_weights, long long next_bytes)
@@ -318,24 +324,24 @@ gemm_int8_few_kernel(const __grid_constant__ CUtensorMap map_w, const __grid_con
         }
     } else {
         // warp w reads tensor-memory lanes 32 (w % 4) .. + 31, i.e. weight rows of the tile
-        const int quarter = warp & 3, row = quarter * 32 + lane, tid = threadIdx.x - 64;
+        const int quarter = warp & 3, turns = (warp - 2) >> 2, row = quarter * 32 + lane, tid = threadIdx.x - 64;
         const int tokens = min(BN, M - y0), x_end = min(N, x0 + tile_rows);
         const int share = BM / splits, part = rank * share + (tid & (share - 1));        // K cut: the weight row that this thread finishes
         const int x = x0 + (splits > 1 ? part : row);
         const float sw = x < x_end ? w_scale[x] : 0.f;
         pdl_wait();                           // the tokens' scales and the output belong to kernels ahead in the stream until here
         if (tid < BN) sa[tid] = tid < tokens ? a_scale[y0 + tid] : 0.f;
-        epilogue_barrier();
+        epilogue_barrier<T::WARPS>();
         // one lane asks for the warp: lanes that left the wait one by one would meet the warp-wide loads and barriers behind it apart
         const bool ok = mbar_wait_warp(accum_bar, 0, abort_flag);
         __syncwarp();
         fence_after_sync();
         const uint32_t acc = tmem_base + ((uint32_t)(quarter * 32) << 16);
-        constexpr int COLS = BN < 32 ? BN : 32;
+        constexpr int COLS = T::COLS, STEP = COLS * (T::WARPS / 4);
         if (splits == 1) {
-            float* turn = reinterpret_cast<float*>(tiles + quarter * TURN_BYTES);
+            float* turn = reinterpret_cast<float*>(tiles + (warp - 2) * turn_bytes(COLS));
 #pragma unroll 1
-            for (int c = 0; c < tokens && ok; c += COLS) {
+            for (int c = turns * COLS; c < tokens && ok; c += STEP) {
                 uint32_t r[COLS];
                 tmem_load<COLS>(acc + (uint32_t)c, r);
                 tmem_wait_ld();
@@ -346,7 +352,7 @@ gemm_int8_few_kernel(const __grid_constant__ CUtensorMap map_w, const __grid_con
             cluster_wait();
             const uint32_t to = map_to_rank(smem_u32(mail + (size_t)rank * (BN / 4) * share + (row & (share - 1))), row / share);
 #pragma unroll 1
-            for (int c = 0; c < tokens && ok; c += COLS) {
+            for (int c = turns * COLS; c < tokens && ok; c += STEP) {
                 uint32_t r[COLS];
                 tmem_load<COLS>(acc + (uint32_t)c, r);
                 tmem_wait_ld();
@@ -391,7 +397,7 @@ gemm_int8_few_kernel(const __grid_constant__ CUtensorMap map_w, const __grid_con
 // ---- many tokens -----------------------------------------------------------------------------------------------------------------
 // A cluster of two blocks on neighbouring SMs computes one tile of 256 weight rows and up to 256 tokens: each block loads its 128 weight rows and its
 // half of the tile's tokens, the leader (rank 0) issues tcgen05.mma.cta_group::2 instructions that read both blocks' shared memory and
-// accumulate each block's 128 rows in its own tensor memory; both blocks' four epilogue warps read their halves back and turn them in shared memory
+// accumulate each block's 128 rows in its own tensor memory; both blocks' epilogue warps read their halves back and turn them in shared memory
 // on the way out.  The TMA loads of both blocks complete on the leader's full barrier; a commit frees a stage, and publishes an accumulator, in both
 // blocks; the peer's epilogue threads arrive on the leader's accumulator-empty barrier.  Cluster c walks tiles c, c + clusters, ...; tiles are numbered
 // with the token tiles fastest, so that clusters side by side share weight tiles in L2.
@@ -416,7 +422,10 @@ constexpr int PAIR_BN = 256;                                 // tensor-memory co
 constexpr int PAIR_MAX_STAGES = 10;
 constexpr int PAIR_X_BYTES = BM * BK;
 constexpr int PAIR_AREA = 6 * 2 * PAIR_X_BYTES;              // the ring: six stages at 256 tokens a tile, more at fewer
-constexpr size_t PAIR_SMEM = (size_t)PAIR_AREA + 4 * TURN_BYTES + 1024 /* alignment slack */ + 256 /* barriers */;
+constexpr int PAIR_COLS = 16;                                // tokens of a chunk that an epilogue warp reads out at a time
+constexpr int PAIR_WARPS = epilogue_warps(PAIR_BN);
+constexpr int PAIR_THREADS = block_threads(PAIR_BN);
+constexpr size_t PAIR_SMEM = (size_t)PAIR_AREA + PAIR_WARPS * turn_bytes(PAIR_COLS) + 1024 /* alignment slack */ + 256 /* barriers */;
 __host__ __device__ constexpr int pair_stage_bytes(int token_rows) { return PAIR_X_BYTES + token_rows / 2 * BK; }
 __host__ __device__ constexpr int pair_stages(int token_rows)
 {
@@ -425,7 +434,7 @@ __host__ __device__ constexpr int pair_stages(int token_rows)
 }
 
 template <typename TC, bool GATED>
-__global__ void __launch_bounds__(NUM_THREADS, 1)
+__global__ void __launch_bounds__(PAIR_THREADS, 1)
 gemm_int8_pair_kernel(const __grid_constant__ CUtensorMap map_w, const __grid_constant__ CUtensorMap map_a, const float* __restrict__ w_scale,
                       const float* __restrict__ a_scale, TC* __restrict__ out, long long ld, int N, int M, int k_blocks, TokenTiles tokens, int num_tiles,
                       int* status)
@@ -433,10 +442,10 @@ gemm_int8_pair_kernel(const __grid_constant__ CUtensorMap map_w, const __grid_co
     const int stages = pair_stages(tokens.rows), stage_bytes = pair_stage_bytes(tokens.rows);   // a lower tile's copies bring spare rows behind its own
     extern __shared__ uint8_t smem_raw[];
     uint8_t* tiles = reinterpret_cast<uint8_t*>((reinterpret_cast<uintptr_t>(smem_raw) + 1023) & ~(uintptr_t)1023);
-    uint64_t* full_bar = reinterpret_cast<uint64_t*>(tiles + PAIR_AREA + 4 * TURN_BYTES);   // the leader's are used
+    uint64_t* full_bar = reinterpret_cast<uint64_t*>(tiles + PAIR_AREA + PAIR_WARPS * turn_bytes(PAIR_COLS));   // the leader's are used
     uint64_t* empty_bar = full_bar + PAIR_MAX_STAGES;   // every block's own
     uint64_t* acc_full = empty_bar + PAIR_MAX_STAGES;   // [2] every block's own
-    uint64_t* acc_empty = acc_full + 2;                 // [2] the leader's are used: 256 arrivals
+    uint64_t* acc_empty = acc_full + 2;                 // [2] the leader's are used: an arrival of every epilogue thread of both
     uint32_t* tmem_slot = reinterpret_cast<uint32_t*>(acc_empty + 2);
     volatile int* abort_flag = reinterpret_cast<volatile int*>(tmem_slot + 1);
 
@@ -450,7 +459,7 @@ gemm_int8_pair_kernel(const __grid_constant__ CUtensorMap map_w, const __grid_co
         }
         for (int b = 0; b < 2; ++b) {
             mbar_init(acc_full + b, 1);
-            mbar_init(acc_empty + b, 256);
+            mbar_init(acc_empty + b, 2 * 32 * PAIR_WARPS);
         }
         *abort_flag = 0;
         asm volatile("fence.mbarrier_init.release.cluster;" ::: "memory");
@@ -458,43 +467,45 @@ gemm_int8_pair_kernel(const __grid_constant__ CUtensorMap map_w, const __grid_co
     __syncwarp();
     // The allocation is one for the pair.  Asked for before the other block runs it never comes back: without this barrier prompts of 640 tokens
     // through 36 layers, where a block's start can be held up by the many small blocks of a quantisation on its SM, stopped within some hundred steps.
-    cluster_sync();
-    if (warp == 1) tmem_alloc_pair(tmem_slot, 2u * PAIR_BN);
+    cluster_sync();   // both blocks run, and their barriers are initialised
+    // the weights of the first stages are requested beside the allocation and before the wait for the kernels ahead in the stream
+    const int pre = min(k_blocks, stages);
+    if (warp == 0) {
+        if (lane == 0) {
+            const int x0 = (cluster / tokens.count) * (2 * BM) + (int)rank * BM;
+            for (int i = 0; i < pre; ++i) {
+                if (rank == 0) mbar_expect_tx(full_bar + i, 2u * stage_bytes);     // both blocks' bytes
+                tma_load_2d_pair(smem_u32(tiles + (size_t)i * stage_bytes), &map_w, i * BK, x0, map_to_rank(smem_u32(full_bar + i), 0));
+            }
+        }
+        __syncwarp();
+    } else if (warp == 1) {
+        tmem_alloc_pair(tmem_slot, 2u * PAIR_BN);
+    }
     fence_before_sync();
-    __syncthreads();
-    cluster_sync();   // both blocks' barriers are initialised and their tensor memory is allocated before either is used from the other side
+    cluster_sync();   // both blocks' tensor memory is allocated before it is used from the other side
     fence_after_sync();
     const uint32_t tmem_base = *tmem_slot;
 
     pdl_launch_dependents();
     if (warp == 0) {
         if (lane == 0) {
-            int s = 0;
-            uint32_t phase = 0;   // of the ring's round; the first round's waits end at once
-            bool ok = true, first = true;
+            pdl_wait();
+            int s = pre == stages ? 0 : pre;
+            uint32_t phase = pre == stages ? 1 : 0;   // of the ring's round; the first round's waits end at once
+            bool ok = true;
             for (int tile = cluster; ok && tile < num_tiles; tile += clusters) {
                 const int ty = tile % tokens.count;
                 const int x0 = (tile / tokens.count) * (2 * BM) + (int)rank * BM, y0 = tokens.first(ty) + (int)rank * (tokens.height(ty) / 2);
                 int kb = 0;
-                if (first) {
-                    // the weights of the first stages are requested before the wait for the kernels ahead in the stream
-                    const int pre = min(k_blocks, stages);
-                    for (int i = 0; i < pre; ++i) {
-                        if (rank == 0) mbar_expect_tx(full_bar + i, 2u * stage_bytes);
-                        tma_load_2d_pair(smem_u32(tiles + (size_t)i * stage_bytes), &map_w, i * BK, x0, map_to_rank(smem_u32(full_bar + i), 0));
-                    }
-                    pdl_wait();
-                    for (int i = 0; i < pre; ++i)
-                        tma_load_2d_pair(smem_u32(tiles + (size_t)i * stage_bytes + PAIR_X_BYTES), &map_a, i * BK, y0, map_to_rank(smem_u32(full_bar + i), 0));
-                    kb = pre;
-                    if (pre == stages) phase = 1;
-                    else s = pre;
-                    first = false;
+                if (tile == cluster) {
+                    for (; kb < pre; ++kb)
+                        tma_load_2d_pair(smem_u32(tiles + (size_t)kb * stage_bytes + PAIR_X_BYTES), &map_a, kb * BK, y0, map_to_rank(smem_u32(full_bar + kb), 0));
                 }
                 for (; kb < k_blocks; ++kb) {
                     if (!mbar_wait(empty_bar + s, phase ^ 1, abort_flag)) { ok = false; break; }
                     uint8_t* xs = tiles + (size_t)s * stage_bytes;
-                    if (rank == 0) mbar_expect_tx(full_bar + s, 2u * stage_bytes);   // both blocks' bytes
+                    if (rank == 0) mbar_expect_tx(full_bar + s, 2u * stage_bytes);
                     const uint32_t leader_full = map_to_rank(smem_u32(full_bar + s), 0);
                     tma_load_2d_pair(smem_u32(xs), &map_w, kb * BK, x0, leader_full);
                     tma_load_2d_pair(smem_u32(xs + PAIR_X_BYTES), &map_a, kb * BK, y0, leader_full);
@@ -540,8 +551,8 @@ gemm_int8_pair_kernel(const __grid_constant__ CUtensorMap map_w, const __grid_co
             }
         }
     } else {
-        const int quarter = warp & 3;
-        float* turn = reinterpret_cast<float*>(tiles + PAIR_AREA + quarter * TURN_BYTES);
+        const int quarter = warp & 3, turns = (warp - 2) >> 2;
+        float* turn = reinterpret_cast<float*>(tiles + PAIR_AREA + (warp - 2) * turn_bytes(PAIR_COLS));
         pdl_wait();   // the scales and the output belong to kernels ahead in the stream until here
         int i = 0;
         for (int tile = cluster; tile < num_tiles; tile += clusters, ++i) {
@@ -550,16 +561,30 @@ gemm_int8_pair_kernel(const __grid_constant__ CUtensorMap map_w, const __grid_co
             const int x0 = (tile / tokens.count) * (2 * BM) + (int)rank * BM + quarter * 32, ty = tile % tokens.count;   // the warp's first weight row
             const int y0 = tokens.first(ty), height = tokens.height(ty), y_end = min(M, y0 + height);
             const float sw = x0 + lane < N ? w_scale[x0 + lane] : 0.f;
+            // the scales of a chunk's tokens, and the chunk itself, are requested a chunk ahead
+            constexpr int STEP = PAIR_COLS * (PAIR_WARPS / 4);
+            auto scale_of = [&](int c) { return lane < PAIR_COLS && y0 + c + lane < y_end ? a_scale[y0 + c + lane] : 0.f; };
+            const uint32_t acc = tmem_base + ((uint32_t)(quarter * 32) << 16) + (uint32_t)(buf * PAIR_BN);
+            int c = turns * PAIR_COLS;
+            float sa = scale_of(c);
             const bool ok = mbar_wait_warp(acc_full + buf, aph, abort_flag);     // one lane asks: the warp goes on together
             __syncwarp();
             if (!ok) break;
             fence_after_sync();
+            uint32_t ahead[PAIR_COLS];
+            if (c < height) tmem_load<PAIR_COLS>(acc + (uint32_t)c, ahead);
 #pragma unroll 1
-            for (int c = 0; c < height; c += 32) {
-                uint32_t r[32];
-                tmem_load<32>(tmem_base + ((uint32_t)(quarter * 32) << 16) + (uint32_t)(buf * PAIR_BN + c), r);
+            for (; c < height; c += STEP) {
+                uint32_t r[PAIR_COLS];
                 tmem_wait_ld();
-                store_chunk<32, TC, GATED>(out, ld, lane, x0, y0 + c, N, y_end, r, sw, y0 + c + lane < y_end ? a_scale[y0 + c + lane] : 0.f, turn);
+#pragma unroll
+                for (int j = 0; j < PAIR_COLS; ++j) r[j] = ahead[j];
+                const float sa_now = sa;
+                if (c + STEP < height) {
+                    tmem_load<PAIR_COLS>(acc + (uint32_t)(c + STEP), ahead);
+                    sa = scale_of(c + STEP);
+                }
+                store_chunk<PAIR_COLS, TC, GATED>(out, ld, lane, x0, y0 + c, N, y_end, r, sw, sa_now, turn);
             }
             fence_before_sync();
             if (rank == 0) mbar_arrive(acc_empty + buf);
@@ -633,10 +658,10 @@ static int launch_few(const Plan& p, const CUtensorMap& mw, const CUtensorMap& m
     const dim3 grid((unsigned)((M + BN - 1) / BN * p.splits), (unsigned)((N + p.tile_rows - 1) / p.tile_rows));
     if (grid.y > 65535) SPY_FAIL("gemm_int8: %u weight tiles exceed the launch limits", grid.y);
     if (p.splits == 1)
-        spy_launch(kernel, grid, dim3(NUM_THREADS), T::SMEM, stream, mw, ma, w_scale, a_scale, (TC*)C, ldc, N, M, k_blocks, p.splits, p.tile_rows, status,
+        spy_launch(kernel, grid, dim3(T::THREADS), T::SMEM, stream, mw, ma, w_scale, a_scale, (TC*)C, ldc, N, M, k_blocks, p.splits, p.tile_rows, status,
                    (const uint8_t*)next_weights, next_bytes);
     else
-        spy_launch_cluster(kernel, grid, dim3(NUM_THREADS), T::SMEM, stream, (unsigned)p.splits, mw, ma, w_scale, a_scale, (TC*)C, ldc, N, M, k_blocks,
+        spy_launch_cluster(kernel, grid, dim3(T::THREADS), T::SMEM, stream, (unsigned)p.splits, mw, ma, w_scale, a_scale, (TC*)C, ldc, N, M, k_blocks,
                            p.splits, p.tile_rows, status, (const uint8_t*)next_weights, next_bytes);
     SPY_CHECK_LAUNCH("gemm_int8");
     return 0;
@@ -654,7 +679,7 @@ static int launch_pairs(const Plan& p, const CUtensorMap& mw, const CUtensorMap&
         const int sms = spy_sm_count();
         cudaLaunchConfig_t cfg = {};
         cfg.gridDim = dim3(sms / 2 * 2);
-        cfg.blockDim = dim3(NUM_THREADS);
+        cfg.blockDim = dim3(PAIR_THREADS);
         cfg.dynamicSmemBytes = PAIR_SMEM;
         cudaLaunchAttribute attr[1];
         attr[0].id = cudaLaunchAttributeClusterDimension;
@@ -671,7 +696,7 @@ static int launch_pairs(const Plan& p, const CUtensorMap& mw, const CUtensorMap&
     const long long num_tiles = (long long)((N + 2 * BM - 1) / (2 * BM)) * tokens.count;
     if (num_tiles > 0x7fffffffLL) SPY_FAIL("gemm_int8: %lld tiles exceed the kernel's range", num_tiles);
     const int clusters = (int)(num_tiles < clusters_max ? num_tiles : clusters_max);
-    spy_launch_cluster(kernel, dim3(2 * clusters), dim3(NUM_THREADS), PAIR_SMEM, stream, 2u, mw, ma, w_scale, a_scale, (TC*)C, ldc, N, M, k_blocks, tokens,
+    spy_launch_cluster(kernel, dim3(2 * clusters), dim3(PAIR_THREADS), PAIR_SMEM, stream, 2u, mw, ma, w_scale, a_scale, (TC*)C, ldc, N, M, k_blocks, tokens,
                        (int)num_tiles, status);
     SPY_CHECK_LAUNCH("gemm_int8 (pairs)");
     return 0;
