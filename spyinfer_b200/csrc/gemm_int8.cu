@@ -14,6 +14,7 @@
 //
 // The reference has no integer product (its own are half precision: spymaster2h/spyinfer src/backends/cuda/cublas/sgemm.cu:37-55).
 #include <cuda.h>
+#include <math.h>
 
 #include "common.cuh"
 #include "tcgen05.cuh"
@@ -631,19 +632,59 @@ struct Plan {
     int count, bn, splits, tile_rows;
 };
 
+// The plan is the one of the least expected time, in us, with rates in bytes a us.  Both kernels: what is fixed, plus the slowest of what the main loop
+// waits for, plus the read-out behind it.  The numbers were fitted to 5,559 measurements of 13 weight sizes (512 x 8,192 to 51,200 x 5,120) at 1 to 4,096 tokens
+// with all tiles and cuts: the chosen plans take 2 % longer than the fastest of all measured on average, 20 % at worst (1,024 x 1,024, 320 tokens).  Which
+// kernel, for instance (us, few / pairs): 6,144 x 4,096 at 128 tokens 11.5 / 15.2, 384 15.0 / 17.5, 640 17.9 / 19.0; 34,816 x 5,120 gated at 64 tokens 30.5 / 34.2, 192
+// 48.9 / 39.3.  How K is cut (1 / 2 / 4 / 8 ways, 8 tokens): 6,144 x 4,096 11.4 / 8.1 / 6.9 / 9.7, 4,096 x 12,288 37.8 / 18.4 / 12.4 / 11.8, 24,576 x 4,096 18.3 / 23.0 / 23.6 / -.
+static double few_time(int M, int N, int k_blocks, int bn, int splits, int rows, int sms)
+{
+    const double blocks = (double)((M + bn - 1) / bn) * ((N + rows - 1) / rows) * splits, depth = (k_blocks + splits - 1) / splits;
+    const double stage = (double)(rows + bn) * BK, tokens = (M < bn ? M : bn) / 128.0;
+    const double even = blocks / sms, most = (double)(((long long)blocks + sms - 1) / sms);
+    const double per_sm = blocks <= 2 * sms ? fmax(1.0, 0.46 * most + 0.54 * even) : 1.48 * even;      // an SM with one more; the last of many waves is not full
+    double load = (double)N * k_blocks * BK / 8.2e6;                                  // the weights from memory
+    load = fmax(load, depth * stage / 6.4e4);                                         // a block's stages, one after the other
+    load = fmax(load, per_sm * depth * stage / 9.6e4);                                // an SM's
+    load = fmax(load, blocks * depth * stage / 2.06e7);                               // everybody's, from L2
+    return 2.1 + (splits > 1 ? 0.8 + 1.7 * tokens : 0.0) + 1.9 * tokens + load;
+}
+static double pair_time(int M, int N, int k_blocks, int count, int sms)
+{
+    const TokenTiles t = token_tiles(M, count);
+    const int clusters = sms / 2 > 0 ? sms / 2 : 1;
+    const double height = t.rows / 256.0, rounds = (double)(((long long)((N + 2 * BM - 1) / (2 * BM)) * count + clusters - 1) / clusters);
+    const double load = fmax((double)N * k_blocks * BK / 8.2e6, rounds * k_blocks * pair_stage_bytes(t.rows) / 7.9e4);
+    return 6.1 + load + 2.0 * height + 1.2 * (rounds - 1) * height;
+}
+
 static Plan choose(int M, int N, int K)
 {
     const int k_blocks = (K + BK - 1) / BK, sms = spy_sm_count();
-    Plan p = {false, 0, M <= 16 ? 16 : (M <= 32 ? 32 : (M <= 64 ? 64 : 128)), 1, BM};
-    const long long w_tiles2 = (N + 2 * BM - 1) / (2 * BM);
-    if (M > 128 && w_tiles2 * ((M + 255) / 256) >= sms / 4) {
-        p.pairs = true;
-        p.count = (M + 255) / 256;
-        return p;
+    const int tile = M <= 16 ? 16 : (M <= 32 ? 32 : (M <= 64 ? 64 : 128));
+    Plan best = {false, 0, tile, 1, BM};
+    double least = 1e30;
+    for (int bn = tile; bn >= 16 && 2 * bn >= tile; bn /= 2) {
+        for (int splits = 1; splits <= 8 && (splits == 1 || k_blocks >= 2 * splits); splits *= 2) {
+            for (int rows = BM; rows >= (splits == 1 ? 64 : BM); rows -= 32) {      // weight rows of a multiple of what a warp reads out
+                const double t = few_time(M, N, k_blocks, bn, splits, rows, sms);
+                if (t < least && (N + rows - 1) / rows <= 65535) {
+                    least = t;
+                    best = {false, 0, bn, splits, rows};
+                }
+            }
+        }
     }
-    const long long tiles = (long long)((N + BM - 1) / BM) * ((M + p.bn - 1) / p.bn);
-    while (p.splits < 8 && tiles * p.splits * 2 <= 2 * sms && k_blocks >= 2 * 2 * p.splits) p.splits *= 2;
-    return p;
+    if (M < 64) return best;
+    const int lowest = (M + 255) / 256, runs = (M + 31) / 32;
+    for (int count = lowest; count <= runs && count <= 2 * lowest + 2; ++count) {
+        const double t = pair_time(M, N, k_blocks, count, sms);
+        if (t < least) {
+            least = t;
+            best = {true, count, 0, 1, BM};
+        }
+    }
+    return best;
 }
 
 template <int BN, typename TC, bool GATED>
@@ -656,7 +697,7 @@ static int launch_few(const Plan& p, const CUtensorMap& mw, const CUtensorMap& m
         SPY_CUDA(cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)T::SMEM));
     }
     const dim3 grid((unsigned)((M + BN - 1) / BN * p.splits), (unsigned)((N + p.tile_rows - 1) / p.tile_rows));
-    if (grid.y > 65535) SPY_FAIL("gemm_int8: %u weight tiles exceed the launch limits", grid.y);
+    if (grid.y > 65535) SPY_FAIL("gemm_int8: %u weight tiles exceed the launch limits", grid.y);   // beyond 8 million outputs
     if (p.splits == 1)
         spy_launch(kernel, grid, dim3(T::THREADS), T::SMEM, stream, mw, ma, w_scale, a_scale, (TC*)C, ldc, N, M, k_blocks, p.splits, p.tile_rows, status,
                    (const uint8_t*)next_weights, next_bytes);
