@@ -2093,9 +2093,13 @@ class Int8Rows(NamedTuple):
         return self.codes.device
 
 
+def _pitch(length: int) -> int:
+    return (length + 15) // 16 * 16
+
+
 def empty_int8(rows: int, length: int, device) -> Int8Rows:
     """Room for ``rows`` rows of ``length`` codes, a multiple of 16 bytes apart, and their scales."""
-    pitch = (length + 15) // 16 * 16
+    pitch = _pitch(length)
     codes = torch.empty((rows, pitch), dtype=torch.int8, device=device)
     return Int8Rows(codes if pitch == length else codes[:, :length], torch.empty((rows,), dtype=torch.float32, device=device))
 
@@ -2150,7 +2154,7 @@ def _int8_layout(m: Int8Rows, what: str, device: Optional[int] = None):
         _on_current_device(codes, what)
     pitch, step = codes.stride()
     if rows <= 1 or length == 0:
-        pitch = (length + 15) // 16 * 16
+        pitch = _pitch(length)
     address = codes.data_ptr()
     if (step != 1 and length > 1) or pitch < length or pitch & 15 or address & 15:
         raise KernelError(f"{what}: rows of codes must be contiguous and start on 16-byte borders, found strides {codes.stride()} at address "
@@ -2174,9 +2178,11 @@ def quantize_int8(x: torch.Tensor, out: Optional[Int8Rows] = None) -> Int8Rows:
         raise KernelError(f"quantize_int8 input: rows overlap (strides {x.stride()} for shape {tuple(x.shape)})")
     if out is None:
         out = empty_int8(n, length, x.device)
-    rows, width, pitch, codes, scales = _int8_layout(out, "quantize_int8 output", device)
-    if (rows, width) != (n, length):
-        raise KernelError(f"quantize_int8 output: {(rows, width)} does not fit the input {(n, length)}")
+        pitch, codes, scales = _pitch(length), out.codes.data_ptr(), out.scales.data_ptr()
+    else:
+        rows, width, pitch, codes, scales = _int8_layout(out, "quantize_int8 output", device)
+        if (rows, width) != (n, length):
+            raise KernelError(f"quantize_int8 output: {(rows, width)} does not fit the input {(n, length)}")
     _quantize_int8(x.data_ptr(), code, ldx, codes, pitch, scales, n, length, _raw_stream(device))
     return out
 
@@ -2206,9 +2212,11 @@ def rmsnorm_int8(x: torch.Tensor, weight: torch.Tensor, eps: float, out: Optiona
             raise KernelError(f"rmsnorm_int8 {what}: lies on {t.device}, the input on {x.device}")
     if out is None:
         out = empty_int8(n, H, x.device)
-    got, width, pitch, codes, scales = _int8_layout(out, "rmsnorm_int8 output", device)
-    if (got, width) != (n, H):
-        raise KernelError(f"rmsnorm_int8 output: expected {(n, H)}, found {(got, width)}")
+        pitch, codes, scales = _pitch(H), out.codes.data_ptr(), out.scales.data_ptr()
+    else:
+        got, width, pitch, codes, scales = _int8_layout(out, "rmsnorm_int8 output", device)
+        if (got, width) != (n, H):
+            raise KernelError(f"rmsnorm_int8 output: expected {(n, H)}, found {(got, width)}")
     _rmsnorm_int8(x.data_ptr(), _code(x, "rmsnorm_int8 input"), delta.data_ptr() if delta is not None else 0,
                   _code(delta, "rmsnorm_int8 delta") if delta is not None else 0, splits, split_stride, rows.data_ptr() if rows is not None else 0,
                   weight.data_ptr(), _code(weight, "rmsnorm_int8 weight"), codes, pitch, scales, n, H, eps, 1 if write_back else 0, _raw_stream(device))
