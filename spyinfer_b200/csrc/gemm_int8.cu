@@ -33,6 +33,7 @@ constexpr int UMMA_K = 32;
 __host__ __device__ constexpr int epilogue_warps(int tokens) { return tokens >= 64 ? 8 : 4; }
 __host__ __device__ constexpr int block_threads(int tokens) { return 64 + 32 * epilogue_warps(tokens); }
 constexpr int MAX_K = 131071;
+constexpr int MAX_ROWS = 1 << 22;  // of weights: the grid's second dimension at 64 a block; coordinates and tile numbers stay far inside 32 bits
 
 // Instruction descriptor of kind::i8: signed 8-bit operands, both K-major, a 32-bit integer accumulator.
 __device__ __forceinline__ uint32_t instr_desc_s8(int m, int n)
@@ -223,8 +224,8 @@ __device__ __forceinline__ void finish_cut(TC* __restrict__ out, long long ld, c
 template <int BN, typename TC, bool GATED>
 __global__ void __launch_bounds__(block_threads(BN), 2)
 gemm_int8_few_kernel(const __grid_constant__ CUtensorMap map_w, const __grid_constant__ CUtensorMap map_a, const float* __restrict__ w_scale,
-                     const float* __restrict__ a_scale, TC* __restrict__ out, long long ld, int N, int M, int k_blocks, int splits, int tile_rows, int* status,
-                     const uint8_t* __restrict__ next_weights, long long next_bytes)
+                     const float* __restrict__ a_scale, TC* __restrict__ out, long long ld, int N, int M, int k_blocks, int splits, int tile_rows, int settled,
+                     int* status, const uint8_t* __restrict__ next_weights, long long next_bytes)
 {
     using T = Tile<BN>;
     extern __shared__ uint8_t smem_raw[];
@@ -265,7 +266,8 @@ gemm_int8_few_kernel(const __grid_constant__ CUtensorMap map_w, const __grid_con
     if (splits > 1 && (!T::MAIL_IN_RING || warp < 2)) cluster_arrive();
     if (warp == 0) {
         if (lane == 0) {
-            // the weights depend on no earlier kernel: their tiles for the first stages are requested before the wait for the kernels ahead in the stream
+            // settled weights depend on no earlier kernel: their tiles for the first stages are requested before the wait for the kernels ahead in the stream
+            if (!settled) pdl_wait();
             const int pre = min(num_kb, stages);
 #pragma unroll 1
             for (int i = 0; i < pre; ++i) {
@@ -304,6 +306,7 @@ gemm_int8_few_kernel(const __grid_constant__ CUtensorMap map_w, const __grid_con
             const uint32_t idesc = instr_desc_s8(BM, BN);
             int s = 0;
             uint32_t phase = 0;
+            pdl_wait();                       // the limit of the waits below is not for the kernels ahead
 #pragma unroll 1
             for (int i = 0; i < num_kb; ++i) {
                 if (!mbar_wait(full_bar + s, phase, abort_flag)) break;
@@ -329,8 +332,9 @@ gemm_int8_few_kernel(const __grid_constant__ CUtensorMap map_w, const __grid_con
         const int tokens = min(BN, M - y0), x_end = min(N, x0 + tile_rows);
         const int share = BM / splits, part = rank * share + (tid & (share - 1));        // K cut: the weight row that this thread finishes
         const int x = x0 + (splits > 1 ? part : row);
-        const float sw = x < x_end ? w_scale[x] : 0.f;
+        float sw = settled && x < x_end ? w_scale[x] : 0.f;
         pdl_wait();                           // the tokens' scales and the output belong to kernels ahead in the stream until here
+        if (!settled && x < x_end) sw = w_scale[x];
         if (tid < BN) sa[tid] = tid < tokens ? a_scale[y0 + tid] : 0.f;
         epilogue_barrier<T::WARPS>();
         // one lane asks for the warp: lanes that left the wait one by one would meet the warp-wide loads and barriers behind it apart
@@ -438,7 +442,7 @@ template <typename TC, bool GATED>
 __global__ void __launch_bounds__(PAIR_THREADS, 1)
 gemm_int8_pair_kernel(const __grid_constant__ CUtensorMap map_w, const __grid_constant__ CUtensorMap map_a, const float* __restrict__ w_scale,
                       const float* __restrict__ a_scale, TC* __restrict__ out, long long ld, int N, int M, int k_blocks, TokenTiles tokens, int num_tiles,
-                      int* status)
+                      int settled, int* status)
 {
     const int stages = pair_stages(tokens.rows), stage_bytes = pair_stage_bytes(tokens.rows);   // a lower tile's copies bring spare rows behind its own
     extern __shared__ uint8_t smem_raw[];
@@ -469,11 +473,12 @@ gemm_int8_pair_kernel(const __grid_constant__ CUtensorMap map_w, const __grid_co
     // The allocation is one for the pair.  Asked for before the other block runs it never comes back: without this barrier prompts of 640 tokens
     // through 36 layers, where a block's start can be held up by the many small blocks of a quantisation on its SM, stopped within some hundred steps.
     cluster_sync();   // both blocks run, and their barriers are initialised
-    // the weights of the first stages are requested beside the allocation and before the wait for the kernels ahead in the stream
+    // settled weights' first stages are requested beside the allocation and before the wait for the kernels ahead in the stream
     const int pre = min(k_blocks, stages);
     if (warp == 0) {
         if (lane == 0) {
             const int x0 = (cluster / tokens.count) * (2 * BM) + (int)rank * BM;
+            if (!settled) pdl_wait();
             for (int i = 0; i < pre; ++i) {
                 if (rank == 0) mbar_expect_tx(full_bar + i, 2u * stage_bytes);     // both blocks' bytes
                 tma_load_2d_pair(smem_u32(tiles + (size_t)i * stage_bytes), &map_w, i * BK, x0, map_to_rank(smem_u32(full_bar + i), 0));
@@ -523,6 +528,7 @@ gemm_int8_pair_kernel(const __grid_constant__ CUtensorMap map_w, const __grid_co
             uint32_t phase = 0;
             int i = 0;
             bool ok = true;
+            pdl_wait();       // the limit of the waits below is not for the kernels ahead
             for (int tile = cluster; ok && tile < num_tiles; tile += clusters, ++i) {
                 const uint32_t idesc = instr_desc_s8(2 * BM, tokens.height(tile % tokens.count));
                 const int buf = i & 1;
@@ -668,7 +674,7 @@ static Plan choose(int M, int N, int K)
         for (int splits = 1; splits <= 8 && (splits == 1 || k_blocks >= 2 * splits); splits *= 2) {
             for (int rows = BM; rows >= (splits == 1 ? 64 : BM); rows -= 32) {      // weight rows of a multiple of what a warp reads out
                 const double t = few_time(M, N, k_blocks, bn, splits, rows, sms);
-                if (t < least && (N + rows - 1) / rows <= 65535) {
+                if (t < least && (N + rows - 1) / rows <= 65535) {       // the launch's limit
                     least = t;
                     best = {false, 0, bn, splits, rows};
                 }
@@ -677,7 +683,7 @@ static Plan choose(int M, int N, int K)
     }
     if (M < 64) return best;
     const int lowest = (M + 255) / 256, runs = (M + 31) / 32;
-    for (int count = lowest; count <= runs && count <= 2 * lowest + 2; ++count) {
+    for (int count = lowest; count <= runs && count <= 2 * lowest + 2 && count <= lowest + 16; ++count) {
         const double t = pair_time(M, N, k_blocks, count, sms);
         if (t < least) {
             least = t;
@@ -689,7 +695,7 @@ static Plan choose(int M, int N, int K)
 
 template <int BN, typename TC, bool GATED>
 static int launch_few(const Plan& p, const CUtensorMap& mw, const CUtensorMap& ma, const float* w_scale, const float* a_scale, void* C, long long ldc, int M,
-                      int N, int k_blocks, int* status, cudaStream_t stream, const void* next_weights, long long next_bytes)
+                      int N, int k_blocks, int settled, int* status, cudaStream_t stream, const void* next_weights, long long next_bytes)
 {
     using T = Tile<BN>;
     auto kernel = gemm_int8_few_kernel<BN, TC, GATED>;
@@ -697,20 +703,19 @@ static int launch_few(const Plan& p, const CUtensorMap& mw, const CUtensorMap& m
         SPY_CUDA(cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)T::SMEM));
     }
     const dim3 grid((unsigned)((M + BN - 1) / BN * p.splits), (unsigned)((N + p.tile_rows - 1) / p.tile_rows));
-    if (grid.y > 65535) SPY_FAIL("gemm_int8: %u weight tiles exceed the launch limits", grid.y);   // beyond 8 million outputs
     if (p.splits == 1)
-        spy_launch(kernel, grid, dim3(T::THREADS), T::SMEM, stream, mw, ma, w_scale, a_scale, (TC*)C, ldc, N, M, k_blocks, p.splits, p.tile_rows, status,
-                   (const uint8_t*)next_weights, next_bytes);
+        spy_launch(kernel, grid, dim3(T::THREADS), T::SMEM, stream, mw, ma, w_scale, a_scale, (TC*)C, ldc, N, M, k_blocks, p.splits, p.tile_rows, settled,
+                   status, (const uint8_t*)next_weights, next_bytes);
     else
         spy_launch_cluster(kernel, grid, dim3(T::THREADS), T::SMEM, stream, (unsigned)p.splits, mw, ma, w_scale, a_scale, (TC*)C, ldc, N, M, k_blocks,
-                           p.splits, p.tile_rows, status, (const uint8_t*)next_weights, next_bytes);
+                           p.splits, p.tile_rows, settled, status, (const uint8_t*)next_weights, next_bytes);
     SPY_CHECK_LAUNCH("gemm_int8");
     return 0;
 }
 
 template <typename TC, bool GATED>
 static int launch_pairs(const Plan& p, const CUtensorMap& mw, const CUtensorMap& ma, const float* w_scale, const float* a_scale, void* C, long long ldc, int M,
-                        int N, int k_blocks, const TokenTiles& tokens, int* status, cudaStream_t stream)
+                        int N, int k_blocks, const TokenTiles& tokens, int settled, int* status, cudaStream_t stream)
 {
     auto kernel = gemm_int8_pair_kernel<TC, GATED>;
     static int clusters_of_device[SPY_MAX_DEVICES] = {};
@@ -738,14 +743,14 @@ static int launch_pairs(const Plan& p, const CUtensorMap& mw, const CUtensorMap&
     if (num_tiles > 0x7fffffffLL) SPY_FAIL("gemm_int8: %lld tiles exceed the kernel's range", num_tiles);
     const int clusters = (int)(num_tiles < clusters_max ? num_tiles : clusters_max);
     spy_launch_cluster(kernel, dim3(2 * clusters), dim3(PAIR_THREADS), PAIR_SMEM, stream, 2u, mw, ma, w_scale, a_scale, (TC*)C, ldc, N, M, k_blocks, tokens,
-                       (int)num_tiles, status);
+                       (int)num_tiles, settled, status);
     SPY_CHECK_LAUNCH("gemm_int8 (pairs)");
     return 0;
 }
 
 template <typename TC, bool GATED>
 static int run(const void* A, long long lda, const float* a_scale, const void* W, long long ldw, const float* w_scale, void* C, long long ldc, int M, int N,
-               int K, int* status, cudaStream_t stream, const void* next_weights, long long next_bytes)
+               int K, int settled, int* status, cudaStream_t stream, const void* next_weights, long long next_bytes)
 {
     const Plan p = choose(M, N, K);
     const int k_blocks = (K + BK - 1) / BK;
@@ -753,22 +758,23 @@ static int run(const void* A, long long lda, const float* a_scale, const void* W
     if (p.pairs) {
         const TokenTiles tokens = token_tiles(M, p.count);
         if (make_map(&mw, W, N, K, ldw, BM) || make_map(&ma, A, M, K, lda, tokens.rows / 2)) return 1;
-        return launch_pairs<TC, GATED>(p, mw, ma, w_scale, a_scale, C, ldc, M, N, k_blocks, tokens, status, stream);
+        return launch_pairs<TC, GATED>(p, mw, ma, w_scale, a_scale, C, ldc, M, N, k_blocks, tokens, settled, status, stream);
     }
     if (make_map(&mw, W, N, K, ldw, p.tile_rows) || make_map(&ma, A, M, K, lda, p.bn)) return 1;
-    if (p.bn == 16) return launch_few<16, TC, GATED>(p, mw, ma, w_scale, a_scale, C, ldc, M, N, k_blocks, status, stream, next_weights, next_bytes);
-    if (p.bn == 32) return launch_few<32, TC, GATED>(p, mw, ma, w_scale, a_scale, C, ldc, M, N, k_blocks, status, stream, next_weights, next_bytes);
-    if (p.bn == 64) return launch_few<64, TC, GATED>(p, mw, ma, w_scale, a_scale, C, ldc, M, N, k_blocks, status, stream, next_weights, next_bytes);
-    return launch_few<128, TC, GATED>(p, mw, ma, w_scale, a_scale, C, ldc, M, N, k_blocks, status, stream, next_weights, next_bytes);
+    if (p.bn == 16) return launch_few<16, TC, GATED>(p, mw, ma, w_scale, a_scale, C, ldc, M, N, k_blocks, settled, status, stream, next_weights, next_bytes);
+    if (p.bn == 32) return launch_few<32, TC, GATED>(p, mw, ma, w_scale, a_scale, C, ldc, M, N, k_blocks, settled, status, stream, next_weights, next_bytes);
+    if (p.bn == 64) return launch_few<64, TC, GATED>(p, mw, ma, w_scale, a_scale, C, ldc, M, N, k_blocks, settled, status, stream, next_weights, next_bytes);
+    return launch_few<128, TC, GATED>(p, mw, ma, w_scale, a_scale, C, ldc, M, N, k_blocks, settled, status, stream, next_weights, next_bytes);
 }
 
 }  // namespace
 
 // A [M, K] and W [N, K] int8, rows lda / ldw bytes apart (multiples of 16); a_scale [M], w_scale [N]; C [M, N] of c_dtype, rows ldc elements apart.
 // gated: W's rows alternate gate and up rows, C is [M, N / 2] bfloat16.  status: null, or two ints that receive a code if a bounded wait runs out.
+// settled: no kernel that may still run writes W or w_scale; they are then read ahead of the wait for the kernels before this one.
 // next_weights / next_bytes (may be null / 0): memory that a later kernel of the stream will read, which the kernel for few tokens asks to be brought into L2.
 extern "C" int spy_gemm_int8(const void* A, long long lda, const float* a_scale, const void* W, long long ldw, const float* w_scale, void* C, int c_dtype,
-                             long long ldc, int M, int N, int K, int gated, int* status, cudaStream_t stream, const void* next_weights,
+                             long long ldc, int M, int N, int K, int gated, int settled, int* status, cudaStream_t stream, const void* next_weights,
                              long long next_bytes)
 {
     if (next_weights == nullptr || next_bytes <= 0 || (reinterpret_cast<uintptr_t>(next_weights) & 15)) {
@@ -776,12 +782,13 @@ extern "C" int spy_gemm_int8(const void* A, long long lda, const float* a_scale,
         next_bytes = 0;
     }
     if (M <= 0 || N <= 0) return 0;
+    if (M > MAX_ROWS || N > MAX_ROWS) SPY_FAIL("gemm_int8: %d x %d results: at most %d a side", M, N, MAX_ROWS);
     if (K <= 0 || K > MAX_K) SPY_FAIL("gemm_int8: K %d must lie in 1..%d (32-bit sums)", K, MAX_K);
     if (lda % 16 != 0 || ldw % 16 != 0) SPY_FAIL("gemm_int8: row distances %lld/%lld must be multiples of 16 bytes", lda, ldw);
     if ((reinterpret_cast<uintptr_t>(A) & 15) || (reinterpret_cast<uintptr_t>(W) & 15)) SPY_FAIL("gemm_int8: operands must be 16-byte aligned");
     if (gated && (N % 2 != 0 || c_dtype != SPY_BF16)) SPY_FAIL("gemm_int8: the gated epilogue needs an even N and bfloat16 output");
-    if (gated) return run<bf16, true>(A, lda, a_scale, W, ldw, w_scale, C, ldc, M, N, K, status, stream, next_weights, next_bytes);
-    if (c_dtype == SPY_BF16) return run<bf16, false>(A, lda, a_scale, W, ldw, w_scale, C, ldc, M, N, K, status, stream, next_weights, next_bytes);
-    if (c_dtype == SPY_F32) return run<float, false>(A, lda, a_scale, W, ldw, w_scale, C, ldc, M, N, K, status, stream, next_weights, next_bytes);
+    if (gated) return run<bf16, true>(A, lda, a_scale, W, ldw, w_scale, C, ldc, M, N, K, settled, status, stream, next_weights, next_bytes);
+    if (c_dtype == SPY_BF16) return run<bf16, false>(A, lda, a_scale, W, ldw, w_scale, C, ldc, M, N, K, settled, status, stream, next_weights, next_bytes);
+    if (c_dtype == SPY_F32) return run<float, false>(A, lda, a_scale, W, ldw, w_scale, C, ldc, M, N, K, settled, status, stream, next_weights, next_bytes);
     SPY_FAIL("gemm_int8: unknown output dtype code %d", c_dtype);
 }

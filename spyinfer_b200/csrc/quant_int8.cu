@@ -20,6 +20,7 @@ SPY_MODULE(spy_quant_int8)
 
 namespace {
 
+constexpr int STATUS_BAD_ROW = 5;      // beside the codes of common.cuh
 constexpr float MAGIC = 12582912.0f;   // 1.5 * 2^23: added to a small number it leaves the nearest integer in the low bits
 
 __device__ __forceinline__ void load8(const float* p, float (&v)[8])
@@ -261,15 +262,30 @@ __global__ void __launch_bounds__(1024) quantize_long_kernel(const T* __restrict
 template <typename TX, typename TD, typename TW, bool WHOLE, int GROUPS>
 __global__ void __launch_bounds__(1024) rmsnorm_int8_kernel(TX* x, const TD* __restrict__ delta, int splits, long long split_stride, const int* __restrict__ rows,
                                                             const TW* __restrict__ w, int8_t* __restrict__ codes, long long ldc,
-                                                            float* __restrict__ scales, int len, float eps, int write_back)
+                                                            float* __restrict__ scales, int total, int len, float eps, int write_back, int settled, int* status)
 {
     __shared__ uint32_t part[64];
     pdl_launch_dependents();
-    // few rows: the weight, which depends on no kernel ahead in the stream, is loaded before the wait for them
+    // a settled weight depends on no kernel ahead in the stream: it is loaded before the wait for them (a row of 4,096: 2.1 us, behind it 2.4)
     float w_first[8];
-    if constexpr (GROUPS == 1) fetch<WHOLE>(w, 0, len, w_first);
+    if constexpr (GROUPS == 1) {
+        if (settled) fetch<WHOLE>(w, 0, len, w_first);
+    }
     pdl_wait();
-    const int src = rows ? rows[blockIdx.x] : blockIdx.x;
+    if constexpr (GROUPS == 1) {
+        if (!settled) fetch<WHOLE>(w, 0, len, w_first);
+    }
+    int src = blockIdx.x;
+    if (rows) src = rows[blockIdx.x];
+    if (rows && (src < 0 || src >= total)) {         // no row of x: nothing is read, the result is not a number
+#pragma unroll
+        for (int g = 0; g < GROUPS; ++g) put_codes<WHOLE>(codes + (size_t)blockIdx.x * ldc, g, len, make_uint2(0, 0));
+        if (threadIdx.x == 0) {
+            scales[blockIdx.x] = __int_as_float(0x7fc00000);
+            report_status(status, STATUS_BAD_ROW, blockIdx.x);
+        }
+        return;
+    }
     TX* xr = x + (size_t)src * len;
     const TD* dr = delta ? delta + (size_t)src * len : nullptr;
     float v[GROUPS][8];
@@ -346,7 +362,7 @@ static int quantize(const T* x, long long ldx, int8_t* codes, long long ldc, flo
 
 template <typename TX, typename TD, typename TW>
 static int norm(TX* x, const TD* delta, int splits, long long split_stride, const int* rows, const TW* w, int8_t* codes, long long ldc, float* scales,
-                int n, int len, float eps, int write_back, cudaStream_t stream)
+                int total, int n, int len, float eps, int write_back, int settled, int* status, cudaStream_t stream)
 {
     const bool whole = len % 8 == 0 && aligned16(x) && aligned16(delta) && aligned16(w) && split_stride * (long long)sizeof(TD) % 16 == 0;
     // us with 1 / 2 / 4 groups a thread.  Whole rows: 64 x 5,120 3.0 / 3.1 / 3.3, 512 x 4,096 5.7 / 5.7 / 8.4, 4,096 x 5,120 36.5 / 38.1 / 42.1 (a norm with a
@@ -354,8 +370,8 @@ static int norm(TX* x, const TD* delta, int splits, long long split_stride, cons
     const int groups = row_groups(len, whole || n < 512 ? 1 : 2);
     auto kernel = whole ? (groups == 4 ? rmsnorm_int8_kernel<TX, TD, TW, true, 4> : groups == 2 ? rmsnorm_int8_kernel<TX, TD, TW, true, 2> : rmsnorm_int8_kernel<TX, TD, TW, true, 1>)
                         : (groups == 4 ? rmsnorm_int8_kernel<TX, TD, TW, false, 4> : groups == 2 ? rmsnorm_int8_kernel<TX, TD, TW, false, 2> : rmsnorm_int8_kernel<TX, TD, TW, false, 1>);
-    spy_launch(kernel, dim3(n), dim3(row_threads(len, groups)), 0, stream, x, delta, splits, split_stride, rows, w, codes, ldc, scales, len, eps,
-               write_back);
+    spy_launch(kernel, dim3(n), dim3(row_threads(len, groups)), 0, stream, x, delta, splits, split_stride, rows, w, codes, ldc, scales, total, len, eps,
+               write_back, settled, status);
     SPY_CHECK_LAUNCH("rmsnorm_int8");
     return 0;
 }
@@ -378,11 +394,13 @@ extern "C" int spy_quantize_int8(const void* x, int dtype, long long ldx, int8_t
     return 0;
 }
 
-// x: [*, len] of x_dtype; delta: null or `splits` stacked [*, len] arrays of delta_dtype, split_stride elements apart, added to x in order;
-// rows: null or n row indices (gather); w: [len] of w_dtype; codes and scales as above.  write_back stores the sum into x and needs rows == null.
+// x: [total, len] of x_dtype; delta: null or `splits` stacked [*, len] arrays of delta_dtype, split_stride elements apart, added to x in order;
+// rows: null or n row indices (gather), one outside x gives a row that is not a number
+// and is reported in status (null, or two ints); w: [len] of w_dtype (settled: no
+// kernel that may still run writes it); codes and scales as above.  write_back stores the sum into x and needs rows == null.
 extern "C" int spy_rmsnorm_int8(void* x, int x_dtype, const void* delta, int delta_dtype, int splits, long long split_stride, const int* rows,
-                                const void* w, int w_dtype, int8_t* codes, long long ldc, float* scales, int n, int len, float eps, int write_back,
-                                cudaStream_t stream)
+                                const void* w, int w_dtype, int8_t* codes, long long ldc, float* scales, int total, int n, int len, float eps,
+                                int write_back, int settled, int* status, cudaStream_t stream)
 {
     if (n <= 0) return 0;
     if (int rc = check_codes("rmsnorm_int8", codes, ldc, len)) return rc;
@@ -393,7 +411,7 @@ extern "C" int spy_rmsnorm_int8(void* x, int x_dtype, const void* delta, int del
     SPY_DISPATCH_DTYPE(x_dtype, TX, {
         SPY_DISPATCH_DTYPE(delta_dtype, TD, {
             SPY_DISPATCH_DTYPE(w_dtype, TW, {
-                return norm<TX, TD, TW>((TX*)x, (const TD*)delta, splits, split_stride, rows, (const TW*)w, codes, ldc, scales, n, len, eps, write_back, stream);
+                return norm<TX, TD, TW>((TX*)x, (const TD*)delta, splits, split_stride, rows, (const TW*)w, codes, ldc, scales, total, n, len, eps, write_back, settled, status, stream);
             })
         })
     })

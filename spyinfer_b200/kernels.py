@@ -22,6 +22,7 @@ STATUS_MESSAGES = {
     2: "a position beyond the position table (batch token index {detail})",
     3: "a block-table entry that is no page of the pool (batch token index {detail})",
     4: "a wait inside it ran out of its time limit (code {detail})",
+    5: "a row index outside the matrix it gathers from (entry {detail})",
 }
 STATUS_WAIT_TIMEOUT = 4
 
@@ -2126,8 +2127,8 @@ class _Kernel:
 
 _P, _L, _I, _F = ctypes.c_void_p, ctypes.c_longlong, ctypes.c_int, ctypes.c_float
 _quantize_int8 = _Kernel("quant_int8", "spy_quantize_int8", _P, _I, _L, _P, _L, _P, _I, _I, _P)
-_rmsnorm_int8 = _Kernel("quant_int8", "spy_rmsnorm_int8", _P, _I, _P, _I, _I, _L, _P, _P, _I, _P, _L, _P, _I, _I, _F, _I, _P)
-_gemm_int8 = _Kernel("gemm_int8", "spy_gemm_int8", _P, _L, _P, _P, _L, _P, _P, _I, _L, _I, _I, _I, _I, _P, _P, _P, _L)
+_rmsnorm_int8 = _Kernel("quant_int8", "spy_rmsnorm_int8", _P, _I, _P, _I, _I, _L, _P, _P, _I, _P, _L, _P, _I, _I, _I, _F, _I, _I, _P, _P)
+_gemm_int8 = _Kernel("gemm_int8", "spy_gemm_int8", _P, _L, _P, _P, _L, _P, _P, _I, _L, _I, _I, _I, _I, _I, _P, _P, _P, _L)
 
 
 def _on_current_device(t: torch.Tensor, what: str) -> int:
@@ -2174,6 +2175,8 @@ def quantize_int8(x: torch.Tensor, out: Optional[Int8Rows] = None) -> Int8Rows:
     ldx = _check_weight(x, "quantize_int8 input")
     device = _on_current_device(x, "quantize_int8 input")
     n, length = x.shape
+    if n > 0x7fffffff or length > 0x7fffffff:
+        raise KernelError(f"quantize_int8 input: {tuple(x.shape)} exceeds 31 bits")
     if n > 1 and ldx < length:
         raise KernelError(f"quantize_int8 input: rows overlap (strides {x.stride()} for shape {tuple(x.shape)})")
     if out is None:
@@ -2188,15 +2191,18 @@ def quantize_int8(x: torch.Tensor, out: Optional[Int8Rows] = None) -> Int8Rows:
 
 
 def rmsnorm_int8(x: torch.Tensor, weight: torch.Tensor, eps: float, out: Optional[Int8Rows] = None, delta: Optional[torch.Tensor] = None,
-                 rows: Optional[torch.Tensor] = None, write_back: bool = False) -> Int8Rows:
+                 rows: Optional[torch.Tensor] = None, write_back: bool = False, weight_settled: bool = False) -> Int8Rows:
     """``rmsnorm(x [+ delta]) * weight`` row by row as ``rmsnorm`` has it, the result in 8 bits for ``gemm_int8``.  The row that is quantised is ``y = (x + delta)
     * weight`` in 32 bits: ``code`` is the integer nearest to ``127 y / max |y|`` (as ``quantize_int8``), and the scale ``max |y| / 127 / sqrt(mean((x + delta)^2)
     + eps)``.  ``delta``: x's shape, or a stack ``[splits, rows, len]`` of partial sums that are added in order; ``write_back`` stores the sum into ``x``; ``rows``
-    gathers rows of x (and delta).  Rows of up to 32,768 elements."""
+    gathers rows of x (and delta); an index outside x gives codes 0 and the scale NaN and is reported in the status word.  Rows of up to 32,768 elements.
+    ``weight_settled=True``: as ``gemm_int8``'s ``w_settled``, for ``weight``."""
     _check(x, "rmsnorm_int8 input", ndim=2)
     device = _on_current_device(x, "rmsnorm_int8 input")
     _check(weight, "rmsnorm_int8 weight", ndim=1)
     n, H = x.shape
+    if n > 0x7fffffff or H > 0x7fffffff:
+        raise KernelError(f"rmsnorm_int8 input: {tuple(x.shape)} exceeds 31 bits")
     if weight.shape[0] != H:
         raise KernelError(f"rmsnorm_int8: row lengths differ: input {H}, weight {weight.shape[0]}")
     delta, splits, split_stride = _stack_of(delta, x, "rmsnorm_int8 delta")
@@ -2217,21 +2223,26 @@ def rmsnorm_int8(x: torch.Tensor, weight: torch.Tensor, eps: float, out: Optiona
         got, width, pitch, codes, scales = _int8_layout(out, "rmsnorm_int8 output", device)
         if (got, width) != (n, H):
             raise KernelError(f"rmsnorm_int8 output: expected {(n, H)}, found {(got, width)}")
+    status = _int8_status_word(device).data_ptr() if rows is not None else 0
     _rmsnorm_int8(x.data_ptr(), _code(x, "rmsnorm_int8 input"), delta.data_ptr() if delta is not None else 0,
                   _code(delta, "rmsnorm_int8 delta") if delta is not None else 0, splits, split_stride, rows.data_ptr() if rows is not None else 0,
-                  weight.data_ptr(), _code(weight, "rmsnorm_int8 weight"), codes, pitch, scales, n, H, eps, 1 if write_back else 0, _raw_stream(device))
+                  weight.data_ptr(), _code(weight, "rmsnorm_int8 weight"), codes, pitch, scales, x.shape[0], n, H, eps, 1 if write_back else 0, 1 if weight_settled else 0, status, _raw_stream(device))
     return out
 
 
 def gemm_int8(a: Int8Rows, w: Int8Rows, out: Optional[torch.Tensor] = None, status: Optional[torch.Tensor] = None, out_dtype: Optional[torch.dtype] = None,
-              epilogue: Optional[str] = None, prefetch: Optional[torch.Tensor] = None, prefetch_bytes: int = 0) -> torch.Tensor:
+              epilogue: Optional[str] = None, prefetch: Optional[torch.Tensor] = None, prefetch_bytes: int = 0,
+              w_settled: bool = False) -> torch.Tensor:
     """``a [M, K] @ w [N, K]^T`` of 8-bit rows on the tensor cores, ``(sum_k a w) * a.scales[m] * w.scales[n]`` with the sum in 32-bit integers (exact; K below
     131,072), in bfloat16 (default) or float32.  ``epilogue="swiglu"``: ``w``'s rows alternate gate and up rows and the result is ``silu(gate) * up``,
     ``[M, N / 2]`` bfloat16.  A row whose scale is NaN gives a row of NaN.  A token's result does not depend on the rest of the batch.
-    ``prefetch``, ``prefetch_bytes``: as ``gemm_tcgen05`` has them."""
+    ``prefetch``, ``prefetch_bytes``: as ``gemm_tcgen05`` has them.  ``w_settled=True`` says that no kernel that may still be running when this one is
+    launched writes ``w`` (a model's weights): its first tiles are then requested while the kernels ahead finish.  Not for a ``w`` that was quantised just before."""
     M, K, lda, a_codes, a_scales = _int8_layout(a, "gemm_int8 input")
     device = a.codes.get_device()
     N, k_of_w, ldw, w_codes, w_scales = _int8_layout(w, "gemm_int8 weight", device)
+    if max(M, N, K) > 0x7fffffff:
+        raise KernelError(f"gemm_int8: input {(M, K)}, weight {(N, k_of_w)} exceed 31 bits")
     if k_of_w != K:
         raise KernelError(f"gemm_int8: shapes do not fit: input {(M, K)}, weight {(N, k_of_w)}")
     if epilogue is not None and epilogue != "swiglu":
@@ -2244,22 +2255,31 @@ def gemm_int8(a: Int8Rows, w: Int8Rows, out: Optional[torch.Tensor] = None, stat
         if out.shape != (M, n_out) or out.get_device() != device:
             raise KernelError(f"gemm_int8: output {tuple(out.shape)} on {out.device} does not fit [{M}, {n_out}] on cuda:{device}")
     if status is None:
-        status = _int8_status.get(device)
-        if status is None:
-            # the word must not come from a captured graph's memory
-            if torch.cuda.is_current_stream_capturing() and str(a.codes.device) not in _status_words:
-                raise KernelError("gemm_int8: the device's status word does not exist yet: make one call (or status_word()) before the capture, or give a status")
-            status = _int8_status[device] = status_word(a.codes.device)
+        status = _int8_status_word(device)
     next_at = next_bytes = 0
     if prefetch is not None and M <= 256:
         if prefetch.get_device() != device:
             raise KernelError(f"gemm_int8: the tensor to prefetch lies on {prefetch.device}, the operands on cuda:{device}")
+        if not prefetch.is_contiguous():
+            _check_weight(prefetch, "gemm_int8 prefetch")
+            if prefetch.stride(0) < prefetch.shape[1]:
+                raise KernelError("gemm_int8: the tensor to prefetch has overlapping rows")
         next_at, next_bytes = prefetch.data_ptr(), prefetch.numel() * prefetch.element_size()
         if prefetch_bytes > 0:
             next_bytes = min(next_bytes, prefetch_bytes)
     _gemm_int8(a_codes, lda, a_scales, w_codes, ldw, w_scales, out.data_ptr(), _code(out, "gemm_int8 output"), n_out, M, N, K, 1 if epilogue else 0,
-               status.data_ptr(), _raw_stream(device), next_at, next_bytes)
+               1 if w_settled else 0, status.data_ptr(), _raw_stream(device), next_at, next_bytes)
     return out
 
 
 _int8_status = {}        # device index -> its status word
+
+
+def _int8_status_word(device: int) -> torch.Tensor:
+    status = _int8_status.get(device)
+    if status is None:
+        # the word must not come from a captured graph's memory
+        if torch.cuda.is_current_stream_capturing() and f"cuda:{device}" not in _status_words:
+            raise KernelError("the device's status word does not exist yet: make one call (or status_word()) before the capture, or give a status")
+        status = _int8_status[device] = status_word(torch.device("cuda", device))
+    return status

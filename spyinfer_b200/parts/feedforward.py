@@ -121,7 +121,7 @@ class GatedMLP(FeedForward):
         if self.leave_output_bias:           # the consumer adds it (and may then take the down product's split-K parts unsummed)
             self.output_bias, down_bias = down_bias, None
         self.down = linear_for(self.ctx, tensors[p + n["down"]], bias=down_bias)
-        self.gate_up.hint_next = not self.fused       # fused: the down product follows at once
+        self.gate_up.hint_next = not self.fused or self.ctx.quantization == "int8"       # fused: the down product follows at once, but for a quantisation
 
     def linears(self):
         return [self.gate_up, self.down]

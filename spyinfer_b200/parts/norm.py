@@ -59,7 +59,8 @@ class RMSNorm(Norm):
 
     def forward_add(self, residual, delta, rows=None, out_dtype=None):
         if self.emits_int8:
-            return kernels.rmsnorm_int8(residual, self.weight, self.eps, delta=delta, rows=rows, write_back=delta is not None and rows is None)
+            return kernels.rmsnorm_int8(residual, self.weight, self.eps, delta=delta, rows=rows, write_back=delta is not None and rows is None,
+                                        weight_settled=True)
         n = residual.shape[0] if rows is None else rows.shape[0]
         out = torch.empty((n, self.size), dtype=out_dtype or self.ctx.dtype, device=residual.device)
         return kernels.rmsnorm(residual, self.weight, self.eps, out, delta=delta, rows=rows, write_back=delta is not None and rows is None)

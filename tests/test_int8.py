@@ -296,6 +296,82 @@ def test_a_feed_forward(M):
 
 
 @gpu
+@pytest.mark.parametrize("M,N,K", [(1, 4096, 4096), (40, 2048, 1024), (300, 9472, 512), (2, 40000, 256)])
+def test_weights_quantised_by_the_call_ahead(M, N, K):
+    """A product may follow the quantisation of its weight at once: it reads nothing of it before that has ended.  Every round has other weights in the
+    same memory, so that what an earlier round left would show."""
+    x = wild_rows(M, K, 1).to(torch.bfloat16)
+    w = kernels.empty_int8(N, K, DEV)
+    weights = [torch.randn(N, K, device=DEV).to(torch.bfloat16) * (i + 1) for i in range(4)]
+    outs = []
+    for i in range(12):
+        kernels.quantize_int8(weights[i % 4], w)
+        outs.append(kernels.gemm_int8(kernels.quantize_int8(x), w, out_dtype=torch.float32))
+    for i in range(4):
+        kernels.quantize_int8(weights[i], w)
+        a = kernels.quantize_int8(x)
+        torch.cuda.synchronize()
+        check_product(outs[i], product_of(a, w), torch.float32)
+        assert torch.equal(outs[i], outs[i + 4]) and torch.equal(outs[i], outs[i + 8])
+        assert torch.equal(outs[i], kernels.gemm_int8(a, w, out_dtype=torch.float32, w_settled=True, prefetch=weights[0]))
+
+
+@gpu
+def test_gather_of_rows_that_there_are_not():
+    """An index outside the stream reads nothing: its row is not a number, the others are as they are, and the status word says so."""
+    x, w = wild_rows(5, 264, 1), torch.ones(264, device=DEV)
+    rows = torch.tensor([4, -1, 0, 5, 2 ** 31 - 1, 2], dtype=torch.int32, device=DEV)
+    kernels.status_word(torch.device(DEV)).zero_()
+    got = kernels.rmsnorm_int8(x, w, 1e-6, rows=rows)
+    good = torch.tensor([0, 2, 5], device=DEV)
+    want = kernels.rmsnorm_int8(x, w, 1e-6)
+    assert torch.equal(got.codes[good], want.codes[torch.tensor([4, 0, 2], device=DEV)]) and torch.equal(got.scales[good], want.scales[torch.tensor([4, 0, 2], device=DEV)])
+    bad = torch.tensor([1, 3, 4], device=DEV)
+    assert bool(torch.isnan(got.scales[bad]).all()) and int(got.codes[bad].abs().max()) == 0
+    status = kernels.status_word(torch.device(DEV))
+    assert status[0].item() == 5 and status[1].item() in (1, 3, 4)
+    status.zero_()
+
+
+@gpu
+def test_two_streams_at_once():
+    """Nothing is shared between calls: products, norms and quantisations on two streams side by side give what they give alone."""
+    sides = [torch.cuda.Stream(), torch.cuda.Stream()]
+    jobs = []
+    for i, (M, N, K) in enumerate(((9, 6144, 2048), (700, 4096, 1024))):
+        x, d, g = wild_rows(M, K, i), wild_rows(M, K, i + 5).to(torch.bfloat16), torch.ones(K, device=DEV)
+        w = kernels.quantize_int8(torch.randn(N, K, device=DEV).to(torch.bfloat16))
+        jobs.append((x, d, g, w))
+
+    def run(job):
+        x, d, g, w = job
+        rows = kernels.rmsnorm_int8(x, g, 1e-6, delta=d)
+        y = kernels.gemm_int8(rows, w)
+        return kernels.quantize_int8(y)
+
+    alone = [run(j) for j in jobs]
+    torch.cuda.synchronize()
+    got = [[], []]
+    for _ in range(20):
+        for i, side in enumerate(sides):
+            with torch.cuda.stream(side):
+                got[i].append(run(jobs[i]))
+    torch.cuda.synchronize()
+    for i in range(2):
+        assert all(torch.equal(r.codes, alone[i].codes) and torch.equal(r.scales, alone[i].scales) for r in got[i])
+
+
+@gpu
+def test_tensors_of_another_device_than_the_current_one(monkeypatch):
+    """The launch goes to the current device's stream: tensors that lie elsewhere are refused."""
+    a, w, x = rows_of_codes(4, 48, 1), rows_of_codes(6, 48, 2), torch.randn(4, 48, device=DEV)
+    monkeypatch.setattr(torch.cuda, "current_device", lambda: 1)
+    for call in (lambda: kernels.gemm_int8(a, w), lambda: kernels.quantize_int8(x), lambda: kernels.rmsnorm_int8(x, torch.ones(48, device=DEV), 1e-6)):
+        with pytest.raises(KernelError, match="current device"):
+            call()
+
+
+@gpu
 def test_no_rows_and_no_outputs():
     a, w = kernels.empty_int8(0, 48, DEV), rows_of_codes(20, 48, 1)
     assert tuple(kernels.gemm_int8(a, w).shape) == (0, 20)
@@ -328,6 +404,8 @@ def test_refusals():
             (lambda: kernels.gemm_int8(a, w, epilogue="swiglu", out_dtype=torch.float32), "bfloat16 output"),
             (lambda: kernels.gemm_int8(a, w, out=torch.empty(4, 5, device=DEV)), "does not fit"),
             (lambda: kernels.gemm_int8(a, w, out_dtype=torch.float16), "float32 or bfloat16"),
+            (lambda: kernels.gemm_int8(a, w, prefetch=x[:1].expand(4, 48)), "overlapping"),
+            (lambda: kernels.gemm_int8(a, w, prefetch=x.cpu()), "prefetch lies on"),
             (lambda: kernels.gemm_int8(kernels.empty_int8(1, 131072, DEV), kernels.empty_int8(1, 131072, DEV)), "131071"),
             (lambda: kernels.gemm_int8(kernels.empty_int8(2, 0, DEV), kernels.empty_int8(2, 0, DEV)), "must lie in"),
             (lambda: kernels.quantize_int8(x.half()), "float32 or bfloat16"),
