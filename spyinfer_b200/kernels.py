@@ -2236,8 +2236,9 @@ def gemm_int8(a: Int8Rows, w: Int8Rows, out: Optional[torch.Tensor] = None, stat
     """``a [M, K] @ w [N, K]^T`` of 8-bit rows on the tensor cores, ``(sum_k a w) * a.scales[m] * w.scales[n]`` with the sum in 32-bit integers (exact; K below
     131,072), in bfloat16 (default) or float32.  ``epilogue="swiglu"``: ``w``'s rows alternate gate and up rows and the result is ``silu(gate) * up``,
     ``[M, N / 2]`` bfloat16.  A row whose scale is NaN gives a row of NaN.  A token's result does not depend on the rest of the batch.
-    ``prefetch``, ``prefetch_bytes``: as ``gemm_tcgen05`` has them.  ``w_settled=True`` says that no kernel that may still be running when this one is
-    launched writes ``w`` (a model's weights): its first tiles are then requested while the kernels ahead finish.  Not for a ``w`` that was quantised just before."""
+    ``prefetch``, ``prefetch_bytes``: as ``gemm_tcgen05`` has them.  ``w_settled=True`` says that what writes ``w`` has ended before this launch
+    (a model's weights, once the host has waited for their quantisation): its first tiles are then requested while the kernels ahead finish.  Not for a ``w``
+    whose quantisation may still run: kernels overlap several deep, so one launch in between does not part them."""
     M, K, lda, a_codes, a_scales = _int8_layout(a, "gemm_int8 input")
     device = a.codes.get_device()
     N, k_of_w, ldw, w_codes, w_scales = _int8_layout(w, "gemm_int8 weight", device)

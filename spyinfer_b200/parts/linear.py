@@ -113,7 +113,8 @@ class Int8Linear:
             raise ValueError(f"a bias of shape {tuple(bias.shape)} does not fit a weight of shape {tuple(weight.shape)}")
         self.rows, self.bias = kernels.quantize_int8(weight), bias
         self.weight = self.rows.codes               # what the product ahead asks for ahead of time
-        self.settled = False                        # the first call may follow the quantisation; its wait for the kernels ahead covers all later ones
+        # a product asks for its weight ahead of the kernels before it, which may not include the quantisation: kernels overlap more than one deep
+        torch.cuda.current_stream(weight.device).synchronize()
         self.out_features, self.in_features = weight.shape
         self.prefetch_bytes = _prefetch_cap()
 
@@ -127,8 +128,7 @@ class Int8Linear:
         if not isinstance(x, kernels.Int8Rows):
             x = kernels.quantize_int8(x)
         hint = self.next_weight if self.hint_next and x.codes.shape[0] <= 256 and self.prefetch_bytes > 0 else None
-        y = kernels.gemm_int8(x, self.rows, out_dtype=out_dtype, epilogue=epilogue, prefetch=hint, prefetch_bytes=self.prefetch_bytes, w_settled=self.settled)
-        self.settled = True
+        y = kernels.gemm_int8(x, self.rows, out_dtype=out_dtype, epilogue=epilogue, prefetch=hint, prefetch_bytes=self.prefetch_bytes, w_settled=True)
         return kernels.add_bias(y, self.bias) if self.bias is not None else y
 
 

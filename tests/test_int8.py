@@ -317,6 +317,29 @@ def test_weights_quantised_by_the_call_ahead(M, N, K):
 
 
 @gpu
+@pytest.mark.parametrize("M", [1, 300])
+def test_layer_called_as_soon_as_it_is_made(M):
+    """A layer's product asks for its weight ahead of the kernels before it, so the layer is there only when its weight is; also for another stream, and for
+    calls one behind the other, whose kernels overlap several deep.  The memory of the weight of the layer before is handed out again."""
+    from spyinfer_b200.parts.linear import Int8Linear
+
+    a = kernels.quantize_int8(wild_rows(M, 512, 1).to(torch.bfloat16))
+    torch.cuda.synchronize()
+    side = torch.cuda.Stream()
+    for i in range(4):
+        weight = torch.randn(9472, 512, device=DEV) * (i + 1)
+        layer = Int8Linear(weight)
+        with torch.cuda.stream(side):
+            outs = [layer(a, out_dtype=torch.float32)]
+        outs += [layer(a, out_dtype=torch.float32) for _ in range(3)]
+        torch.cuda.synchronize()
+        want = product_of(a, kernels.quantize_int8(weight))
+        for out in outs:
+            check_product(out, want, torch.float32)
+        del layer, weight
+
+
+@gpu
 def test_gather_of_rows_that_there_are_not():
     """An index outside the stream reads nothing: its row is not a number, the others are as they are, and the status word says so."""
     x, w = wild_rows(5, 264, 1), torch.ones(264, device=DEV)
