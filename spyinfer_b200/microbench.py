@@ -3,7 +3,9 @@
     python -m spyinfer_b200.microbench gemm --m 2048 --n 24576 --k 4096 [--out-dtype float32] [--iters 20] [--graph] [--defer] [--epilogue swiglu]
     python -m spyinfer_b200.microbench attention --batch 8 --context 8192 [--q-len 1] [--split-keys 576] [--kernel tc|mma|decode] [--iters 10]
                                                  [--heads 64 --kv-heads 8 --head-dim 128] [--graph]
-    python -m spyinfer_b200.microbench rmsnorm --rows 2048 [--size 4096] [--splits 6]
+    python -m spyinfer_b200.microbench rmsnorm --rows 2048 [--size 4096] [--splits 6] [--int8]
+    python -m spyinfer_b200.microbench gemm --int8 --m 8 --n 24576 --k 4096 [--epilogue swiglu] [--graph]               # 8-bit rows by 8-bit weights
+    python -m spyinfer_b200.microbench quantize --rows 2048 [--size 4096] [--dtype float32]
     python -m spyinfer_b200.microbench step --batch 8 --context 8192 [--layers 4] [--prompt-tokens 2048]      # one step's kernels on the time axis
 
 Defaults are Qwen3-8B's sizes (32 query heads, 8 key/value heads, head size 128, pages of 16).
@@ -64,6 +66,49 @@ def bench_gemm(M: int, N: int, K: int, out_dtype=torch.bfloat16, iters: int = 20
     return {"us": ms * 1e3, "tflops": 2.0 * M * N * K / ms / 1e9, "gbs": (N * K * 2 + M * K * 2 + M * n_out * (4 if out_dtype == torch.float32 else 2)) / ms / 1e6}
 
 
+def _timed_launches(run, iters: int, graph: bool = True) -> float:
+    """Milliseconds a launch of ``run(i)``, by events around ``iters`` of them, replayed from a graph or launched one by one."""
+    run(0)
+    torch.cuda.synchronize()
+    e0, e1 = torch.cuda.Event(enable_timing=True), torch.cuda.Event(enable_timing=True)
+    if graph:
+        g = torch.cuda.CUDAGraph()
+        with torch.cuda.graph(g):
+            for i in range(iters):
+                run(i)
+        g.replay()
+        torch.cuda.synchronize()
+        e0.record()
+        g.replay()
+        e1.record()
+    else:
+        e0.record()
+        for i in range(iters):
+            run(i)
+        e1.record()
+    torch.cuda.synchronize()
+    return e0.elapsed_time(e1) / iters
+
+
+def bench_gemm_int8(M: int, N: int, K: int, out_dtype=torch.bfloat16, iters: int = 20, graph: bool = False, epilogue=None) -> dict:
+    """The product of 8-bit rows with settled weights, as a model's layers run it; the weights are cycled past L2."""
+    copies = max(1, int(300e6 // (N * K)) + 1)
+    ws = [kernels.quantize_int8(torch.randn(N, K, device=DEV) / math.sqrt(K)) for _ in range(copies)]
+    a = kernels.quantize_int8(torch.randn(M, K, device=DEV))
+    out = torch.empty(M, N // 2 if epilogue else N, device=DEV, dtype=out_dtype)
+    torch.cuda.synchronize()
+    ms = _timed_launches(lambda i: kernels.gemm_int8(a, ws[i % copies], out, epilogue=epilogue, w_settled=True), iters, graph)
+    return {"us": ms * 1e3, "tops": 2.0 * M * N * K / ms / 1e9, "gbs": (N * K + M * K + out.numel() * out.element_size()) / ms / 1e6}
+
+
+def bench_quantize(rows: int, size: int, dtype=torch.bfloat16, iters: int = 20) -> dict:
+    copies = max(2, int(200e6 // (rows * size * 3)) + 1)
+    xs = [torch.randn(rows, size, device=DEV).to(dtype) for _ in range(copies)]
+    out = kernels.empty_int8(rows, size, DEV)
+    ms = _timed_launches(lambda i: kernels.quantize_int8(xs[i % copies], out), iters)
+    return {"us": ms * 1e3, "gbs": rows * size * (xs[0].element_size() + 1) / ms / 1e6}
+
+
 def bench_attention(batch: int, context: int, q_len: int = 1, split_keys: int = 0, nh: int = 32, nkv: int = 8, hd: int = 128,
                     page_size: int = 16, iters: int = 10, kernel: str = "auto", share: str = "auto", graph: bool = False) -> dict:
     width = (context + page_size - 1) // page_size
@@ -111,40 +156,25 @@ def bench_attention(batch: int, context: int, q_len: int = 1, split_keys: int = 
     return {"us": ms * 1e3, "kv_gbs": kv_bytes / ms / 1e6, "tflops": flops / ms / 1e9}
 
 
-def bench_rmsnorm(rows: int, size: int, splits: int = 0, iters: int = 20, graph: bool = True) -> dict:
+def bench_rmsnorm(rows: int, size: int, splits: int = 0, iters: int = 20, graph: bool = True, int8: bool = False) -> dict:
     """The residual norm as a layer runs it: ``h += delta; x = norm(h) * weight`` with a float32 stream ``h``, bfloat16 ``x``
     and a bfloat16 ``delta`` (``splits == 0``) or ``splits`` stacked float32 partial products.  Several copies of the
-    buffers are cycled so that a launch does not find the last one's in L2."""
+    buffers are cycled so that a launch does not find the last one's in L2.  ``int8``: ``x`` in 8 bits with a scale a row."""
     copies = max(2, int(200e6 // (rows * size * 10)) + 1)
     hs = [torch.randn(rows, size, device=DEV) for _ in range(copies)]
     ds = [torch.randn(splits, rows, size, device=DEV) if splits else torch.randn(rows, size, device=DEV).to(torch.bfloat16) for _ in range(copies)]
     w = torch.ones(size, device=DEV, dtype=torch.bfloat16)
-    out = torch.empty(rows, size, device=DEV, dtype=torch.bfloat16)
+    out = kernels.empty_int8(rows, size, DEV) if int8 else torch.empty(rows, size, device=DEV, dtype=torch.bfloat16)
 
     def run(i):
-        kernels.rmsnorm(hs[i % copies], w, 1e-6, out, delta=ds[i % copies], write_back=True)
+        if int8:
+            kernels.rmsnorm_int8(hs[i % copies], w, 1e-6, out, delta=ds[i % copies], write_back=True, weight_settled=True)
+        else:
+            kernels.rmsnorm(hs[i % copies], w, 1e-6, out, delta=ds[i % copies], write_back=True)
 
-    run(0)
     torch.cuda.synchronize()
-    e0, e1 = torch.cuda.Event(enable_timing=True), torch.cuda.Event(enable_timing=True)
-    if graph:
-        g = torch.cuda.CUDAGraph()
-        with torch.cuda.graph(g):
-            for i in range(iters):
-                run(i)
-        g.replay()
-        torch.cuda.synchronize()
-        e0.record()
-        g.replay()
-        e1.record()
-    else:
-        e0.record()
-        for i in range(iters):
-            run(i)
-        e1.record()
-    torch.cuda.synchronize()
-    ms = e0.elapsed_time(e1) / iters
-    nbytes = rows * size * (4 + 4 + 2 + (4 * splits if splits else 2))
+    ms = _timed_launches(run, iters, graph)
+    nbytes = rows * size * (4 + 4 + (1 if int8 else 2) + (4 * splits if splits else 2))
     return {"us": ms * 1e3, "gbs": nbytes / ms / 1e6}
 
 
@@ -223,11 +253,18 @@ def main(argv=None) -> int:
     g.add_argument("--graph", action="store_true", help="replay the launches from a CUDA graph (device time without host launch cost)")
     g.add_argument("--defer", action="store_true", help="split-K parts may stay unsummed, as inside the model")
     g.add_argument("--epilogue", default=None, choices=["swiglu"])
+    g.add_argument("--int8", action="store_true", help="8-bit rows by 8-bit weights (no --defer)")
     n = sub.add_parser("rmsnorm")
     n.add_argument("--rows", type=int, required=True)
     n.add_argument("--size", type=int, default=4096)
     n.add_argument("--splits", type=int, default=0, help="the delta is a stack of this many float32 partial products (0: one bfloat16 tensor)")
     n.add_argument("--iters", type=int, default=20)
+    n.add_argument("--int8", action="store_true", help="the result in 8 bits with a scale a row")
+    q = sub.add_parser("quantize", help="rows to 8 bits with a scale each")
+    q.add_argument("--rows", type=int, required=True)
+    q.add_argument("--size", type=int, default=4096)
+    q.add_argument("--dtype", default="bfloat16", choices=["bfloat16", "float32"])
+    q.add_argument("--iters", type=int, default=20)
     t = sub.add_parser("step", help="the kernels of one step on the device's time axis")
     t.add_argument("--batch", type=int, default=8)
     t.add_argument("--context", type=int, default=8192)
@@ -249,15 +286,23 @@ def main(argv=None) -> int:
                    help="auto: tcgen05 for tiles mode, mma.sync for split mode; decode: the persistent tcgen05 decode kernel (q-len 1)")
     args = ap.parse_args(argv)
     kernels.require_cuda()
-    if args.what == "gemm":
+    if args.what == "gemm" and args.int8:
+        if args.defer:
+            ap.error("the 8-bit product always sums its parts")
+        r = bench_gemm_int8(args.m, args.n, args.k, getattr(torch, args.out_dtype), args.iters, graph=args.graph, epilogue=args.epilogue)
+        print(f"int8 gemm M={args.m} N={args.n} K={args.k}: {r['us']:.1f} us, {r['tops']:.1f} TOP/s, {r['gbs']:.1f} GB/s")
+    elif args.what == "quantize":
+        r = bench_quantize(args.rows, args.size, getattr(torch, args.dtype), args.iters)
+        print(f"quantize rows={args.rows} size={args.size} {args.dtype}: {r['us']:.1f} us, {r['gbs']:.1f} GB/s")
+    elif args.what == "gemm":
         r = bench_gemm(args.m, args.n, args.k, getattr(torch, args.out_dtype), args.iters, graph=args.graph, defer=args.defer, epilogue=args.epilogue)
         print(f"gemm M={args.m} N={args.n} K={args.k}: {r['us']:.1f} us, {r['tflops']:.1f} TFLOP/s, {r['gbs']:.1f} GB/s")
     elif args.what == "step":
         print_timeline(step_timeline(args.batch, args.context, args.layers, prompt_tokens=args.prompt_tokens))
         return 0
     elif args.what == "rmsnorm":
-        r = bench_rmsnorm(args.rows, args.size, args.splits, args.iters)
-        print(f"rmsnorm rows={args.rows} size={args.size} splits={args.splits}: {r['us']:.1f} us, {r['gbs']:.1f} GB/s")
+        r = bench_rmsnorm(args.rows, args.size, args.splits, args.iters, int8=args.int8)
+        print(f"rmsnorm{' int8' if args.int8 else ''} rows={args.rows} size={args.size} splits={args.splits}: {r['us']:.1f} us, {r['gbs']:.1f} GB/s")
     else:
         r = bench_attention(args.batch, args.context, args.q_len, args.split_keys, nh=args.heads, nkv=args.kv_heads, hd=args.head_dim, page_size=args.page_size,
                             iters=args.iters, kernel=args.kernel, share=args.share, graph=args.graph)

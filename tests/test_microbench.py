@@ -23,3 +23,10 @@ def test_microbench_commands_run():
     assert "GB/s" in run("rmsnorm", "--rows", 64, "--size", 1024, "--splits", 3, "--iters", 3)
     out = run("step", "--batch", 2, "--context", 100, "--layers", 1)
     assert "whole step" in out and "attention_decode_kernel" in out
+
+
+def test_microbench_8_bit_commands_run():
+    assert "TOP/s" in run("gemm", "--int8", "--m", 8, "--n", 512, "--k", 512, "--iters", 3, "--graph", "--epilogue", "swiglu")
+    assert "TOP/s" in run("gemm", "--int8", "--m", 300, "--n", 520, "--k", 513, "--iters", 3, "--out-dtype", "float32")
+    assert "GB/s" in run("rmsnorm", "--rows", 64, "--size", 1024, "--splits", 3, "--iters", 3, "--int8")
+    assert "GB/s" in run("quantize", "--rows", 65, "--size", 1025, "--iters", 3, "--dtype", "float32")
