@@ -7,7 +7,8 @@
 // The codes are exact: 127 y / amax is compared with the half between two integers without being rounded first.  In 32 bits
 // t = y * (127 / amax) is off by at most |t| 2^-24 <= 7.6e-6 from the quotient (the fused multiply-add rounds t itself to the integer
 // directly), so only where t lies within 2e-5 of a half is the question left open; there 254 y and (2 n + 1) amax are compared without rounding
-// (one group of eight in 3,000 of float32 numbers; bfloat16 rows have exact halves, and one in sixty).  The codes depend on no summation order and on no approximation, and a test can ask for equality.
+// (one group of eight in 3,000 of float32 numbers; bfloat16 rows have exact halves, and one in sixty).  The codes depend on no summation order and on no
+// approximation, and a test can ask for equality.
 //
 // A row of zeros has codes 0 and scale 0.  A row with a NaN or an infinity has codes 0 and the scale NaN: what is made of it is NaN, and no
 // other row is touched.  |code| <= 127: -128 does not occur.
@@ -395,9 +396,9 @@ extern "C" int spy_quantize_int8(const void* x, int dtype, long long ldx, int8_t
 }
 
 // x: [total, len] of x_dtype; delta: null or `splits` stacked [*, len] arrays of delta_dtype, split_stride elements apart, added to x in order;
-// rows: null or n row indices (gather), one outside x gives a row that is not a number
-// and is reported in status (null, or two ints); w: [len] of w_dtype (settled: no
-// kernel that may still run writes it); codes and scales as above.  write_back stores the sum into x and needs rows == null.
+// rows: null or n row indices (gather), one outside x gives a row that is not a number and is reported in status (null, or two ints);
+// w: [len] of w_dtype (settled: no kernel that may still run writes it); codes and scales as above.  write_back stores the sum into x and needs
+// rows == null.
 extern "C" int spy_rmsnorm_int8(void* x, int x_dtype, const void* delta, int delta_dtype, int splits, long long split_stride, const int* rows,
                                 const void* w, int w_dtype, int8_t* codes, long long ldc, float* scales, int total, int n, int len, float eps,
                                 int write_back, int settled, int* status, cudaStream_t stream)
