@@ -73,6 +73,13 @@ __device__ __forceinline__ void umma_s8_pair(uint32_t tmem_d, uint64_t desc_a, u
 // below -87 gives g / inf = -0, the limit.
 __device__ __forceinline__ float silu_mul(float g, float u) { return __fdividef(g, 1.0f + __expf(-g)) * u; }
 
+// One lane of a warp that has come together, always the same.
+__device__ __forceinline__ bool elect_one()
+{
+    uint32_t chosen;
+    asm volatile("{\n\t.reg .pred p;\n\telect.sync _|p, 0xffffffff;\n\tselp.u32 %0, 1, 0, p;\n\t}" : "=r"(chosen));
+    return chosen != 0;
+}
 template <int WARPS> __device__ __forceinline__ void epilogue_barrier() { asm volatile("bar.sync 1, %0;" ::"n"(32 * WARPS) : "memory"); }
 __device__ __forceinline__ void cluster_arrive() { asm volatile("barrier.cluster.arrive.release.aligned;" ::: "memory"); }
 __device__ __forceinline__ void cluster_wait() { asm volatile("barrier.cluster.wait.acquire.aligned;" ::: "memory"); }
@@ -269,67 +276,77 @@ gemm_int8_few_kernel(const __grid_constant__ CUtensorMap map_w, const __grid_con
     // the cluster's first barrier: a block's mail may be written.  All but the warps that free the ring arrive here.
     if (splits > 1 && (!T::MAIL_IN_RING || warp < 2)) cluster_arrive();
     if (warp == 0) {
-        if (lane == 0) {
-            // settled weights depend on no earlier kernel: their tiles for the first stages are requested before the wait for the kernels ahead in the stream
-            if (!settled) pdl_wait();
-            const int pre = min(num_kb, stages);
+        // The whole warp walks the loops of this role and the next, and one lane of it requests and issues: what the instructions take is then the same for
+        // the warp, not a lane's (a block's K block of 128 codes, 16 tokens: 0.32 us with all of it on one lane, 0.22 now).
+        const bool lead = elect_one();
+        // settled weights depend on no earlier kernel: their tiles for the first stages are requested before the wait for the kernels ahead in the stream
+        if (!settled) pdl_wait();
+        const int pre = min(num_kb, stages);
 #pragma unroll 1
-            for (int i = 0; i < pre; ++i) {
+        for (int i = 0; i < pre; ++i) {
+            if (lead) {
                 mbar_expect_tx(full_bar + i, stage_tx);
                 tma_load_2d(smem_u32(tiles + (size_t)i * stage_bytes), &map_w, (kb0 + i) * BK, x0, full_bar + i);
             }
-            pdl_wait();
+        }
+        pdl_wait();
 #pragma unroll 1
-            for (int i = 0; i < pre; ++i) tma_load_2d(smem_u32(tiles + (size_t)i * stage_bytes + x_bytes), &map_a, (kb0 + i) * BK, y0, full_bar + i);
-            int s = 0;
-            uint32_t phase = 1;   // of the round before: the first wait on a stage is for its first release
+        for (int i = 0; i < pre; ++i)
+            if (lead) tma_load_2d(smem_u32(tiles + (size_t)i * stage_bytes + x_bytes), &map_a, (kb0 + i) * BK, y0, full_bar + i);
+        int s = 0;
+        uint32_t phase = 1;   // of the round before: the first wait on a stage is for its first release
 #pragma unroll 1
-            for (int i = pre; i < num_kb; ++i) {
-                if (!mbar_wait(empty_bar + s, phase ^ 1, abort_flag)) break;
+        for (int i = pre; i < num_kb; ++i) {
+            if (!__all_sync(0xffffffffu, mbar_wait(empty_bar + s, phase ^ 1, abort_flag))) break;
+            if (lead) {
                 uint8_t* xs = tiles + (size_t)s * stage_bytes;
                 mbar_expect_tx(full_bar + s, stage_tx);
                 tma_load_2d(smem_u32(xs), &map_w, (kb0 + i) * BK, x0, full_bar + s);
                 tma_load_2d(smem_u32(xs + x_bytes), &map_a, (kb0 + i) * BK, y0, full_bar + s);
-                if (++s == stages) {
-                    s = 0;
-                    phase ^= 1;
-                }
             }
-            // Every load of this block has been requested: what follows in a decode step are short kernels that leave the memory idle, and then a product
-            // whose weights are known now.  This block asks for its share of them to be brought into L2 meanwhile.  A hint only: nothing waits for it.
-            if (next_bytes > 0) {
-                const long long blocks = (long long)gridDim.x * gridDim.y, me = blockIdx.x + (long long)gridDim.x * blockIdx.y;
-                const long long piece = ((next_bytes + blocks - 1) / blocks + 127) / 128 * 128;
-                const long long stop = min(next_bytes, (me + 1) * piece);
+            if (++s == stages) {
+                s = 0;
+                phase ^= 1;
+            }
+        }
+        // Every load of this block has been requested: what follows in a decode step are short kernels that leave the memory idle, and then a product
+        // whose weights are known now.  This block asks for its share of them to be brought into L2 meanwhile.  A hint only: nothing waits for it.
+        if (lead && next_bytes > 0) {
+            const long long blocks = (long long)gridDim.x * gridDim.y, me = blockIdx.x + (long long)gridDim.x * blockIdx.y;
+            const long long piece = ((next_bytes + blocks - 1) / blocks + 127) / 128 * 128;
+            const long long stop = min(next_bytes, (me + 1) * piece);
 #pragma unroll 1
-                for (long long at = me * piece; at < stop; at += 16384) l2_prefetch(next_weights + at, (uint32_t)(min(stop - at, 16384LL) & ~15LL));
-            }
+            for (long long at = me * piece; at < stop; at += 16384) l2_prefetch(next_weights + at, (uint32_t)(min(stop - at, 16384LL) & ~15LL));
         }
     } else if (warp == 1) {
-        if (lane == 0) {
-            const uint32_t idesc = instr_desc_s8(BM, BN);
-            int s = 0;
-            uint32_t phase = 0;
-            pdl_wait();                       // the limit of the waits below is not for the kernels ahead
+        const bool lead = elect_one();
+        const uint32_t idesc = instr_desc_s8(BM, BN);
+        const uint64_t dx0 = desc_k_major(smem_u32(tiles)), dy0 = desc_k_major(smem_u32(tiles + x_bytes));
+        const uint32_t step = (uint32_t)stage_bytes >> 4, end = step * stages;
+        int s = 0;
+        uint32_t phase = 0, at = 0;           // at: where the stage lies, in the descriptors' units
+        pdl_wait();                           // the limit of the waits below is not for the kernels ahead
 #pragma unroll 1
-            for (int i = 0; i < num_kb; ++i) {
-                if (!mbar_wait(full_bar + s, phase, abort_flag)) break;
-                fence_after_sync();
-                const uint8_t* xs = tiles + (size_t)s * stage_bytes;
-                const uint64_t dx = desc_k_major(smem_u32(xs)), dy = desc_k_major(smem_u32(xs + x_bytes));
+        for (int i = 0; i < num_kb; ++i) {
+            if (!__all_sync(0xffffffffu, mbar_wait(full_bar + s, phase, abort_flag))) break;
+            fence_after_sync();
+            if (lead) {
 #pragma unroll
                 for (int k = 0; k < BK / UMMA_K; ++k) {
-                    const uint64_t adv = (uint64_t)((k * UMMA_K) >> 4);
-                    umma_s8(tmem_base, dx + adv, dy + adv, idesc, (i > 0 || k > 0) ? 1u : 0u);
+                    const uint32_t adv = at + (uint32_t)((k * UMMA_K) >> 4);
+                    umma_s8(tmem_base, dx0 + adv, dy0 + adv, idesc, (i > 0 || k > 0) ? 1u : 0u);
                 }
                 umma_commit(empty_bar + s);   // the stage is free again when these MMAs have read it
-                if (++s == stages) {
-                    s = 0;
-                    phase ^= 1;
-                }
             }
-            umma_commit(accum_bar);           // the accumulator is complete when every MMA has finished
+            ++s;
+            at += step;
+            if (at == end) {
+                s = 0;
+                at = 0;
+                phase ^= 1;
+            }
         }
+        if (lead) umma_commit(accum_bar);     // the accumulator is complete when every MMA has finished
     } else {
         // warp w reads tensor-memory lanes 32 (w % 4) .. + 31, i.e. weight rows of the tile
         const int quarter = warp & 3, turns = (warp - 2) >> 2, row = quarter * 32 + lane, tid = threadIdx.x - 64;
@@ -479,10 +496,11 @@ gemm_int8_pair_kernel(const __grid_constant__ CUtensorMap map_w, const __grid_co
     cluster_sync();   // both blocks run, and their barriers are initialised
     // settled weights' first stages are requested beside the allocation and before the wait for the kernels ahead in the stream
     const int pre = min(k_blocks, stages);
+    const bool lead = elect_one();      // whole warps walk the loops, as in the kernel above (2,048 x 6,144 x 4,096: 41.5 us on one lane, 37 now)
     if (warp == 0) {
-        if (lane == 0) {
-            const int x0 = (cluster / tokens.count) * (2 * BM) + (int)rank * BM;
-            if (!settled) pdl_wait();
+        const int x0 = (cluster / tokens.count) * (2 * BM) + (int)rank * BM;
+        if (!settled) pdl_wait();
+        if (lead) {
             for (int i = 0; i < pre; ++i) {
                 if (rank == 0) mbar_expect_tx(full_bar + i, 2u * stage_bytes);     // both blocks' bytes
                 tma_load_2d_pair(smem_u32(tiles + (size_t)i * stage_bytes), &map_w, i * BK, x0, map_to_rank(smem_u32(full_bar + i), 0));
@@ -499,37 +517,41 @@ gemm_int8_pair_kernel(const __grid_constant__ CUtensorMap map_w, const __grid_co
 
     pdl_launch_dependents();
     if (warp == 0) {
-        if (lane == 0) {
-            pdl_wait();
-            int s = pre == stages ? 0 : pre;
-            uint32_t phase = pre == stages ? 1 : 0;   // of the ring's round; the first round's waits end at once
-            bool ok = true;
-            for (int tile = cluster; ok && tile < num_tiles; tile += clusters) {
-                const int ty = tile % tokens.count;
-                const int x0 = (tile / tokens.count) * (2 * BM) + (int)rank * BM, y0 = tokens.first(ty) + (int)rank * (tokens.height(ty) / 2);
-                int kb = 0;
-                if (tile == cluster) {
-                    for (; kb < pre; ++kb)
-                        tma_load_2d_pair(smem_u32(tiles + (size_t)kb * stage_bytes + PAIR_X_BYTES), &map_a, kb * BK, y0, map_to_rank(smem_u32(full_bar + kb), 0));
-                }
-                for (; kb < k_blocks; ++kb) {
-                    if (!mbar_wait(empty_bar + s, phase ^ 1, abort_flag)) { ok = false; break; }
+        pdl_wait();
+        int s = pre == stages ? 0 : pre;
+        uint32_t phase = pre == stages ? 1 : 0;   // of the ring's round; the first round's waits end at once
+        bool ok = true;
+        for (int tile = cluster; ok && tile < num_tiles; tile += clusters) {
+            const int ty = tile % tokens.count;
+            const int x0 = (tile / tokens.count) * (2 * BM) + (int)rank * BM, y0 = tokens.first(ty) + (int)rank * (tokens.height(ty) / 2);
+            int kb = 0;
+            if (tile == cluster) {
+                for (; kb < pre; ++kb)
+                    if (lead) tma_load_2d_pair(smem_u32(tiles + (size_t)kb * stage_bytes + PAIR_X_BYTES), &map_a, kb * BK, y0, map_to_rank(smem_u32(full_bar + kb), 0));
+            }
+#pragma unroll 1
+            for (; kb < k_blocks; ++kb) {
+                ok = __all_sync(0xffffffffu, mbar_wait(empty_bar + s, phase ^ 1, abort_flag));
+                if (!ok) break;
+                if (lead) {
                     uint8_t* xs = tiles + (size_t)s * stage_bytes;
                     if (rank == 0) mbar_expect_tx(full_bar + s, 2u * stage_bytes);
                     const uint32_t leader_full = map_to_rank(smem_u32(full_bar + s), 0);
                     tma_load_2d_pair(smem_u32(xs), &map_w, kb * BK, x0, leader_full);
                     tma_load_2d_pair(smem_u32(xs + PAIR_X_BYTES), &map_a, kb * BK, y0, leader_full);
-                    if (++s == stages) {
-                        s = 0;
-                        phase ^= 1;
-                    }
+                }
+                if (++s == stages) {
+                    s = 0;
+                    phase ^= 1;
                 }
             }
         }
     } else if (warp == 1) {
-        if (lane == 0 && rank == 0) {
+        if (rank == 0) {
+            const uint64_t dx0 = desc_k_major(smem_u32(tiles)), dy0 = desc_k_major(smem_u32(tiles + PAIR_X_BYTES));
+            const uint32_t step = (uint32_t)stage_bytes >> 4, end = step * stages;
             int s = 0;
-            uint32_t phase = 0;
+            uint32_t phase = 0, at = 0;       // at: where the stage lies, in the descriptors' units
             int i = 0;
             bool ok = true;
             pdl_wait();       // the limit of the waits below is not for the kernels ahead
@@ -537,28 +559,32 @@ gemm_int8_pair_kernel(const __grid_constant__ CUtensorMap map_w, const __grid_co
                 const uint32_t idesc = instr_desc_s8(2 * BM, tokens.height(tile % tokens.count));
                 const int buf = i & 1;
                 const uint32_t aph = (uint32_t)(i >> 1) & 1;
-                if (i >= 2) ok = mbar_wait(acc_empty + buf, aph ^ 1, abort_flag);   // both blocks' epilogues have read this buffer's last tile
+                if (i >= 2) ok = __all_sync(0xffffffffu, mbar_wait(acc_empty + buf, aph ^ 1, abort_flag));   // both blocks' epilogues have read this buffer's last tile
                 if (!ok) break;
                 fence_after_sync();
                 const uint32_t acc = tmem_base + (uint32_t)buf * PAIR_BN;
+#pragma unroll 1
                 for (int kb = 0; kb < k_blocks; ++kb) {
-                    ok = mbar_wait(full_bar + s, phase, abort_flag);
+                    ok = __all_sync(0xffffffffu, mbar_wait(full_bar + s, phase, abort_flag));
                     if (!ok) break;
                     fence_after_sync();
-                    const uint8_t* xs = tiles + (size_t)s * stage_bytes;
-                    const uint64_t dx = desc_k_major(smem_u32(xs)), dy = desc_k_major(smem_u32(xs + PAIR_X_BYTES));
+                    if (lead) {
 #pragma unroll
-                    for (int k = 0; k < BK / UMMA_K; ++k) {
-                        const uint64_t adv = (uint64_t)((k * UMMA_K) >> 4);
-                        umma_s8_pair(acc, dx + adv, dy + adv, idesc, (kb > 0 || k > 0) ? 1u : 0u);
+                        for (int k = 0; k < BK / UMMA_K; ++k) {
+                            const uint32_t adv = at + (uint32_t)((k * UMMA_K) >> 4);
+                            umma_s8_pair(acc, dx0 + adv, dy0 + adv, idesc, (kb > 0 || k > 0) ? 1u : 0u);
+                        }
+                        umma_commit_pair(empty_bar + s);
                     }
-                    umma_commit_pair(empty_bar + s);
-                    if (++s == stages) {
+                    ++s;
+                    at += step;
+                    if (at == end) {
                         s = 0;
+                        at = 0;
                         phase ^= 1;
                     }
                 }
-                if (ok) umma_commit_pair(acc_full + buf);
+                if (ok && lead) umma_commit_pair(acc_full + buf);
             }
         }
     } else {
