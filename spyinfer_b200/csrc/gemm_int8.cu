@@ -669,29 +669,31 @@ struct Plan {
 };
 
 // The plan is the one of the least expected time, in us, with rates in bytes a us.  Both kernels: what is fixed, plus the slowest of what the main loop
-// waits for, plus the read-out behind it.  The numbers were fitted to 5,559 measurements of 13 weight sizes (512 x 8,192 to 51,200 x 5,120) at 1 to 4,096 tokens
-// with all tiles and cuts: the chosen plans take 2 % longer than the fastest of all measured on average, 20 % at worst (1,024 x 1,024, 320 tokens).  Which
-// kernel, for instance (us, few / pairs): 6,144 x 4,096 at 128 tokens 11.5 / 15.2, 384 15.0 / 17.5, 640 17.9 / 19.0; 34,816 x 5,120 gated at 64 tokens 30.5 / 34.2, 192
-// 48.9 / 39.3.  How K is cut (1 / 2 / 4 / 8 ways, 8 tokens): 6,144 x 4,096 11.4 / 8.1 / 6.9 / 9.7, 4,096 x 12,288 37.8 / 18.4 / 12.4 / 11.8, 24,576 x 4,096 18.3 / 23.0 / 23.6 / -.
+// waits for, plus the read-out behind it.  The numbers were fitted to the measurements of 18 weight sizes (512 x 8,192 to 51,200 x 5,120) at 1 to 4,096
+// tokens with all tiles and cuts: the chosen plans take 1.4 % longer than the fastest of all measured on average, 20 % at worst (5,003 x 2,055, 512 tokens).
+// Which kernel, for instance (us, few / pairs): 6,144 x 4,096 at 128 tokens 10.7 / 11.5, 384 13.8 / 13.7; 34,816 x 5,120 gated at 64 tokens 29.5 / 31.8, 200
+// 46.2 / 37.1.  How K is cut (1 / 2 / 4 / 8 ways, 8 tokens): 6,144 x 4,096 9.0 / 7.5 / 6.7 / 9.9, 4,096 x 12,288 22.7 / 14.1 / 11.3 / 10.7, 24,576 x 4,096
+// 17.9 / 21.9 / 22.6 / -.
 static double few_time(int M, int N, int k_blocks, int bn, int splits, int rows, int sms)
 {
     const double blocks = (double)((M + bn - 1) / bn) * ((N + rows - 1) / rows) * splits, depth = (k_blocks + splits - 1) / splits;
     const double stage = (double)(rows + bn) * BK, tokens = (M < bn ? M : bn) / 128.0;
     const double even = blocks / sms, most = (double)(((long long)blocks + sms - 1) / sms);
-    const double per_sm = blocks <= 2 * sms ? fmax(1.0, 0.46 * most + 0.54 * even) : 1.48 * even;      // an SM with one more; the last of many waves is not full
-    double load = (double)N * k_blocks * BK / 8.2e6;                                  // the weights from memory
-    load = fmax(load, depth * stage / 6.4e4);                                         // a block's stages, one after the other
-    load = fmax(load, per_sm * depth * stage / 9.6e4);                                // an SM's
-    load = fmax(load, blocks * depth * stage / 2.06e7);                               // everybody's, from L2
-    return 2.1 + (splits > 1 ? 0.8 + 1.7 * tokens : 0.0) + 1.9 * tokens + load;
+    const double room = splits > 2 ? 1.85 * sms : 2.0 * sms;                          // clusters of 4 and 8 leave some SMs with one block
+    const double per_sm = blocks <= room ? fmax(1.0, 0.61 * most + 0.39 * even) : 1.52 * even;      // an SM with one more; the last of many waves is not full
+    double load = (double)N * k_blocks * BK / 1.0e7;                                  // the weights from memory
+    load = fmax(load, depth * fmax(0.22, stage / 8.3e4));                             // a block's stages, one after the other: issued, and fetched
+    load = fmax(load, per_sm * depth * stage / 1.15e5);                               // an SM's
+    const double cut = splits == 1 ? 0.0 : (splits == 2 ? 0.3 : (splits == 4 ? 0.6 : 0.9)) + 2.2 * tokens;      // the sums' way between blocks
+    return 1.95 + cut + 1.8 * tokens + 0.29 * even + load;
 }
 static double pair_time(int M, int N, int k_blocks, int count, int sms)
 {
     const TokenTiles t = token_tiles(M, count);
     const int clusters = sms / 2 > 0 ? sms / 2 : 1;
     const double height = t.rows / 256.0, rounds = (double)(((long long)((N + 2 * BM - 1) / (2 * BM)) * count + clusters - 1) / clusters);
-    const double load = fmax((double)N * k_blocks * BK / 8.2e6, rounds * k_blocks * pair_stage_bytes(t.rows) / 7.9e4);
-    return 6.1 + load + 2.0 * height + 1.2 * (rounds - 1) * height;
+    const double load = fmax((double)N * k_blocks * BK / 1.0e7, rounds * k_blocks * pair_stage_bytes(t.rows) / 1.12e5);
+    return 6.2 + load + 2.2 * height + 1.8 * (rounds - 1) * height;
 }
 
 static Plan choose(int M, int N, int K)
