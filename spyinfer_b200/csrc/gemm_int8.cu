@@ -12,9 +12,9 @@
 // Tails: rows beyond M or N and the end of K are zero-filled by TMA, stores are predicated.  Any K; the rows of A and of W lie a multiple of 16 bytes
 // apart.  No cluster multicast is used.
 //
-// Measured (replayed from a graph, weights cycled past L2; the floor is the bytes at 6,547 GB/s or the operations at 3,279 TOP/s): 1 x 6,144 x 4,096 6.6 us
-// (floor 3.9), 8 x 24,576 x 4,096 gated 18.0 (15.4), 64 x 4,096 x 12,288 13.4 (7.9): the first bytes' way and a microsecond behind the last ones; 2,048 x
-// 6,144 x 4,096 41 (31.4: 2.6 rounds of tiles where 3 are paid, 79 GB/s into an SM), 4,096 x 24,576 x 4,096 gated 262 to 280 (251: the power cap).
+// Measured (replayed from a graph, weights cycled past L2; the floor is the bytes at 6,547 GB/s or the operations at 3,279 TOP/s): 1 x 6,144 x 4,096 6.2 us
+// (floor 3.9), 8 x 24,576 x 4,096 gated 18.0 (15.4), 64 x 4,096 x 12,288 13.4 to 14.2 (7.9): the first bytes' way and a microsecond behind the last ones;
+// 2,048 x 6,144 x 4,096 37.0 (31.4: 2.6 rounds of tiles where 3 are paid), 4,096 x 24,576 x 4,096 gated 242 to 247 (251).
 //
 // The reference has no integer product (its own are half precision: spymaster2h/spyinfer src/backends/cuda/cublas/sgemm.cu:37-55).
 #include <cuda.h>
