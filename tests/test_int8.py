@@ -15,7 +15,17 @@ STEP = {torch.bfloat16: 2.0 ** -8, torch.float32: 2.0 ** -24}      # a rounding 
 
 
 @pytest.fixture(autouse=True)
-def guard_zones(guarded_allocations):
+def guard_zones(guarded_allocations, monkeypatch):
+    """Tensors made by strides lie between guard zones as well; the zone behind a matrix of codes begins where its last row ends."""
+    plain = torch.empty_strided
+
+    def empty_strided(size, stride, **kwargs):
+        if guarded_allocations._plain(kwargs):
+            return plain(size, stride, **kwargs)
+        extent = 1 + sum((n - 1) * s for n, s in zip(size, stride)) if all(size) else 0
+        return torch.empty((extent,), **kwargs).as_strided(size, stride)
+
+    monkeypatch.setattr(torch, "empty_strided", empty_strided)
     yield guarded_allocations
 
 
