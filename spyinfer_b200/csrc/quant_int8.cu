@@ -7,7 +7,7 @@
 // The codes are exact: 127 y / amax is compared with the half between two integers without being rounded first.  In 32 bits
 // t = y * (127 / amax) is off by at most |t| 2^-24 <= 7.6e-6 from the quotient (the fused multiply-add rounds t itself to the integer
 // directly), so only where t lies within 2e-5 of a half is the question left open; there 254 y and (2 n + 1) amax are compared without rounding
-// (one group of eight in 3,000 of float32 numbers; bfloat16 rows have exact halves, and one in sixty).  The codes depend on no summation order and on no
+// (one group of eight in 3,000 of float32 numbers; bfloat16 rows have exact halves, and one in sixty: those have a shorter way, encode8).  The codes depend on no summation order and on no
 // approximation, and a test can ask for equality.
 //
 // A row of zeros has codes 0 and scale 0.  A row with a NaN or an infinity has codes 0 and the scale NaN: what is made of it is NaN, and no
@@ -104,20 +104,34 @@ __device__ __forceinline__ int nearest_exact(float y, float k, float amax)
     return d > lo ? low + 1 : (d < lo ? low : low + (low & 1));
 }
 
-// The codes of eight numbers, four in a word.  k = 127 / amax.
-__device__ __forceinline__ uint2 encode8(const float (&y)[8], float k, float amax)
+// The codes of eight numbers, four in a word.  k = 127 / amax.  BF16: the numbers and amax have 8 significant bits.  A quotient t is then a half or at least
+// t / (254 * 255) away from one, 250 times what y * k is off by, so that only halves can come out on the wrong side, and 127 y - n amax is exact.
+template <bool BF16> __device__ __forceinline__ uint2 encode8(const float (&y)[8], float k, float amax)
 {
+    // Numbers that are looked at together: of bfloat16 one warp in four has a half among 4 a lane, two in five among 8 (24,576 x 4,096 by 8 / 4 / 2: 50.8 / 49.4
+    // / 53.7 us).
+    constexpr int PART = BF16 ? 4 : 8;
     uint32_t m[8];
-    float far = 0.f;
 #pragma unroll
-    for (int e = 0; e < 8; ++e) {
-        const float n = fmaf(y[e], k, MAGIC);
-        far = fmaxf(far, fabsf(fmaf(y[e], k, MAGIC - n)));
-        m[e] = __float_as_uint(n);
-    }
-    if (far > 0.49998f) {
+    for (int part = 0; part < 8; part += PART) {
+        float far = 0.f;
 #pragma unroll
-        for (int e = 0; e < 8; ++e) m[e] = (uint32_t)nearest_exact(y[e], k, amax);
+        for (int e = part; e < part + PART; ++e) {
+            const float n = fmaf(y[e], k, MAGIC);
+            far = fmaxf(far, fabsf(fmaf(y[e], k, MAGIC - n)));
+            m[e] = __float_as_uint(n);
+        }
+        if (far > 0.49998f) {
+#pragma unroll
+            for (int e = part; e < part + PART; ++e) {
+                if constexpr (BF16) {
+                    const float d = fmaf(MAGIC - __uint_as_float(m[e]), amax, 127.0f * y[e]);
+                    if (fabsf(d) * 2.0f == amax && (m[e] & 1)) m[e] += d > 0.f ? 1u : 0xffffffffu;
+                } else {
+                    m[e] = (uint32_t)nearest_exact(y[e], k, amax);
+                }
+            }
+        }
     }
     return make_uint2(__byte_perm(__byte_perm(m[0], m[1], 0x0040), __byte_perm(m[2], m[3], 0x0040), 0x5410),
                       __byte_perm(__byte_perm(m[4], m[5], 0x0040), __byte_perm(m[6], m[7], 0x0040), 0x5410));
@@ -174,20 +188,20 @@ __device__ __forceinline__ float scale_of(uint32_t size, float factor)
 {
     return size >= 0x7f800000u ? __int_as_float(0x7fc00000) : __uint_as_float(size) / 127.0f * factor;
 }
-__device__ __forceinline__ uint2 encode_group(float (&y)[8], const RowScale& s)
+template <bool BF16> __device__ __forceinline__ uint2 encode_group(float (&y)[8], const RowScale& s)
 {
     if (!s.plain) {
 #pragma unroll
         for (int e = 0; e < 8; ++e) y[e] = s.none ? 0.f : y[e] * s.lift;
     }
-    return encode8(y, s.k, s.amax);
+    return encode8<BF16>(y, s.k, s.amax);
 }
-template <bool WHOLE, int GROUPS>
+template <bool WHOLE, int GROUPS, bool BF16 = false>
 __device__ __forceinline__ void encode_row(int8_t* row, int len, float (&y)[GROUPS][8], uint32_t size)
 {
     const RowScale s = row_scale(size);
 #pragma unroll
-    for (int g = 0; g < GROUPS; ++g) put_codes<WHOLE>(row, g, len, encode_group(y[g], s));
+    for (int g = 0; g < GROUPS; ++g) put_codes<WHOLE>(row, g, len, encode_group<BF16>(y[g], s));
 }
 
 // Sum and largest size over the block, one barrier; `part` holds 2 x 32 words and is used once a launch.
@@ -222,7 +236,7 @@ __global__ void __launch_bounds__(1024) quantize_kernel(const T* __restrict__ x,
 #pragma unroll
         for (int e = 0; e < 8; ++e) size = size_max(size, v[g][e]);
     block_reduce<false>(none, size, part);
-    encode_row<WHOLE, GROUPS>(codes + (size_t)blockIdx.x * ldc, len, v, size);
+    encode_row<WHOLE, GROUPS, sizeof(T) == 2>(codes + (size_t)blockIdx.x * ldc, len, v, size);
     if (threadIdx.x == 0) scales[blockIdx.x] = scale_of(size, 1.f);
 }
 
@@ -253,7 +267,7 @@ __global__ void __launch_bounds__(1024) quantize_packed_kernel(const bf16* __res
     for (int g = 0; g < GROUPS; ++g) {
         float y[8] = {__uint_as_float(v[g].x << 16), __uint_as_float(v[g].x & 0xffff0000u), __uint_as_float(v[g].y << 16), __uint_as_float(v[g].y & 0xffff0000u),
                       __uint_as_float(v[g].z << 16), __uint_as_float(v[g].z & 0xffff0000u), __uint_as_float(v[g].w << 16), __uint_as_float(v[g].w & 0xffff0000u)};
-        put_codes<true>(out, g, len, encode_group(y, s));
+        put_codes<true>(out, g, len, encode_group<true>(y, s));
     }
     if (threadIdx.x == 0) scales[blockIdx.x] = scale_of(size, 1.f);
 }
@@ -281,7 +295,7 @@ __global__ void __launch_bounds__(1024) quantize_long_kernel(const T* __restrict
     for (int at = 0; len - at > 0; at += piece) {
         float v[1][8];
         fetch<false>(row + at, 0, len - at, v[0]);
-        encode_row<false, 1>(out + at, len - at, v, size);
+        encode_row<false, 1, sizeof(T) == 2>(out + at, len - at, v, size);
         if (len - at <= piece) break;
     }
     if (threadIdx.x == 0) scales[blockIdx.x] = scale_of(size, 1.f);
@@ -369,8 +383,8 @@ static int quantize(const T* x, long long ldx, int8_t* codes, long long ldc, flo
     }
     // Few rows: the row spread as wide as it goes.  Many: more groups a thread, as what a warp does once a row (reduction, barrier, division) is bought
     // once for more elements.  us with 1 / 2 / 4 / 8 groups, whole rows of bfloat16: 64 x 4,096 1.9 / 1.9 / 2.1 / 2.9, 2,048 x 4,096 8.4 / 7.3 / 7.2 / 7.4,
-    // 2,048 x 12,288 - / 20.5 / 17.4 / 16.2, 24,576 x 4,096 81 / 63.7 / 59.3 / 52.9 (0.87 of the copy rate; two thirds of the issue slots are taken); of float32 2,048 x
-    // 4,096 8.3 / 7.4 / 6.5 (0.98).  Others, float32, 1 / 2 / 4 groups with codes stored one
+    // 2,048 x 12,288 - / 20.5 / 17.4 / 16.2, 24,576 x 4,096 81 / 63.7 / 59.3 / 52.9 (two thirds of the issue slots taken); with halves decided the short way 6.8, 15.3
+    // and 49.4 (0.93 of the copy rate) with the groups taken here; of float32 2,048 x 4,096 8.3 / 7.4 / 6.5 (0.98).  Others, float32, 1 / 2 / 4 groups with codes stored one
     // by one: 1,531 x 4,999 20.8 / 12.6 / 14.6, 64 x 4,999 2.6 / 3.7 / 5.4; in words 9.3 and 2.3 with the groups taken here (bfloat16 10.7 and 2.7).
     const bool packed = whole && sizeof(T) == 2;
     const int groups = row_groups(len, n < 1024 ? 1 : (!whole ? 2 : (packed && (long long)n * len >= (1 << 24) ? 8 : 4))), threads = row_threads(len, groups);
