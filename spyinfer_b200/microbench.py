@@ -6,7 +6,7 @@
     python -m spyinfer_b200.microbench rmsnorm --rows 2048 [--size 4096] [--splits 6] [--int8]
     python -m spyinfer_b200.microbench gemm --int8 --m 8 --n 24576 --k 4096 [--epilogue swiglu] [--graph]               # 8-bit rows by 8-bit weights
     python -m spyinfer_b200.microbench quantize --rows 2048 [--size 4096] [--dtype float32]
-    python -m spyinfer_b200.microbench step --batch 8 --context 8192 [--layers 4] [--prompt-tokens 2048]      # one step's kernels on the time axis
+    python -m spyinfer_b200.microbench step --batch 8 --context 8192 [--layers 4] [--prompt-tokens 2048] [--int8]   # one step's kernels on the time axis
 
 Defaults are Qwen3-8B's sizes (32 query heads, 8 key/value heads, head size 128, pages of 16).
 Timing is by CUDA events around ``iters`` launches after a warm-up (``--graph``: replayed from a CUDA graph, which
@@ -178,7 +178,7 @@ def bench_rmsnorm(rows: int, size: int, splits: int = 0, iters: int = 20, graph:
     return {"us": ms * 1e3, "gbs": nbytes / ms / 1e6}
 
 
-def step_timeline(batch: int, context: int, layers: int = 4, shape: dict = None, prompt_tokens: int = 0) -> list:
+def step_timeline(batch: int, context: int, layers: int = 4, shape: dict = None, prompt_tokens: int = 0, quantization: str = None) -> list:
     """The kernels of one step of a model with ``layers`` layers of the given layer sizes (default: Qwen3-8B's), as the
     profiler (CUPTI) saw them on the device: ``(name, start µs, duration µs)`` in the order of their starts.  A decode step
     of ``batch`` requests holding ``context`` keys each, replayed from its graph; with ``prompt_tokens`` a prompt of that
@@ -195,7 +195,7 @@ def step_timeline(batch: int, context: int, layers: int = 4, shape: dict = None,
     cfg.update(shape or {})
     page = 16
     tokens = max(context + 16, prompt_tokens + 16)
-    engine = LLMEngine(model_config=config_from_json(cfg), seed=0, dtype="bfloat16", max_num_seqs=max(batch, 1), max_model_len=tokens,
+    engine = LLMEngine(model_config=config_from_json(cfg), seed=0, dtype="bfloat16", quantization=quantization, max_num_seqs=max(batch, 1), max_model_len=tokens,
                        kvcache_block_size=page, num_kvcache_blocks=max(batch, 1) * (tokens // page + 2) + 8, max_num_batched_tokens=max(prompt_tokens, batch, 16))
     runner, cache = engine.runner, engine.runner.cache
     if prompt_tokens:
@@ -270,6 +270,7 @@ def main(argv=None) -> int:
     t.add_argument("--context", type=int, default=8192)
     t.add_argument("--layers", type=int, default=4)
     t.add_argument("--prompt-tokens", type=int, default=0, help="a prompt of this many tokens instead of a decode step")
+    t.add_argument("--int8", action="store_true", help="the layers' products in 8 bits")
     a = sub.add_parser("attention")
     a.add_argument("--batch", type=int, required=True)
     a.add_argument("--context", type=int, required=True)
@@ -298,7 +299,7 @@ def main(argv=None) -> int:
         r = bench_gemm(args.m, args.n, args.k, getattr(torch, args.out_dtype), args.iters, graph=args.graph, defer=args.defer, epilogue=args.epilogue)
         print(f"gemm M={args.m} N={args.n} K={args.k}: {r['us']:.1f} us, {r['tflops']:.1f} TFLOP/s, {r['gbs']:.1f} GB/s")
     elif args.what == "step":
-        print_timeline(step_timeline(args.batch, args.context, args.layers, prompt_tokens=args.prompt_tokens))
+        print_timeline(step_timeline(args.batch, args.context, args.layers, prompt_tokens=args.prompt_tokens, quantization="int8" if args.int8 else None))
         return 0
     elif args.what == "rmsnorm":
         r = bench_rmsnorm(args.rows, args.size, args.splits, args.iters, int8=args.int8)

@@ -30,3 +30,5 @@ def test_microbench_8_bit_commands_run():
     assert "TOP/s" in run("gemm", "--int8", "--m", 300, "--n", 520, "--k", 513, "--iters", 3, "--out-dtype", "float32")
     assert "GB/s" in run("rmsnorm", "--rows", 64, "--size", 1024, "--splits", 3, "--iters", 3, "--int8")
     assert "GB/s" in run("quantize", "--rows", 65, "--size", 1025, "--iters", 3, "--dtype", "float32")
+    out = run("step", "--batch", 2, "--context", 100, "--layers", 1, "--int8")
+    assert "whole step" in out and "gemm_int8_few_kernel" in out
