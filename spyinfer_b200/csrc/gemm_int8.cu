@@ -12,8 +12,8 @@
 // Tails: rows beyond M or N and the end of K are zero-filled by TMA, stores are predicated.  Any K; the rows of A and of W lie a multiple of 16 bytes
 // apart.  No cluster multicast is used.
 //
-// Measured (replayed from a graph, weights cycled past L2; the floor is the bytes at 6,547 GB/s or the operations at 3,279 TOP/s): 1 x 6,144 x 4,096 6.2 us
-// (floor 3.9), 8 x 24,576 x 4,096 gated 18.0 (15.4), 64 x 4,096 x 12,288 13.4 to 14.2 (7.9): the first bytes' way and a microsecond behind the last ones;
+// Measured (replayed from a graph, weights cycled past L2; the floor is the bytes at 6,547 GB/s or the operations at 3,279 TOP/s): 1 x 6,144 x 4,096 6.1 us
+// (floor 3.9), 8 x 24,576 x 4,096 gated 17.6 (15.4), 64 x 4,096 x 12,288 13.2 (7.9): the first bytes' way and a microsecond behind the last ones;
 // 2,048 x 6,144 x 4,096 37.0 (31.4: 2.6 rounds of tiles where 3 are paid), 4,096 x 24,576 x 4,096 gated 242 to 247 (251).
 //
 // The reference has no integer product (its own are half precision: spymaster2h/spyinfer src/backends/cuda/cublas/sgemm.cu:37-55).
@@ -681,18 +681,18 @@ static double few_time(int M, int N, int k_blocks, int bn, int splits, int rows,
     const double even = blocks / sms, most = (double)(((long long)blocks + sms - 1) / sms);
     const double room = splits > 2 ? 1.85 * sms : 2.0 * sms;                          // clusters of 4 and 8 leave some SMs with one block
     const double per_sm = blocks <= room ? fmax(1.0, 0.61 * most + 0.39 * even) : 1.52 * even;      // an SM with one more; the last of many waves is not full
-    double load = (double)N * k_blocks * BK / 1.0e7;                                  // the weights from memory
+    double load = (double)N * k_blocks * BK / 1.2e7;                                  // the weights from memory; some come while what is fixed passes
     load = fmax(load, depth * fmax(0.22, stage / 8.3e4));                             // a block's stages, one after the other: issued, and fetched
     load = fmax(load, per_sm * depth * stage / 1.15e5);                               // an SM's
     const double cut = splits == 1 ? 0.0 : (splits == 2 ? 0.3 : (splits == 4 ? 0.6 : 0.9)) + 2.2 * tokens;      // the sums' way between blocks
-    return 1.95 + cut + 1.8 * tokens + 0.29 * even + load;
+    return 1.95 + cut + 1.8 * tokens + 0.25 * even + load;
 }
 static double pair_time(int M, int N, int k_blocks, int count, int sms)
 {
     const TokenTiles t = token_tiles(M, count);
     const int clusters = sms / 2 > 0 ? sms / 2 : 1;
     const double height = t.rows / 256.0, rounds = (double)(((long long)((N + 2 * BM - 1) / (2 * BM)) * count + clusters - 1) / clusters);
-    const double load = fmax((double)N * k_blocks * BK / 1.0e7, rounds * k_blocks * pair_stage_bytes(t.rows) / 1.12e5);
+    const double load = fmax((double)N * k_blocks * BK / 1.2e7, rounds * k_blocks * pair_stage_bytes(t.rows) / 1.12e5);
     return 6.2 + load + 2.2 * height + 1.8 * (rounds - 1) * height;
 }
 
