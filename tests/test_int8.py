@@ -228,6 +228,27 @@ def test_product_gated(M, N, K):
     assert torch.equal(alone[0], got[M - 1])
 
 
+# a size of each way that a product can be run, by the plan of 148 SMs: tokens a block 16, 32, 64, 128; K whole, cut 2, 4, 8 ways; tiles of 64, 96, 128 weight
+# rows; pairs of blocks with one to five token tiles, even and uneven
+EVERY_WAY = [(72, 14486, 306), (69, 10094, 273), (65, 11354, 2020), (65, 4562, 2090), (65, 1410, 2811), (1, 1278, 271), (1, 100, 267), (1, 130, 517), (1, 132, 1093),
+             (1, 130, 2062), (19, 15348, 262), (18, 15804, 1105), (38, 100, 258), (17, 4972, 1021), (39, 142, 1065), (35, 132, 2246), (33, 14772, 278), (66, 66, 296),
+             (65, 4546, 268), (35, 8786, 2069), (71, 140, 1413), (72, 130, 2414), (139, 29266, 532), (185, 27562, 651), (260, 22444, 709), (739, 8604, 795),
+             (846, 1354, 4280), (258, 16242, 783), (402, 12298, 795), (324, 3958, 3491), (903, 2614, 2055)]
+
+
+@gpu
+@pytest.mark.parametrize("M,N,K", EVERY_WAY)
+def test_product_in_every_way(M, N, K):
+    """Results that leave one by one (N no multiple of 8) and in rows of 16 bytes (N a multiple of 16)."""
+    for n in (N, N + -N % 16):
+        a, w = rows_of_codes(M, K, 5), rows_of_codes(n, K, 6)
+        w = Int8Rows(w.codes, w.scales * (8.0 / K ** 0.5))
+        ref = product_of(a, w)
+        for dtype in (torch.bfloat16, torch.float32):
+            check_product(kernels.gemm_int8(a, w, out_dtype=dtype), ref, dtype)
+        check_gated(kernels.gemm_int8(a, w, epilogue="swiglu", w_settled=True), ref)
+
+
 @gpu
 @pytest.mark.parametrize("M", [3, 140])
 def test_product_of_the_largest_sums(M):
