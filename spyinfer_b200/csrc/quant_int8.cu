@@ -11,10 +11,13 @@
 // approximation, and a test can ask for equality.
 //
 // A row of zeros has codes 0 and scale 0.  A row with a NaN or an infinity has codes 0 and the scale NaN: what is made of it is NaN, and no
-// other row is touched.  |code| <= 127: -128 does not occur.
+// other row is touched.  |code| <= 127: -128 does not occur.  Squares that sum beyond the largest 32-bit number (values from 2^64 / sqrt(len) on) are summed
+// once more of the row times 2^-80, so that finite rows have finite scales that are not 0 (rmsnorm.cu, with the same formula, gives zeros there).
 //
 // Rows of codes lie a multiple of 16 bytes apart (the product fetches them by TMA); bytes between a row's end and the next row are not written.
 // The reference keeps no 8-bit values anywhere (its weights are half precision: spymaster2h/spyinfer src/utils/safetensors_reader.cpp:101-122).
+#include <math.h>
+
 #include "common.cuh"
 
 SPY_MODULE(spy_quant_int8)
@@ -219,6 +222,17 @@ template <bool WITH_SUM> __device__ __forceinline__ void block_reduce(float& sum
     if (WITH_SUM) sum = warp_sum(lane < warps ? __uint_as_float(part[32 + lane]) : 0.f);
 }
 
+// One more sum over the block behind block_reduce, through the same words.
+__device__ __forceinline__ float block_sum_again(float sum, uint32_t* part)
+{
+    const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5, warps = blockDim.x >> 5;
+    sum = warp_sum(sum);
+    __syncthreads();          // every warp has read what block_reduce left
+    if (lane == 0) part[warp] = __float_as_uint(sum);
+    __syncthreads();
+    return warp_sum(lane < warps ? __uint_as_float(part[lane]) : 0.f);
+}
+
 template <typename T, bool WHOLE, int GROUPS>
 __global__ void __launch_bounds__(1024) quantize_kernel(const T* __restrict__ x, long long ldx, int8_t* __restrict__ codes, long long ldc,
                                                         float* __restrict__ scales, int len)
@@ -342,22 +356,35 @@ __global__ void __launch_bounds__(1024) rmsnorm_int8_kernel(TX* x, const TD* __r
             for (int e = 0; e < 8; ++e) v[g][e] = __fadd_rn(v[g][e], d[e]);
         }
     }
-    float ss = 0.f;
+    float ss = 0.f, low = 0.f;       // low: this thread's sum times 2^-160, formed where the sum itself has become infinite
     uint32_t size = 0;
 #pragma unroll
     for (int g = 0; g < GROUPS; ++g) {
         if (write_back) put<WHOLE>(xr, g, len, v[g]);
         float wv[8];
         if constexpr (GROUPS > 1) fetch<WHOLE>(w, g, len, wv);
+        const float before = ss;
+#pragma unroll
+        for (int e = 0; e < 8; ++e) ss += v[g][e] * v[g][e];
+        if (ss == INFINITY) {
+            if (before < INFINITY) low = before * 0x1p-80f * 0x1p-80f;
+#pragma unroll
+            for (int e = 0; e < 8; ++e) low += (v[g][e] * 0x1p-80f) * (v[g][e] * 0x1p-80f);
+        }
 #pragma unroll
         for (int e = 0; e < 8; ++e) {
-            ss += v[g][e] * v[g][e];
             v[g][e] = __fmul_rn(v[g][e], GROUPS > 1 ? wv[e] : w_first[e]);
             size = size_max(size, v[g][e]);
         }
     }
+    if (ss < INFINITY) low = ss * 0x1p-80f * 0x1p-80f;
     block_reduce<true>(ss, size, part);
     encode_row<WHOLE, GROUPS>(codes + (size_t)blockIdx.x * ldc, len, v, size);
+    if (ss == INFINITY && size < 0x7f800000u) {        // the same for the whole block, and rare: the sum again, times 2^-160; eps is nothing beside it
+        const float factor = 0x1p-40f / sqrtf(block_sum_again(low, part) / (float)len);
+        if (threadIdx.x == 0) scales[blockIdx.x] = scale_of(size, factor) * 0x1p-40f;
+        return;
+    }
     if (threadIdx.x == 0) scales[blockIdx.x] = scale_of(size, 1.0f / sqrtf(ss / (float)len + eps));
 }
 

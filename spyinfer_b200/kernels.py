@@ -2196,6 +2196,8 @@ def rmsnorm_int8(x: torch.Tensor, weight: torch.Tensor, eps: float, out: Optiona
     * weight`` in 32 bits: ``code`` is the integer nearest to ``127 y / max |y|`` (as ``quantize_int8``), and the scale ``max |y| / 127 / sqrt(mean((x + delta)^2)
     + eps)``.  ``delta``: x's shape, or a stack ``[splits, rows, len]`` of partial sums that are added in order; ``write_back`` stores the sum into ``x``; ``rows``
     gathers rows of x (and delta); an index outside x gives codes 0 and the scale NaN and is reported in the status word.  Rows of up to 32,768 elements.
+    Finite rows whose squares sum beyond the largest 32-bit number have their scale too, where ``rmsnorm`` gives zeros.  The codes, and for rows of a multiple of
+    8 elements the scale, do not depend on the other rows; the last bit of other rows' scales may differ from 512 rows on (another order of summation).
     ``weight_settled=True``: as ``gemm_int8``'s ``w_settled``, for ``weight``."""
     _check(x, "rmsnorm_int8 input", ndim=2)
     device = _on_current_device(x, "rmsnorm_int8 input")

@@ -496,6 +496,29 @@ def test_rows_of_codes_start_on_borders():
         kernels.rmsnorm_int8(torch.zeros(4, 32), torch.ones(32), 1e-6)
 
 
+@gpu
+@pytest.mark.parametrize("xd,dd", [(torch.float32, torch.bfloat16), (torch.bfloat16, torch.float32)])
+@pytest.mark.parametrize("rows,length", [(8, 1), (8, 72), (8, 1001), (513, 1001), (8, 4096), (8, 5120), (8, 9001), (8, 12288), (8, 20003), (8, 32768)])
+def test_norm_of_rows_whose_squares_exceed_32_bits(rows, length, xd, dd):
+    """Finite rows of which the squares, a thread's sum of them, or only the sum over the row lie beyond the largest 32-bit number, beside ordinary rows: the
+    bound of ``test_norm``, as the sum is only formed of numbers scaled by a power of two."""
+    eps = 1e-6
+    x, w = wild_rows(rows, length, 1), (1 + 0.1 * torch.randn(length, device=DEV).clamp(-3, 3)).to(torch.bfloat16)
+    for r, size in ((0, 3e38), (1, 1e30), (2, 2e19), (3, 1.2e19), (4, 3e18), (5, 4e17)):
+        x[r] = size * (0.3 + 0.4 * torch.rand(length, device=DEV)) * torch.where(torch.rand(length, device=DEV) < 0.5, 1.0, -1.0)
+    x[6, length // 2] = 2e38                      # one such number among ordinary ones
+    x, delta = x.to(xd), (0.01 * wild_rows(rows, length, 2)).to(dd)
+    total = x.float() + delta.float()
+
+    def check(got):
+        check_rows(got, total * w.float(), 1.0 / torch.sqrt(total.double().square().mean(1) + eps), (length / 2 + 4) * 2.0 ** -24)
+        assert bool((got.scales > 0).all())
+
+    check(kernels.rmsnorm_int8(x, w, eps, delta=delta))
+    check(kernels.rmsnorm_int8(x, w, eps, delta=delta, write_back=True))
+    assert torch.equal(x, total.to(xd))
+
+
 # ---- the engine on 8-bit weights ----------------------------------------------------------------------------------------------
 def plain_int8_logits(monkeypatch, weights, cfg, tokens):
     """The plain implementation with every product of the layers on quantised rows and quantised weights, in 32 bits (the sums in 64)."""
