@@ -69,9 +69,14 @@ __device__ __forceinline__ void umma_s8_pair(uint32_t tmem_d, uint64_t desc_a, u
         : "memory");
 }
 
-// silu(g) * u for a bfloat16 result: the fast exponential and division (2 ulp of float each) are far inside the result's rounding.  A gate
-// below -87 gives g / inf = -0, the limit.
-__device__ __forceinline__ float silu_mul(float g, float u) { return __fdividef(g, 1.0f + __expf(-g)) * u; }
+// silu(g) * u = g u / (1 + exp(-g)) for a bfloat16 result.  Below zero it is formed as g exp(g) / (1 + exp(g)): the fast division gives 0 for divisors from
+// 2^126 on, which 1 + exp(-g) is from g = -87.3 down, where a large u still makes a number of it.  The fast exponential is off by about 2 + 1.2 |g| ulp and the
+// division by 2, together below 2^-16 of the result, far inside its rounding; from g = -87.3 down exp(g) is a subnormal number, and the result off by 2^-142 u.
+__device__ __forceinline__ float silu_mul(float g, float u)
+{
+    const float e = __expf(-fabsf(g));
+    return __fdividef(g < 0.f ? g * e : g, 1.0f + e) * u;
+}
 
 // One lane of a warp that has come together, always the same.
 __device__ __forceinline__ bool elect_one()

@@ -519,6 +519,24 @@ def test_norm_of_rows_whose_squares_exceed_32_bits(rows, length, xd, dd):
     assert torch.equal(x, total.to(xd))
 
 
+@gpu
+@pytest.mark.parametrize("M,N,K", [(3, 400, 16), (17, 240, 2062), (70, 1410, 2811), (739, 8604, 795)])
+def test_gates_far_below_zero(M, N, K):
+    """The activation where its exponential leaves 32 bits or nearly does, by every way that results leave: gates from -120 to 100, closely spaced around -88,
+    with ups from small to so large that the tiny activation counts."""
+    gates = torch.cat([torch.linspace(-120, 100, 45), torch.linspace(-90, -85, 51), torch.tensor([0.0, -0.0, -1e-30, 1e-30, -1e30, 1e3])]).to(DEV)
+    ups = torch.tensor([1.0, -3e4, 1e25, -1e33, 1e35], device=DEV)
+    i = torch.arange(N // 2, device=DEV)
+    held = torch.zeros(M + N, (K + 15) // 16 * 16, dtype=torch.int8, device=DEV)
+    held[:M, K - 1] = 1
+    scales = torch.empty(N, device=DEV)
+    for first, of in ((0, gates[i % gates.numel()]), (1, ups[(i // 3) % ups.numel()])):
+        held[M + first::2, K - 1] = (127 * of.sign()).to(torch.int8)
+        scales[first::2] = of.abs() / 127
+    a, w = Int8Rows(held[:M, :K], torch.ones(M, device=DEV)), Int8Rows(held[M:, :K], scales)
+    check_gated(kernels.gemm_int8(a, w, epilogue="swiglu"), product_of(a, w))
+
+
 # ---- the engine on 8-bit weights ----------------------------------------------------------------------------------------------
 def plain_int8_logits(monkeypatch, weights, cfg, tokens):
     """The plain implementation with every product of the layers on quantised rows and quantised weights, in 32 bits (the sums in 64)."""
