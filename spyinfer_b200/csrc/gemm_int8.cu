@@ -375,7 +375,7 @@ gemm_int8_few_kernel(const __grid_constant__ CUtensorMap map_w, const __grid_con
             for (int c = turns * COLS; c < tokens && ok; c += STEP) {
                 uint32_t r[COLS];
                 tmem_load<COLS>(acc + (uint32_t)c, r);
-                tmem_wait_ld();
+                tmem_wait_ld(r);
                 store_chunk<COLS, TC, GATED>(out, ld, lane, x0 + quarter * 32, y0 + c, x_end, M, r, sw, lane < COLS ? sa[c + lane] : 0.f, turn);
             }
         } else {
@@ -386,7 +386,7 @@ gemm_int8_few_kernel(const __grid_constant__ CUtensorMap map_w, const __grid_con
             for (int c = turns * COLS; c < tokens && ok; c += STEP) {
                 uint32_t r[COLS];
                 tmem_load<COLS>(acc + (uint32_t)c, r);
-                tmem_wait_ld();
+                tmem_wait_ld(r);
 #pragma unroll
                 for (int j = 0; j < COLS; j += 4)
                     if (c + j < tokens) store_shared_of(to + (uint32_t)((c + j) / 4 * share) * 16, r[j], r[j + 1], r[j + 2], r[j + 3]);
@@ -618,7 +618,7 @@ gemm_int8_pair_kernel(const __grid_constant__ CUtensorMap map_w, const __grid_co
 #pragma unroll 1
             for (; c < height; c += STEP) {
                 uint32_t r[PAIR_COLS];
-                tmem_wait_ld();
+                tmem_wait_ld(ahead);
 #pragma unroll
                 for (int j = 0; j < PAIR_COLS; ++j) r[j] = ahead[j];
                 const float sa_now = sa;

@@ -537,6 +537,20 @@ def test_gates_far_below_zero(M, N, K):
     check_gated(kernels.gemm_int8(a, w, epilogue="swiglu"), product_of(a, w))
 
 
+def test_waits_for_tensor_memory_name_their_registers():
+    """A load from tensor memory fills registers that may be read behind the wait only, and the pair kernel carries them over a loop's end: every wait of these
+    kernels names them as read and written, so that no read can be moved ahead of it."""
+    from pathlib import Path
+
+    folder = Path(kernels.__file__).parent / "csrc"
+    product, shared = (folder / "gemm_int8.cu").read_text(), (folder / "tcgen05.cuh").read_text()
+    waits = [line.strip() for line in product.splitlines() if "tmem_wait_ld" in line]
+    assert sorted(waits) == ["tmem_wait_ld(ahead);", "tmem_wait_ld(r);", "tmem_wait_ld(r);"]
+    for n in (16, 32):
+        body = shared.split(f"tmem_wait_ld<{n}>", 1)[1].split("}", 1)[0]
+        assert all(f'"+r"(r[{i}])' in body for i in range(n)) and "tcgen05.wait::ld" in body
+
+
 # ---- the engine on 8-bit weights ----------------------------------------------------------------------------------------------
 def plain_int8_logits(monkeypatch, weights, cfg, tokens):
     """The plain implementation with every product of the layers on quantised rows and quantised weights, in 32 bits (the sums in 64)."""
