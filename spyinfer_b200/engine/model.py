@@ -136,7 +136,10 @@ class Model:
         try:
             if self.ctx.dtype == torch.bfloat16:
                 shapes = {d.name: d.shape for d in self.weight_decls()}
-                wide = [n for n, t in tensors.stored_dtypes.items() if len(shapes[n]) == 2 and t in (torch.float32, torch.float16)]
+                # the layers' matrices of a quantised model are held in 8 bits, whatever they are stored as
+                quantised = {layer.prefix + d.name for layer in self.layers for part in layer.parts() if part.ctx.quantization is not None
+                             for d in part.weight_decls()}
+                wide = [n for n, t in tensors.stored_dtypes.items() if len(shapes[n]) == 2 and n not in quantised and t in (torch.float32, torch.float16)]
                 if wide:
                     # a tensor stored in 32-bit stays so, and a 32-bit matrix cannot go to the bfloat16 tensor-core product
                     warnings.warn(f"{model_dir}: {len(wide)} matrices are stored in 32-bit (or 16-bit float, which is widened), the first being "

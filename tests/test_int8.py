@@ -657,3 +657,56 @@ def test_other_architectures_are_refused():
     for config in (BX["a"]["config"], DG["a"]["config"]):
         with pytest.raises(ValueError, match="does not cover"):
             Model(config_from_json(config).to_spec(), torch.bfloat16, None, 256, quantization="int8")
+
+
+def stored_as(folder, weights, cfg, dtype):
+    import json
+    from safetensors.torch import save_file
+    folder.mkdir()
+    (folder / "config.json").write_text(json.dumps(cfg))
+    save_file({k: v.to(dtype).contiguous() for k, v in weights.items()}, str(folder / "model.safetensors"))
+    return str(folder)
+
+
+@pytest.mark.parametrize("name,stay", [("a", 1), ("b", 2)])
+def test_warning_of_wide_matrices_leaves_out_what_is_quantised(name, stay, tiny_models, tmp_path, monkeypatch):
+    """Of a checkpoint in 32 bits (or float16) only the table and the head stay so in a quantised model; its layers' matrices run on the tensor cores."""
+    import warnings
+    from spyinfer_b200 import config_from_json
+    from spyinfer_b200.engine.model import Model
+    _, cfg, weights = tiny_models[name]
+    spec = config_from_json(cfg).to_spec()
+    monkeypatch.setattr(Model, "bind", lambda self, tensors: None)
+    for dtype in (torch.float32, torch.float16, torch.bfloat16):
+        folder = stored_as(tmp_path / str(dtype), weights, cfg, dtype)
+        for quantization in (None, "int8"):
+            with warnings.catch_warnings(record=True) as seen:
+                warnings.simplefilter("always")
+                Model(spec, torch.bfloat16, "cpu", 256, quantization=quantization).load(folder)
+            if dtype == torch.bfloat16:
+                assert not seen
+            else:
+                count = stay if quantization else stay + 7 * cfg["num_hidden_layers"]
+                assert len(seen) == 1 and f": {count} matrices are stored in 32-bit" in str(seen[0].message)
+                assert "embed_tokens" in str(seen[0].message)
+
+
+@gpu
+@pytest.mark.parametrize("dtype", [torch.float32, torch.float16])
+def test_engine_on_a_checkpoint_in_wider_types(dtype, tiny_models, tmp_path, monkeypatch):
+    """The weights are quantised from the numbers as they are stored; the bound of ``test_engine_logits``."""
+    from spyinfer_b200.engine.batch import StepEntry
+    _, cfg, weights = tiny_models["d"]
+    weights = {k: v.float() * (1 + 2.0 ** -9) for k, v in weights.items()}          # not numbers of bfloat16
+    folder = stored_as(tmp_path / "wide", weights, cfg, dtype)
+    g = torch.Generator().manual_seed(9)
+    tokens = torch.randint(0, cfg["vocab_size"], (90,), generator=g).tolist()
+    want = plain_int8_logits(monkeypatch, {k: v.to(dtype).float() for k, v in weights.items()}, cfg, tokens).double()
+    with pytest.warns(UserWarning, match="1 matrices are stored in 32-bit"):
+        engine = int8_engine(folder)
+    got = torch.as_tensor(engine.step_raw([StepEntry("whole", tokens, list(range(90)))])).double()
+    err = (got - want).abs()
+    assert bool(torch.isfinite(got).all())
+    assert float(err.max()) <= 8e-2 * float(want.abs().max()) and float(err.square().mean().sqrt()) <= 4e-2 * float(want.square().mean().sqrt())
+    used = {m for layer in engine.model.layers for p in layer.parts() for m in p.modules()}
+    assert {"gemm_int8", "quant_int8"} <= used and not {"gemm_tcgen05", "gemm_simt"} & used
