@@ -9,6 +9,8 @@
 //   few tokens (gemm_int8_few_kernel): up to 128 weight rows x 16, 32, 64 or 128 tokens a block, two blocks an SM; K may be cut over a cluster of
 //     2, 4 or 8 blocks, which add their integer tiles through distributed shared memory: no scratch, no flags, one launch;
 //   many tokens (gemm_int8_pair_kernel): 256 weight rows x up to 256 tokens on pairs of blocks, persistent, the accumulator double-buffered.
+// The scales are read through pointers without __restrict__, as an earlier kernel may have written them: loads of a const __restrict__ parameter may be moved ahead of
+// the wait for it.
 // Tails: rows beyond M or N and the end of K are zero-filled by TMA, stores are predicated.  Any K; the rows of A and of W lie a multiple of 16 bytes
 // apart.  No cluster multicast is used.
 //
@@ -239,8 +241,8 @@ __device__ __forceinline__ void finish_cut(TC* __restrict__ out, long long ld, c
 // Block (token tile, K range) = (blockIdx.x / splits, blockIdx.x % splits) of weight tile blockIdx.y; the K ranges of a tile are a cluster.
 template <int BN, typename TC, bool GATED>
 __global__ void __launch_bounds__(block_threads(BN), 2)
-gemm_int8_few_kernel(const __grid_constant__ CUtensorMap map_w, const __grid_constant__ CUtensorMap map_a, const float* __restrict__ w_scale,
-                     const float* __restrict__ a_scale, TC* __restrict__ out, long long ld, int N, int M, int k_blocks, int splits, int tile_rows, int settled,
+gemm_int8_few_kernel(const __grid_constant__ CUtensorMap map_w, const __grid_constant__ CUtensorMap map_a, const float* w_scale,
+                     const float* a_scale, TC* __restrict__ out, long long ld, int N, int M, int k_blocks, int splits, int tile_rows, int settled,
                      int* status, const uint8_t* __restrict__ next_weights, long long next_bytes)
 {
     using T = Tile<BN>;
@@ -466,8 +468,8 @@ __host__ __device__ constexpr int pair_stages(int token_rows)
 
 template <typename TC, bool GATED>
 __global__ void __launch_bounds__(PAIR_THREADS, 1)
-gemm_int8_pair_kernel(const __grid_constant__ CUtensorMap map_w, const __grid_constant__ CUtensorMap map_a, const float* __restrict__ w_scale,
-                      const float* __restrict__ a_scale, TC* __restrict__ out, long long ld, int N, int M, int k_blocks, TokenTiles tokens, int num_tiles,
+gemm_int8_pair_kernel(const __grid_constant__ CUtensorMap map_w, const __grid_constant__ CUtensorMap map_a, const float* w_scale,
+                      const float* a_scale, TC* __restrict__ out, long long ld, int N, int M, int k_blocks, TokenTiles tokens, int num_tiles,
                       int settled, int* status)
 {
     const int stages = pair_stages(tokens.rows), stage_bytes = pair_stage_bytes(tokens.rows);   // a lower tile's copies bring spare rows behind its own

@@ -15,6 +15,10 @@
 // once more of the row times 2^-80, so that finite rows have finite scales that are not 0 (rmsnorm.cu, with the same formula, gives zeros there).
 //
 // Rows of codes lie a multiple of 16 bytes apart (the product fetches them by TMA); bytes between a row's end and the next row are not written.
+// What an earlier kernel may have written is read through pointers without __restrict__: of a const __restrict__ parameter the compiler takes it that nothing
+// changes while the kernel runs, and then moves its loads ahead of the wait for the kernels before (pdl_wait), whose blocks this one's run beside.
+// The outputs have it, which is enough for loads to pass stores.
+//
 // The reference keeps no 8-bit values anywhere (its weights are half precision: spymaster2h/spyinfer src/utils/safetensors_reader.cpp:101-122).
 #include <math.h>
 
@@ -234,7 +238,7 @@ __device__ __forceinline__ float block_sum_again(float sum, uint32_t* part)
 }
 
 template <typename T, bool WHOLE, int GROUPS>
-__global__ void __launch_bounds__(1024) quantize_kernel(const T* __restrict__ x, long long ldx, int8_t* __restrict__ codes, long long ldc,
+__global__ void __launch_bounds__(1024) quantize_kernel(const T* x, long long ldx, int8_t* __restrict__ codes, long long ldc,
                                                         float* __restrict__ scales, int len)
 {
     __shared__ uint32_t part[32];
@@ -256,7 +260,7 @@ __global__ void __launch_bounds__(1024) quantize_kernel(const T* __restrict__ x,
 
 // bfloat16 rows of whole groups: the row is kept as it was read, two elements in a register, and the largest size is taken of two at once.
 template <int GROUPS>
-__global__ void __launch_bounds__(1024) quantize_packed_kernel(const bf16* __restrict__ x, long long ldx, int8_t* __restrict__ codes, long long ldc,
+__global__ void __launch_bounds__(1024) quantize_packed_kernel(const bf16* x, long long ldx, int8_t* __restrict__ codes, long long ldc,
                                                                float* __restrict__ scales, int len)
 {
     __shared__ uint32_t part[32];
@@ -288,7 +292,7 @@ __global__ void __launch_bounds__(1024) quantize_packed_kernel(const bf16* __res
 
 // Rows longer than a block holds: read once for the largest size and once more, from L2, for the codes.
 template <typename T>
-__global__ void __launch_bounds__(1024) quantize_long_kernel(const T* __restrict__ x, long long ldx, int8_t* __restrict__ codes, long long ldc,
+__global__ void __launch_bounds__(1024) quantize_long_kernel(const T* x, long long ldx, int8_t* __restrict__ codes, long long ldc,
                                                              float* __restrict__ scales, int len)
 {
     __shared__ uint32_t part[32];
@@ -316,8 +320,8 @@ __global__ void __launch_bounds__(1024) quantize_long_kernel(const T* __restrict
 }
 
 template <typename TX, typename TD, typename TW, bool WHOLE, int GROUPS>
-__global__ void __launch_bounds__(1024) rmsnorm_int8_kernel(TX* x, const TD* __restrict__ delta, int splits, long long split_stride, const int* __restrict__ rows,
-                                                            const TW* __restrict__ w, int8_t* __restrict__ codes, long long ldc,
+__global__ void __launch_bounds__(1024) rmsnorm_int8_kernel(TX* x, const TD* delta, int splits, long long split_stride, const int* rows,
+                                                            const TW* w, int8_t* __restrict__ codes, long long ldc,
                                                             float* __restrict__ scales, int total, int len, float eps, int write_back, int settled, int* status)
 {
     __shared__ uint32_t part[64];
@@ -356,11 +360,14 @@ __global__ void __launch_bounds__(1024) rmsnorm_int8_kernel(TX* x, const TD* __r
             for (int e = 0; e < 8; ++e) v[g][e] = __fadd_rn(v[g][e], d[e]);
         }
     }
+    if (write_back) {        // all of it ahead of the weight's loads, which may not pass a store to x
+#pragma unroll
+        for (int g = 0; g < GROUPS; ++g) put<WHOLE>(xr, g, len, v[g]);
+    }
     float ss = 0.f, low = 0.f;       // low: this thread's sum times 2^-160, formed where the sum itself has become infinite
     uint32_t size = 0;
 #pragma unroll
     for (int g = 0; g < GROUPS; ++g) {
-        if (write_back) put<WHOLE>(xr, g, len, v[g]);
         float wv[8];
         if constexpr (GROUPS > 1) fetch<WHOLE>(w, g, len, wv);
         const float before = ss;
@@ -413,6 +420,8 @@ static int quantize(const T* x, long long ldx, int8_t* codes, long long ldc, flo
     // 2,048 x 12,288 - / 20.5 / 17.4 / 16.2, 24,576 x 4,096 81 / 63.7 / 59.3 / 52.9 (two thirds of the issue slots taken); with halves decided the short way 6.8, 15.3
     // and 49.4 (0.93 of the copy rate) with the groups taken here; of float32 2,048 x 4,096 8.3 / 7.4 / 6.5 (0.98).  Others, float32, 1 / 2 / 4 groups with codes stored one
     // by one: 1,531 x 4,999 20.8 / 12.6 / 14.6, 64 x 4,999 2.6 / 3.7 / 5.4; in words 9.3 and 2.3 with the groups taken here (bfloat16 10.7 and 2.7).
+    // All of that with loads that ran ahead of the wait; where they belong, with the groups taken here: bfloat16 2,048 x 4,096 7.0, 2,048 x 12,288 16.6, 24,576 x 4,096 51.1
+    // (0.90 of the copy rate), 1,531 x 4,999 10.4; float32 2,048 x 4,096 7.8 (0.82), 1,531 x 4,999 9.9.
     const bool packed = whole && sizeof(T) == 2;
     const int groups = row_groups(len, n < 1024 ? 1 : (!whole ? 2 : (packed && (long long)n * len >= (1 << 24) ? 8 : 4))), threads = row_threads(len, groups);
     if constexpr (sizeof(T) == 2) {

@@ -551,6 +551,78 @@ def test_waits_for_tensor_memory_name_their_registers():
         assert all(f'"+r"(r[{i}])' in body for i in range(n)) and "tcgen05.wait::ld" in body
 
 
+# ---- nothing is read before the kernels ahead have ended ------------------------------------------------------------------------
+def behind_a_product(dtype, consume, M=64, N=24576, K=4096):
+    """``consume`` of what a product of some 20 us writes, launched right behind it so that its blocks start beside the product's last ones: one launch after
+    the other and from a captured graph, with other inputs every time and the product's output cleared before.  What it gives has to be, to the last bit, what it
+    gives of the same numbers when nothing runs any more."""
+    a, w = rows_of_codes(M, K, 1), rows_of_codes(N, K, 2)
+    a, w = Int8Rows(a.codes, a.scales * 0.1), w        # results near one
+    z = torch.empty(M, N, dtype=dtype, device=DEV)
+
+    def run():
+        kernels.gemm_int8(a, w, out=z, w_settled=True)
+        return consume(z)
+
+    def flat(out):
+        return [t for p in (out if type(out) in (tuple, list) else (out,)) for t in (p if isinstance(p, Int8Rows) else (p,))]
+
+    run()
+    side = torch.cuda.Stream()
+    torch.cuda.synchronize()
+    with torch.cuda.stream(side):
+        graph = torch.cuda.CUDAGraph()
+        with torch.cuda.graph(graph, stream=side):
+            held = run()
+        for i in range(6):
+            a.codes.copy_(torch.randint(-128, 128, (M, K), device=DEV).to(torch.int8))
+            z.zero_()
+            if i % 2:
+                graph.replay()
+                got = held
+            else:
+                got = run()
+            side.synchronize()
+            want = consume(z.clone())
+            side.synchronize()
+            for g, t in zip(flat(got), flat(want)):
+                assert torch.equal(g, t) or bool(((g == t) | (torch.isnan(g) & torch.isnan(t))).all()), f"pass {i}: {int((g != t).sum())} of {g.numel()} differ"
+
+
+@gpu
+@pytest.mark.parametrize("dtype", [torch.bfloat16, torch.float32])
+@pytest.mark.parametrize("rows,length", [(64, 24576), (96, 16384), (384, 4096), (1536, 1024), (6000, 256), (300, 4999), (1100, 1001), (40, 39000)])
+def test_quantisation_right_behind_what_writes_its_input(rows, length, dtype):
+    behind_a_product(dtype, lambda z: kernels.quantize_int8(z.view(-1)[:rows * length].view(rows, length)))
+
+
+@gpu
+@pytest.mark.parametrize("dtype", [torch.bfloat16, torch.float32])
+@pytest.mark.parametrize("rows,length", [(1, 4096), (64, 8192), (384, 4096), (1500, 1024), (300, 4999), (600, 1001), (40, 32768), (30, 20003), (80, 16392)])
+def test_norm_right_behind_what_writes_its_input(rows, length, dtype):
+    """The stream, the delta, the stacked delta and the weight."""
+    x, weight = wild_rows(rows, length, 3), (1 + 0.1 * torch.randn(length, device=DEV)).to(torch.bfloat16)
+
+    def norms(z):
+        part = z.view(-1)[:rows * length].view(rows, length)
+        half = z.view(-1)[:2 * (rows // 2) * length].view(2, rows // 2, length)
+        return (kernels.rmsnorm_int8(part, weight, 1e-6), kernels.rmsnorm_int8(x, weight, 1e-6, delta=part),
+                kernels.rmsnorm_int8(x[:rows // 2].contiguous(), weight, 1e-6, delta=half) if rows > 1 else kernels.rmsnorm_int8(x, weight, 1e-6))
+
+    behind_a_product(dtype, norms)
+    behind_a_product(dtype, lambda z: kernels.rmsnorm_int8(x, weight, 1e-6, delta=z.view(-1)[:rows * length].view(rows, length)))
+    behind_a_product(dtype, lambda z: kernels.rmsnorm_int8(x, z.view(-1)[-length:], 1e-6))
+
+
+@gpu
+@pytest.mark.parametrize("M,N,K", [(1, 6144, 4096), (64, 4096, 2048), (40, 1000, 300), (300, 9472, 512), (640, 24576, 1024)])
+def test_product_right_behind_what_writes_its_scales(M, N, K):
+    a, w = rows_of_codes(M, K, 3), rows_of_codes(N, K, 4)
+    behind_a_product(torch.float32, lambda z: kernels.gemm_int8(Int8Rows(a.codes, z.view(-1)[-M:]), w, out_dtype=torch.float32))
+    behind_a_product(torch.float32, lambda z: kernels.gemm_int8(a, Int8Rows(w.codes, z.view(-1)[-N:]), out_dtype=torch.float32))
+    behind_a_product(torch.float32, lambda z: kernels.gemm_int8(Int8Rows(a.codes, z.view(-1)[:M]), Int8Rows(w.codes, z.view(-1)[-N:]), epilogue="swiglu"))
+
+
 # ---- the engine on 8-bit weights ----------------------------------------------------------------------------------------------
 def plain_int8_logits(monkeypatch, weights, cfg, tokens):
     """The plain implementation with every product of the layers on quantised rows and quantised weights, in 32 bits (the sums in 64)."""
