@@ -703,9 +703,9 @@ static double pair_time(int M, int N, int k_blocks, int count, int sms)
     return 6.2 + load + 2.2 * height + 1.8 * (rounds - 1) * height;
 }
 
-static Plan choose(int M, int N, int K)
+static Plan choose(int M, int N, int K, int sms)
 {
-    const int k_blocks = (K + BK - 1) / BK, sms = spy_sm_count();
+    const int k_blocks = (K + BK - 1) / BK;
     const int tile = M <= 16 ? 16 : (M <= 32 ? 32 : (M <= 64 ? 64 : 128));
     Plan best = {false, 0, tile, 1, BM};
     double least = 1e30;
@@ -791,7 +791,7 @@ template <typename TC, bool GATED>
 static int run(const void* A, long long lda, const float* a_scale, const void* W, long long ldw, const float* w_scale, void* C, long long ldc, int M, int N,
                int K, int settled, int* status, cudaStream_t stream, const void* next_weights, long long next_bytes)
 {
-    const Plan p = choose(M, N, K);
+    const Plan p = choose(M, N, K, spy_sm_count());
     const int k_blocks = (K + BK - 1) / BK;
     CUtensorMap mw, ma;
     if (p.pairs) {
@@ -830,4 +830,18 @@ extern "C" int spy_gemm_int8(const void* A, long long lda, const float* a_scale,
     if (c_dtype == SPY_BF16) return run<bf16, false>(A, lda, a_scale, W, ldw, w_scale, C, ldc, M, N, K, settled, status, stream, next_weights, next_bytes);
     if (c_dtype == SPY_F32) return run<float, false>(A, lda, a_scale, W, ldw, w_scale, C, ldc, M, N, K, settled, status, stream, next_weights, next_bytes);
     SPY_FAIL("gemm_int8: unknown output dtype code %d", c_dtype);
+}
+
+// How a product of these sizes is run on a device of `sms` SMs; needs no device.  plan[5]: 1 on pairs of blocks; tokens of a tile (the tallest, on pairs);
+// token tiles; ways that K is cut; weight rows of a tile.
+extern "C" int spy_gemm_int8_plan(int M, int N, int K, int sms, int* plan)
+{
+    if (M <= 0 || M > MAX_ROWS || N <= 0 || N > MAX_ROWS || K <= 0 || K > MAX_K || sms <= 0) SPY_FAIL("gemm_int8: no plan for %d x %d x %d on %d SMs", M, N, K, sms);
+    const Plan p = choose(M, N, K, sms);
+    plan[0] = p.pairs ? 1 : 0;
+    plan[1] = p.pairs ? token_tiles(M, p.count).rows : p.bn;
+    plan[2] = p.pairs ? p.count : (M + p.bn - 1) / p.bn;
+    plan[3] = p.splits;
+    plan[4] = p.pairs ? 2 * BM : p.tile_rows;
+    return 0;
 }

@@ -2275,6 +2275,31 @@ def gemm_int8(a: Int8Rows, w: Int8Rows, out: Optional[torch.Tensor] = None, stat
     return out
 
 
+
+class Int8Plan(NamedTuple):
+    """How a product of 8-bit rows is run: on pairs of blocks or on single ones (clusters where K is cut), by tiles of ``tile_tokens`` tokens (on pairs: the
+    tallest; others may have 32 fewer) by ``tile_rows`` weight rows."""
+
+    pairs: bool
+    tile_tokens: int
+    token_tiles: int
+    k_cuts: int
+    tile_rows: int
+
+
+def gemm_int8_plan(M: int, N: int, K: int, sms: Optional[int] = None) -> Int8Plan:
+    """The plan that ``gemm_int8`` follows for ``[M, K] @ [N, K]^T`` on a device of ``sms`` SMs (default: the current device's; given, no device is needed)."""
+    if sms is None:
+        require_cuda()
+        sms = torch.cuda.get_device_properties(torch.cuda.current_device()).multi_processor_count
+    if not all(0 < v <= 0x7fffffff for v in (M, N, K, sms)):
+        raise KernelError(f"gemm_int8: no plan for {M} x {N} x {K} on {sms} SMs")
+    plan = (ctypes.c_int * 5)()
+    if build.load("gemm_int8").spy_gemm_int8_plan(ctypes.c_int(M), ctypes.c_int(N), ctypes.c_int(K), ctypes.c_int(sms), plan) != 0:
+        raise KernelError(build.last_error("gemm_int8"))
+    return Int8Plan(plan[0] == 1, *plan[1:])
+
+
 _int8_status = {}        # device index -> its status word
 
 

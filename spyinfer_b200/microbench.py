@@ -291,7 +291,10 @@ def main(argv=None) -> int:
         if args.defer:
             ap.error("the 8-bit product always sums its parts")
         r = bench_gemm_int8(args.m, args.n, args.k, getattr(torch, args.out_dtype), args.iters, graph=args.graph, epilogue=args.epilogue)
-        print(f"int8 gemm M={args.m} N={args.n} K={args.k}: {r['us']:.1f} us, {r['tops']:.1f} TOP/s, {r['gbs']:.1f} GB/s")
+        p = kernels.gemm_int8_plan(args.m, args.n, args.k)
+        how = "pairs of blocks" if p.pairs else "single blocks" + (f", K cut {p.k_cuts} ways" if p.k_cuts > 1 else "")
+        print(f"int8 gemm M={args.m} N={args.n} K={args.k}: {r['us']:.1f} us, {r['tops']:.1f} TOP/s, {r['gbs']:.1f} GB/s "
+              f"({how}, {p.token_tiles} tiles of {p.tile_tokens} tokens by {p.tile_rows} weight rows)")
     elif args.what == "quantize":
         r = bench_quantize(args.rows, args.size, getattr(torch, args.dtype), args.iters)
         print(f"quantize rows={args.rows} size={args.size} {args.dtype}: {r['us']:.1f} us, {r['gbs']:.1f} GB/s")

@@ -230,6 +230,8 @@ def test_product_gated(M, N, K):
 
 # a size of each way that a product can be run, by the plan of 148 SMs: tokens a block 16, 32, 64, 128; K whole, cut 2, 4, 8 ways; tiles of 64, 96, 128 weight
 # rows; pairs of blocks with one to five token tiles, even and uneven
+# (by the plan as it is now these reach pairs with 1, 2, 3, 4, 6 and 9 token tiles of 96, 160 and 192 tokens, and single blocks but for 128 tokens by 64 weight rows;
+# MORE_WAYS below has the rest, and test_sizes_reach_every_plan fails when a change of the plan leaves a way without a size)
 EVERY_WAY = [(72, 14486, 306), (69, 10094, 273), (65, 11354, 2020), (65, 4562, 2090), (65, 1410, 2811), (1, 1278, 271), (1, 100, 267), (1, 130, 517), (1, 132, 1093),
              (1, 130, 2062), (19, 15348, 262), (18, 15804, 1105), (38, 100, 258), (17, 4972, 1021), (39, 142, 1065), (35, 132, 2246), (33, 14772, 278), (66, 66, 296),
              (65, 4546, 268), (35, 8786, 2069), (71, 140, 1413), (72, 130, 2414), (139, 29266, 532), (185, 27562, 651), (260, 22444, 709), (739, 8604, 795),
@@ -621,6 +623,210 @@ def test_product_right_behind_what_writes_its_scales(M, N, K):
     behind_a_product(torch.float32, lambda z: kernels.gemm_int8(Int8Rows(a.codes, z.view(-1)[-M:]), w, out_dtype=torch.float32))
     behind_a_product(torch.float32, lambda z: kernels.gemm_int8(a, Int8Rows(w.codes, z.view(-1)[-N:]), out_dtype=torch.float32))
     behind_a_product(torch.float32, lambda z: kernels.gemm_int8(Int8Rows(a.codes, z.view(-1)[:M]), Int8Rows(w.codes, z.view(-1)[-N:]), epilogue="swiglu"))
+
+
+# ---- which way a product is run ------------------------------------------------------------------------------------------------
+SMS = 148
+
+
+def way_of(M, N, K, sms=SMS):
+    """Pairs: the tallest token tile, and whether others are lower.  Single blocks: tokens, ways that K is cut, and weight rows."""
+    p = kernels.gemm_int8_plan(M, N, K, sms)
+    return ("pairs", p.tile_tokens, (M + 31) // 32 % p.token_tiles != 0) if p.pairs else ("single", p.tile_tokens, p.k_cuts, p.tile_rows)
+
+
+# what the sizes above leave out: the heights of the pairs' token tiles (64 to 256, even and uneven; from 96 on most with three or more tiles a pair, the last
+# one ragged), a ring of six stages filled several times, and 128 tokens by 64 weight rows
+MORE_WAYS = {(6731, 312, 434): ("single", 128, 1, 64), (368, 2836, 9251): ("pairs", 64, False), (131, 6142, 8246): ("pairs", 64, True),
+             (162, 26036, 776): ("pairs", 96, False), (1283, 964, 3966): ("pairs", 96, True), (495, 13620, 977): ("pairs", 128, False),
+             (477, 14008, 993): ("pairs", 128, True), (138, 50300, 280): ("pairs", 160, False), (274, 26346, 514): ("pairs", 160, True),
+             (171, 55968, 286): ("pairs", 192, False), (660, 13970, 536): ("pairs", 192, True), (665, 17436, 407): ("pairs", 224, False),
+             (393, 27334, 404): ("pairs", 224, True), (748, 18690, 426): ("pairs", 256, False), (907, 13986, 397): ("pairs", 256, True),
+             (2041, 6150, 2200): ("pairs", 256, False), (1000, 8192, 2048): ("pairs", 256, False)}
+
+
+def test_plan_of_a_product():
+    """What the plan says fits the sizes, and sizes that the product refuses have none."""
+    import random
+    rng = random.Random(2)
+    for _ in range(2000):
+        M, N, K = (max(1, round(top ** rng.random())) for top in (8192, 60000, 20000))
+        p = kernels.gemm_int8_plan(M, N, K, SMS)
+        if p.pairs:
+            runs = (M + 31) // 32
+            assert p.tile_tokens % 32 == 0 and 32 <= p.tile_tokens <= 256 and p.k_cuts == 1 and p.tile_rows == 256
+            assert p.tile_tokens == 32 * -(-runs // p.token_tiles) and runs >= p.token_tiles
+        else:
+            assert p.tile_tokens in (16, 32, 64, 128) and p.token_tiles == -(-M // p.tile_tokens) and p.tile_rows in (64, 96, 128)
+            assert p.k_cuts == 1 or (p.k_cuts in (2, 4, 8) and p.tile_rows == 128 and K > 128 * (2 * p.k_cuts - 1))
+    for M, N, K, sms in ((0, 1, 1, SMS), (1, 0, 1, SMS), (1, 1, 0, SMS), (1, 1, 131072, SMS), (1, 1, 1, 0), (2 ** 22 + 1, 1, 1, SMS), (1, 2 ** 40, 1, SMS)):
+        with pytest.raises(KernelError, match="no plan"):
+            kernels.gemm_int8_plan(M, N, K, sms)
+
+
+def test_sizes_reach_every_plan():
+    """The plan changes with its constants: the sizes of this file's product tests have to go every way that a product of random sizes goes."""
+    import random
+    for size, way in MORE_WAYS.items():
+        assert way_of(*size) == way
+    tested = {way_of(M, n, K) for M, N, K in SHAPES + EVERY_WAY + list(MORE_WAYS) for n in (N, N + N % 2)}
+    rng = random.Random(4)
+    found = set()
+    for _ in range(20000):
+        found.add(way_of(*(max(low, round(low * (high / low) ** rng.random())) for low, high in ((1, 8192), (1, 60000), (1, 20000)))))
+    assert len(found) >= 30 and not found - tested, found - tested
+
+
+@gpu
+@pytest.mark.parametrize("M,N,K", list(MORE_WAYS))
+def test_product_in_more_ways(M, N, K):
+    """As ``test_product_in_every_way``; and a token alone, which goes another way, gives the same bits."""
+    assert way_of(M, N, K, torch.cuda.get_device_properties(0).multi_processor_count) == MORE_WAYS[M, N, K]
+    a, w = rows_of_codes(M, K, 5), rows_of_codes(N, K, 6)
+    w = Int8Rows(w.codes, w.scales * (8.0 / K ** 0.5))
+    ref = product_of(a, w)
+    outs = {}
+    for dtype in (torch.bfloat16, torch.float32):
+        outs[dtype] = kernels.gemm_int8(a, w, out_dtype=dtype)
+        check_product(outs[dtype], ref, dtype)
+    gated = kernels.gemm_int8(a, w, epilogue="swiglu", w_settled=True)
+    check_gated(gated, ref)
+    for t in (0, 37, M // 2, M - 1):
+        alone = Int8Rows(a.codes[t:t + 1], a.scales[t:t + 1])
+        assert not kernels.gemm_int8_plan(1, N, K).pairs
+        for dtype in outs:
+            assert torch.equal(kernels.gemm_int8(alone, w, out_dtype=dtype)[0], outs[dtype][t])
+        assert torch.equal(kernels.gemm_int8(alone, w, epilogue="swiglu")[0], gated[t])
+
+
+# ---- what the other tests ask of a product, of products on pairs of blocks --------------------------------------------------------
+@gpu
+def test_pairs_scales_and_views():
+    """As ``test_product_scales_and_views``."""
+    M, N, K = 1000, 8192, 1024
+    assert kernels.gemm_int8_plan(M, N, K).pairs
+    a, w = rows_of_codes(M, 1400, 1), rows_of_codes(N, 1400, 2)
+    a, w = Int8Rows(a.codes[:, 32:32 + K], a.scales), Int8Rows(w.codes[:, 176:176 + K], w.scales)
+    check_product(kernels.gemm_int8(a, w), product_of(a, w), torch.bfloat16)
+    a.scales[1], a.scales[2], w.scales[7] = float("nan"), 0.0, 0.0
+    keep = torch.arange(M, device=DEV) != 1
+    got, ref = kernels.gemm_int8(a, w, out_dtype=torch.float32), product_of(a, w)
+    assert bool(torch.isnan(got[1]).all())
+    check_product(got[keep], ref[keep], torch.float32)
+    gated = kernels.gemm_int8(a, w, epilogue="swiglu")
+    assert bool(torch.isnan(gated[1]).all())
+    check_gated(gated[keep], ref[keep])
+
+
+@gpu
+def test_pairs_in_a_feed_forward_captured_and_replayed():
+    """As ``test_a_feed_forward``: both products on pairs, run, captured on another stream and replayed with new inputs."""
+    M, H, inter, eps = 1100, 2048, 5120, 1e-6
+    assert kernels.gemm_int8_plan(M, 2 * inter, H).pairs and kernels.gemm_int8_plan(M, H, inter).pairs
+    x, delta = wild_rows(M, H, 1), wild_rows(M, H, 2).to(torch.bfloat16)
+    norm = (1 + 0.1 * torch.randn(H, device=DEV)).to(torch.bfloat16)
+    gate_up = kernels.quantize_int8((torch.randn(2 * inter, H, device=DEV) / H ** 0.5).to(torch.bfloat16))
+    down = kernels.quantize_int8((torch.randn(H, inter, device=DEV) / inter ** 0.5).to(torch.bfloat16))
+
+    def run(stream):
+        rows = kernels.rmsnorm_int8(stream, norm, eps, delta=delta, write_back=True)
+        z = kernels.gemm_int8(rows, gate_up, epilogue="swiglu")
+        mid = kernels.quantize_int8(z)
+        return rows, z, mid, kernels.gemm_int8(mid, down)
+
+    def parts(out):
+        return [t for p in out for t in (p if isinstance(p, Int8Rows) else (p,))]
+
+    stream = x.clone()
+    rows, z, mid, y = run(stream)
+    check_gated(z, product_of(rows, gate_up))
+    check_rows(mid, z.float())
+    check_product(y, product_of(mid, down), torch.bfloat16)
+    side = torch.cuda.Stream()
+    side.wait_stream(torch.cuda.current_stream())
+    with torch.cuda.stream(side):
+        stream.copy_(x)
+        graph = torch.cuda.CUDAGraph()
+        with torch.cuda.graph(graph, stream=side):
+            held = run(stream)
+        for seed in (5, 6):
+            stream.copy_(wild_rows(M, H, seed))
+            fresh = stream.clone()
+            graph.replay()
+            assert all(torch.equal(s, t) for s, t in zip(parts(held), parts(run(fresh)))) and torch.equal(stream, fresh)
+    torch.cuda.current_stream().wait_stream(side)
+    assert kernels.status_word(torch.device(DEV)).tolist() == [0, 0]
+
+
+@gpu
+def test_pairs_behind_the_quantisation_of_their_weight():
+    """As ``test_weights_quantised_by_the_call_ahead``."""
+    M, N, K = 640, 24576, 1024
+    assert kernels.gemm_int8_plan(M, N, K).pairs
+    x = wild_rows(M, K, 1).to(torch.bfloat16)
+    w = kernels.empty_int8(N, K, DEV)
+    weights = [torch.randn(N, K, device=DEV).to(torch.bfloat16) * (i + 1) for i in range(3)]
+    outs = []
+    for i in range(9):
+        kernels.quantize_int8(weights[i % 3], w)
+        outs.append(kernels.gemm_int8(kernels.quantize_int8(x), w, out_dtype=torch.float32))
+    for i in range(3):
+        kernels.quantize_int8(weights[i], w)
+        a = kernels.quantize_int8(x)
+        torch.cuda.synchronize()
+        check_product(outs[i], product_of(a, w), torch.float32)
+        assert torch.equal(outs[i], outs[i + 3]) and torch.equal(outs[i], outs[i + 6])
+        assert torch.equal(outs[i], kernels.gemm_int8(a, w, out_dtype=torch.float32, w_settled=True))
+
+
+@gpu
+def test_pairs_of_a_layer_called_as_soon_as_it_is_made():
+    """As ``test_layer_called_as_soon_as_it_is_made``."""
+    from spyinfer_b200.parts.linear import Int8Linear
+
+    M, N, K = 400, 20000, 1024
+    assert kernels.gemm_int8_plan(M, N, K).pairs
+    a = kernels.quantize_int8(wild_rows(M, K, 1).to(torch.bfloat16))
+    torch.cuda.synchronize()
+    side = torch.cuda.Stream()
+    for i in range(3):
+        weight = torch.randn(N, K, device=DEV) * (i + 1)
+        layer = Int8Linear(weight)
+        with torch.cuda.stream(side):
+            outs = [layer(a, out_dtype=torch.float32)]
+        outs += [layer(a, out_dtype=torch.float32) for _ in range(3)]
+        torch.cuda.synchronize()
+        want = product_of(a, kernels.quantize_int8(weight))
+        for out in outs:
+            check_product(out, want, torch.float32)
+        del layer, weight
+
+
+@gpu
+def test_pairs_on_two_streams_at_once():
+    """As ``test_two_streams_at_once``: products on pairs on both streams."""
+    sides = [torch.cuda.Stream(), torch.cuda.Stream()]
+    jobs = []
+    for i, (M, N, K) in enumerate(((1100, 10240, 2048), (400, 20000, 1024))):
+        assert kernels.gemm_int8_plan(M, N, K).pairs
+        jobs.append((wild_rows(M, K, i), wild_rows(M, K, i + 5).to(torch.bfloat16), torch.ones(K, device=DEV),
+                     kernels.quantize_int8(torch.randn(N, K, device=DEV).to(torch.bfloat16))))
+
+    def run(job):
+        x, d, g, w = job
+        return kernels.quantize_int8(kernels.gemm_int8(kernels.rmsnorm_int8(x, g, 1e-6, delta=d), w))
+
+    alone = [run(j) for j in jobs]
+    torch.cuda.synchronize()
+    got = [[], []]
+    for _ in range(10):
+        for i, side in enumerate(sides):
+            with torch.cuda.stream(side):
+                got[i].append(run(jobs[i]))
+    torch.cuda.synchronize()
+    for i in range(2):
+        assert all(torch.equal(r.codes, alone[i].codes) and torch.equal(r.scales, alone[i].scales) for r in got[i])
+    assert kernels.status_word(torch.device(DEV)).tolist() == [0, 0]
 
 
 # ---- the engine on 8-bit weights ----------------------------------------------------------------------------------------------
