@@ -44,9 +44,9 @@ template <> struct Vec4<bf16> {
 
 template <typename TA, typename TC>
 __global__ void __launch_bounds__(CHUNK)
-attention_generic_kernel(const TA* __restrict__ q, long long q_row_stride, TA* __restrict__ out, const TC* __restrict__ pages,
-                         const int* __restrict__ block_table, int table_width, int page_size, int num_pages, int nh, int nkv, int hd,
-                         const int* __restrict__ positions, const int* __restrict__ seq_of_token, int window, float scale, int* status, int planes,
+attention_generic_kernel(const TA* q, long long q_row_stride, TA* __restrict__ out, const TC* pages,
+                         const int* block_table, int table_width, int page_size, int num_pages, int nh, int nkv, int hd,
+                         const int* positions, const int* seq_of_token, int window, float scale, int* status, int planes,
                          int keep_first, int sink, SpyScores sc)
 {
     extern __shared__ float smem[];
@@ -312,7 +312,7 @@ template <int LEFT> __device__ __forceinline__ void copy_wait() { asm volatile("
 
 template <typename TA, typename TC, int R, int GROUPS>
 __global__ void __launch_bounds__(CHUNK, 4)
-attention_rows_kernel(const TA* __restrict__ q, TA* __restrict__ out, const TC* __restrict__ pages, AttnArgs A)
+attention_rows_kernel(const TA* q, TA* __restrict__ out, const TC* pages, AttnArgs A)
 {
     constexpr int RG = R / GROUPS, DG = CHUNK / GROUPS;     // rows of a group of threads, dimensions it takes
     constexpr int PLD = R == 4 ? 4 : R + 4;                // four lanes' quads of probabilities meet no bank twice
@@ -615,7 +615,7 @@ __device__ __forceinline__ float reduce_four(float (&v)[4], int* row)
 
 template <typename TA, typename TC>
 __global__ void __launch_bounds__(WIDE_THREADS, 2)
-attention_wide_kernel(const TA* __restrict__ q, TA* __restrict__ out, const TC* __restrict__ pages, AttnArgs A)
+attention_wide_kernel(const TA* q, TA* __restrict__ out, const TC* pages, AttnArgs A)
 {
     constexpr int R = WIDE_ROWS, PLD = WIDE_PLD;
     extern __shared__ __align__(16) float sm[];

@@ -45,9 +45,9 @@ template <> struct Vec4<bf16> {
 constexpr int POOL_TOKENS = 16;
 
 template <typename TC>
-__global__ void pool_store_kernel(const TC* __restrict__ pages, int num_pages, const int* __restrict__ block_table, TC* __restrict__ pooled,
-                                  int num_pooled_pages, const int* __restrict__ pool_table, int table_width, int page_size, int nkv, int hd, int pool,
-                                  const int* __restrict__ positions, const int* __restrict__ seq_of_token, int tokens, int* status)
+__global__ void pool_store_kernel(const TC* pages, int num_pages, const int* block_table, TC* __restrict__ pooled,
+                                  int num_pooled_pages, const int* pool_table, int table_width, int page_size, int nkv, int hd, int pool,
+                                  const int* positions, const int* seq_of_token, int tokens, int* status)
 {
     extern __shared__ float part[];   // [groups][hd]
     __shared__ int pos_s[POOL_TOKENS];
@@ -127,10 +127,10 @@ extern "C" int spy_pool_store(const void* pages, int num_pages, const int* block
 // ---- attention -------------------------------------------------------------------------------------
 template <typename TA, typename TC>
 __global__ void __launch_bounds__(CHUNK)
-attention_pool_kernel(const TA* __restrict__ q, long long q_row_stride, TA* __restrict__ out, const TC* __restrict__ pages, int num_pages,
-                      const int* __restrict__ block_table, const TC* __restrict__ pooled, int num_pooled_pages, const int* __restrict__ pool_table,
-                      int table_width, int page_size, int nh, int nkv, int hd, const int* __restrict__ positions, const int* __restrict__ seq_of_token,
-                      int window, int pool, float scale, const float* __restrict__ lse, int* status)
+attention_pool_kernel(const TA* q, long long q_row_stride, TA* __restrict__ out, const TC* pages, int num_pages,
+                      const int* block_table, const TC* pooled, int num_pooled_pages, const int* pool_table,
+                      int table_width, int page_size, int nh, int nkv, int hd, const int* positions, const int* seq_of_token,
+                      int window, int pool, float scale, const float* lse, int* status)
 {
     extern __shared__ float smem[];
     pdl_enter();

@@ -86,6 +86,9 @@ static inline int spy_sm_count()
 // prologue.  A kernel may do work that depends on no other kernel before its wait: the
 // tensor-core product uses that to prefetch weights.  SPYINFER_PDL=0 in the environment
 // turns the attribute off (the two instructions are then no-ops).
+// What another kernel may have written is read through pointers WITHOUT __restrict__ (and not by __ldg): of a const __restrict__ parameter the compiler
+// takes it that nothing changes while the kernel runs, whoever writes it, and may move its loads ahead of pdl_wait().  __restrict__ is for weights
+// and tables, which are there before the first launch, and for outputs that are only written: with these alone loads may still pass stores.
 static thread_local cudaError_t g_spy_launch_error = cudaSuccess;
 
 static inline bool spy_pdl_enabled()

@@ -65,7 +65,7 @@ struct ConvArgs {
 
 // V neighbouring columns of a projection row, its parts summed
 template <int V, typename TP>
-__device__ __forceinline__ void columns(const TP* __restrict__ row, int splits, long long split_stride, float (&v)[V])
+__device__ __forceinline__ void columns(const TP* row, int splits, long long split_stride, float (&v)[V])
 {
     take<V>(row, v);
     float p[V];
@@ -79,7 +79,7 @@ __device__ __forceinline__ void columns(const TP* __restrict__ row, int splits, 
 
 template <typename TP, typename TQ, int V, int MAXT>
 __global__ void __launch_bounds__(128)
-conv_qkv_kernel(const TP* __restrict__ proj, TQ* __restrict__ q_out, TQ* __restrict__ pages, ConvArgs A)
+conv_qkv_kernel(const TP* proj, TQ* __restrict__ q_out, TQ* __restrict__ pages, ConvArgs A)
 {
     constexpr int PIECE = piece_of(MAXT);
     __shared__ float temp_s[PIECE];          // what a token's queries are multiplied by

@@ -17,10 +17,10 @@
 SPY_MODULE(spy_diff_attention)
 
 template <typename TP, typename TB, typename TW, typename TQ, typename TC>
-__global__ void diff_qkv_store_kernel(const TP* __restrict__ proj, long long ld, int q_col, int k_col, int v_col, const TB* __restrict__ bias,
+__global__ void diff_qkv_store_kernel(const TP* proj, long long ld, int q_col, int k_col, int v_col, const TB* __restrict__ bias,
                                       const TW* __restrict__ q_weight, const TW* __restrict__ k_weight, float eps, const float* __restrict__ rope,
-                                      int rot_half, int table_rows, const int* __restrict__ positions, const int* __restrict__ seq_of_token,
-                                      TQ* __restrict__ q_out, const int* __restrict__ block_table, int table_width, TC* __restrict__ pages,
+                                      int rot_half, int table_rows, const int* positions, const int* seq_of_token,
+                                      TQ* __restrict__ q_out, const int* block_table, int table_width, TC* __restrict__ pages,
                                       int page_size, int num_pages, int heads, int kv_heads, int dim, int vdim, int hd, int* status)
 {
     pdl_enter();
@@ -138,7 +138,7 @@ extern "C" int spy_diff_qkv_store(const void* proj, int proj_dtype, long long ld
 }
 
 template <typename TA, typename TG, typename TO>
-__global__ void diff_combine_kernel(const TA* __restrict__ attn, int hd, const TG* __restrict__ gate, long long gate_ld, int gate_col,
+__global__ void diff_combine_kernel(const TA* attn, int hd, const TG* gate, long long gate_ld, int gate_col,
                                     TO* __restrict__ out, int tokens, int heads, int vdim, float lambda, float post, float eps)
 {
     pdl_enter();

@@ -51,8 +51,8 @@ struct Tanh {
 // ROWS rows a block (1; 4 when there are many): a thread's weights are loaded once for all of them, and their inputs are under way together.
 template <typename TY, typename TW, typename TO, int V, int ROWS>
 __global__ void __launch_bounds__(THREADS)
-dynamic_tanh_kernel(float* __restrict__ hidden, const TY* __restrict__ y, int splits, long long split_stride, Tanh ty, float y_scale,
-                    const int* __restrict__ rows, Tanh tx, TO* __restrict__ out, int n, int len, int write_back)
+dynamic_tanh_kernel(float* hidden, const TY* y, int splits, long long split_stride, Tanh ty, float y_scale,
+                    const int* rows, Tanh tx, TO* __restrict__ out, int n, int len, int write_back)
 {
     pdl_launch_dependents();
     const int i = (blockIdx.y * THREADS + threadIdx.x) * V;

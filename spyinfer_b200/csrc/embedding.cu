@@ -6,7 +6,7 @@
 SPY_MODULE(spy_embedding)
 
 template <typename TW>
-__global__ void embedding_kernel(const TW* __restrict__ table, const int* __restrict__ ids, float* __restrict__ out,
+__global__ void embedding_kernel(const TW* __restrict__ table, const int* ids, float* __restrict__ out,
                                  int hidden, int vocab, int* status)
 {
     pdl_enter();
@@ -40,10 +40,10 @@ extern "C" int spy_embedding(const void* table, int table_dtype, const int* ids,
 // The previous token of a portion's first token is the sequence's state: prev_state[state_slot[seq]], which the block of
 // that first token reads and then overwrites with the portion's last token (one thread does both, so the order holds).
 template <typename TW, typename TP>
-__global__ void embedding_pairs_kernel(const TW* __restrict__ table, const TP* __restrict__ pairs, const int* __restrict__ ids, float* __restrict__ out,
+__global__ void embedding_pairs_kernel(const TW* __restrict__ table, const TP* __restrict__ pairs, const int* ids, float* __restrict__ out,
                                        int hidden, int vocab, float scale, long long buckets, long long mul_prev, long long mul_cur,
-                                       const int* __restrict__ positions, const int* __restrict__ seq_of_token, const int* __restrict__ q_start,
-                                       const int* __restrict__ state_slot, int* prev_state, int num_slots, int* status)
+                                       const int* positions, const int* seq_of_token, const int* q_start,
+                                       const int* state_slot, int* prev_state, int num_slots, int* status)
 {
     __shared__ long long row_s;
     pdl_enter();
@@ -78,7 +78,7 @@ __global__ void embedding_pairs_kernel(const TW* __restrict__ table, const TP* _
 }
 
 template <typename TW>
-__global__ void embedding_scaled_kernel(const TW* __restrict__ table, const int* __restrict__ ids, float* __restrict__ out, int hidden, int vocab,
+__global__ void embedding_scaled_kernel(const TW* __restrict__ table, const int* ids, float* __restrict__ out, int hidden, int vocab,
                                         float scale, int* status)
 {
     pdl_enter();
@@ -125,7 +125,7 @@ extern "C" int spy_embedding_scaled(const void* table, int table_dtype, const in
 // stream[t, :] += table[ids[t], :] + row[:]  (either term optional), in 32-bit: a model that adds its embedding output, or a
 // learned offset, to the residual stream again at a later point of its depth.
 template <typename TW, typename TR>
-__global__ void stream_add_kernel(float* __restrict__ stream, const TW* __restrict__ table, const int* __restrict__ ids, const TR* __restrict__ row,
+__global__ void stream_add_kernel(float* stream, const TW* __restrict__ table, const int* ids, const TR* __restrict__ row,
                                   int hidden, int vocab, int* status)
 {
     pdl_enter();
@@ -167,7 +167,7 @@ extern "C" int spy_stream_add(float* stream, const void* table, int table_dtype,
 // out[t, :] = [stream[t, :] | table[ids[t], :] * scale]: the input of a projection that takes the stream and the embedding output
 // side by side.
 template <typename TW, typename TO>
-__global__ void stream_concat_kernel(const float* __restrict__ stream, const TW* __restrict__ table, const int* __restrict__ ids, float scale,
+__global__ void stream_concat_kernel(const float* stream, const TW* __restrict__ table, const int* ids, float scale,
                                      TO* __restrict__ out, int hidden, int vocab, int* status)
 {
     pdl_enter();
@@ -201,8 +201,8 @@ extern "C" int spy_stream_concat(const float* stream, const void* table, int tab
 // through by a gate that was projected from the stream; gate [T, dim] or a stack of split-K partial sums.  act: 0 the tanh form of gelu.
 template <typename TG, typename TW, typename TO>
 __global__ void __launch_bounds__(128)
-token_gate_kernel(const TG* __restrict__ gate, int splits, long long split_stride, const TW* __restrict__ table, long long table_ld, int col,
-                  const int* __restrict__ ids, int vocab, TO* __restrict__ out, int dim, int* status)
+token_gate_kernel(const TG* gate, int splits, long long split_stride, const TW* __restrict__ table, long long table_ld, int col,
+                  const int* ids, int vocab, TO* __restrict__ out, int dim, int* status)
 {
     pdl_enter();
     const int t = blockIdx.x;

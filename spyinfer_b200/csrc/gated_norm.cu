@@ -25,7 +25,7 @@ template <typename TO> __device__ __forceinline__ void store4(TO* p, const float
 
 // VEC: head sizes, pitch and columns are multiples of four; a row of up to 512 elements stays in registers between the two passes
 template <typename TO, bool VEC>
-__global__ void gated_head_norm_kernel(const float* __restrict__ o, const float* __restrict__ proj, long long ld, int off_g, const float* __restrict__ weight,
+__global__ void gated_head_norm_kernel(const float* o, const float* proj, long long ld, int off_g, const float* __restrict__ weight,
                                        TO* __restrict__ out, long long rows, int H, int dv, float eps, int gate_act)
 {
     pdl_enter();
@@ -94,7 +94,7 @@ extern "C" int spy_gated_head_norm(const float* o, const float* proj, long long 
 // weight.  One block a (token, part); the products stay in shared memory between the two passes.
 template <typename TO, int V>
 __global__ void __launch_bounds__(256)
-gate_group_norm_kernel(const float* __restrict__ o, const float* __restrict__ proj, long long ld, int off_g, const float* __restrict__ weight,
+gate_group_norm_kernel(const float* o, const float* proj, long long ld, int off_g, const float* __restrict__ weight,
                        TO* __restrict__ out, int size, int groups, float eps)
 {
     extern __shared__ __align__(16) float y_s[];

@@ -15,9 +15,9 @@ __device__ __forceinline__ float sigmoidf_(float v) { return 1.0f / (1.0f + expf
 constexpr int SCAN_SLICED_FROM = 16;      // a step whose longest run has more tokens than this is scanned in slices
 
 template <typename TB, typename TO>
-__global__ void mingru_scan_kernel(const float* __restrict__ proj, long long ld, int z_col, int x_col, int g_col, const TB* __restrict__ z_bias,
-                                   const TB* __restrict__ x_bias, float* __restrict__ state, const int* __restrict__ q_start,
-                                   const int* __restrict__ state_slot, TO* __restrict__ out, int width)
+__global__ void mingru_scan_kernel(const float* proj, long long ld, int z_col, int x_col, int g_col, const TB* __restrict__ z_bias,
+                                   const TB* __restrict__ x_bias, float* state, const int* q_start,
+                                   const int* state_slot, TO* __restrict__ out, int width)
 {
     pdl_enter();
     const int c = blockIdx.x * blockDim.x + threadIdx.x, seq = blockIdx.y;
@@ -45,9 +45,9 @@ __global__ void mingru_scan_kernel(const float* __restrict__ proj, long long ld,
 // then walks its tokens again from there in order.  Blocks of 32 channels x TS slices.
 template <typename TB, typename TO, int TS>
 __global__ void __launch_bounds__(32 * TS)
-mingru_scan_sliced_kernel(const float* __restrict__ proj, long long ld, int z_col, int x_col, int g_col, const TB* __restrict__ z_bias,
-                          const TB* __restrict__ x_bias, float* __restrict__ state, const int* __restrict__ q_start,
-                          const int* __restrict__ state_slot, TO* __restrict__ out, int width)
+mingru_scan_sliced_kernel(const float* proj, long long ld, int z_col, int x_col, int g_col, const TB* __restrict__ z_bias,
+                          const TB* __restrict__ x_bias, float* state, const int* q_start,
+                          const int* state_slot, TO* __restrict__ out, int width)
 {
     __shared__ float sa[TS][32], sb[TS][32];
     pdl_enter();
@@ -155,23 +155,23 @@ __device__ __forceinline__ float fast_exp2(float v)
 }
 
 // four consecutive entries of a token's B or C row, as one 16-byte load where the row allows it
-__device__ __forceinline__ float4 row_quad(const float* __restrict__ p, int n, int n_state, bool vec)
+__device__ __forceinline__ float4 row_quad(const float* p, int n, int n_state, bool vec)
 {
-    if (vec) return __ldg(reinterpret_cast<const float4*>(p + n));
+    if (vec) return *reinterpret_cast<const float4*>(p + n);
     float4 v;
-    v.x = n < n_state ? __ldg(p + n) : 0.f;
-    v.y = n + 1 < n_state ? __ldg(p + n + 1) : 0.f;
-    v.z = n + 2 < n_state ? __ldg(p + n + 2) : 0.f;
-    v.w = n + 3 < n_state ? __ldg(p + n + 3) : 0.f;
+    v.x = n < n_state ? p[n] : 0.f;
+    v.y = n + 1 < n_state ? p[n + 1] : 0.f;
+    v.z = n + 2 < n_state ? p[n + 2] : 0.f;
+    v.w = n + 3 < n_state ? p[n + 3] : 0.f;
     return v;
 }
       // states a thread keeps in registers; a channel's states are dealt out over `lanes` threads
 
 template <typename TX, typename TW, typename TO>
-__global__ void selective_scan_kernel(const TX* __restrict__ x, const float* __restrict__ dt_pre, const TW* __restrict__ dt_bias,
-                                      const float* __restrict__ proj, long long proj_ld, int b_col, int c_col, const float* __restrict__ z,
-                                      long long z_ld, const TW* __restrict__ a_log, const TW* __restrict__ d_skip, float* __restrict__ state,
-                                      const int* __restrict__ q_start, const int* __restrict__ state_slot, TO* __restrict__ out, int inner, int n_state,
+__global__ void selective_scan_kernel(const TX* x, const float* dt_pre, const TW* __restrict__ dt_bias,
+                                      const float* proj, long long proj_ld, int b_col, int c_col, const float* z,
+                                      long long z_ld, const TW* __restrict__ a_log, const TW* __restrict__ d_skip, float* state,
+                                      const int* q_start, const int* state_slot, TO* __restrict__ out, int inner, int n_state,
                                       int lanes)
 {
     pdl_enter();
@@ -223,8 +223,8 @@ __global__ void selective_scan_kernel(const TX* __restrict__ x, const float* __r
             for (int j = 0; j < SS_PER_THREAD; ++j) {
                 const int n = part + j * lanes;
                 if (n < n_state) {
-                    S[j] = fast_exp2(dt * A[j]) * S[j] + dx * __ldg(B + n);
-                    y = fmaf(S[j], __ldg(C + n), y);
+                    S[j] = fast_exp2(dt * A[j]) * S[j] + dx * B[n];
+                    y = fmaf(S[j], C[n], y);
                 }
             }
         }
@@ -256,10 +256,10 @@ __global__ void selective_scan_kernel(const TX* __restrict__ x, const float* __r
 // slices; the chain over slices is done by TS threads per channel-lane, one for every TS-th state of the lane.
 template <typename TX, typename TW, typename TO, int TS>
 __global__ void __launch_bounds__(32 * TS)
-selective_scan_sliced_kernel(const TX* __restrict__ x, const float* __restrict__ dt_pre, const TW* __restrict__ dt_bias,
-                             const float* __restrict__ proj, long long proj_ld, int b_col, int c_col, const float* __restrict__ z,
-                             long long z_ld, const TW* __restrict__ a_log, const TW* __restrict__ d_skip, float* __restrict__ state,
-                             const int* __restrict__ q_start, const int* __restrict__ state_slot, TO* __restrict__ out, int inner, int n_state,
+selective_scan_sliced_kernel(const TX* x, const float* dt_pre, const TW* __restrict__ dt_bias,
+                             const float* proj, long long proj_ld, int b_col, int c_col, const float* z,
+                             long long z_ld, const TW* __restrict__ a_log, const TW* __restrict__ d_skip, float* state,
+                             const int* q_start, const int* state_slot, TO* __restrict__ out, int inner, int n_state,
                              int lanes)
 {
     __shared__ float s_end[TS][32][SS_PER_THREAD + 1];
@@ -293,7 +293,7 @@ selective_scan_sliced_kernel(const TX* __restrict__ x, const float* __restrict__
         pre_n = live ? dt_pre[(long long)t * inner + cc] : 0.f;
         x_n = live ? to_f32(x[(long long)t * inner + cc]) : 0.f;
         if (gate) z_n = live ? z[(long long)t * z_ld + cc] : 0.f;
-        if (lanes == 1) bc_n = (lx & 15) < n_state ? __ldg(proj + (long long)t * proj_ld + (lx < 16 ? b_col : c_col) + (lx & 15)) : 0.f;
+        if (lanes == 1) bc_n = (lx & 15) < n_state ? *(proj + (long long)t * proj_ld + (lx < 16 ? b_col : c_col) + (lx & 15)) : 0.f;
     };
     fetch(t0, false);
     for (int t = t0; t < t1; ++t) {
@@ -320,7 +320,7 @@ selective_scan_sliced_kernel(const TX* __restrict__ x, const float* __restrict__
 #pragma unroll
             for (int j = 0; j < SS_PER_THREAD; ++j) {
                 const int n = part + j * lanes;
-                if (n < n_state) S[j] = fast_exp2(dt * A[j]) * S[j] + dx * __ldg(B + n);
+                if (n < n_state) S[j] = fast_exp2(dt * A[j]) * S[j] + dx * B[n];
             }
         }
     }
@@ -370,8 +370,8 @@ selective_scan_sliced_kernel(const TX* __restrict__ x, const float* __restrict__
             for (int j = 0; j < SS_PER_THREAD; ++j) {
                 const int n = part + j * lanes;
                 if (n < n_state) {
-                    S[j] = fast_exp2(dt * A[j]) * S[j] + dx * __ldg(B + n);
-                    y = fmaf(S[j], __ldg(C + n), y);
+                    S[j] = fast_exp2(dt * A[j]) * S[j] + dx * B[n];
+                    y = fmaf(S[j], C[n], y);
                 }
             }
             for (int o = lanes >> 1; o > 0; o >>= 1) y += __shfl_xor_sync(0xffffffffu, y, o);

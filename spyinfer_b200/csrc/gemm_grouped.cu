@@ -76,7 +76,7 @@ struct Walk {
 template <typename TC>
 __global__ void __launch_bounds__(NUM_THREADS, 1)
 gemm_grouped_kernel(const __grid_constant__ CUtensorMap map_a, const __grid_constant__ CUtensorMap map_w, TC* __restrict__ out, long long ld,
-                    const int* __restrict__ tile_expert, int experts, int row_tiles, int tiles, int N, int k_blocks, int row_step, int col_step, int* status)
+                    const int* tile_expert, int experts, int row_tiles, int tiles, int N, int k_blocks, int row_step, int col_step, int* status)
 {
     extern __shared__ uint8_t smem_raw[];
     uint8_t* smem = reinterpret_cast<uint8_t*>((reinterpret_cast<uintptr_t>(smem_raw) + 1023) & ~(uintptr_t)1023);

@@ -14,7 +14,7 @@ constexpr int BM = 64, BN = 64, BK = 16, TM = 4, TN = 4;
 
 template <typename TA, typename TW, typename TC>
 __global__ void __launch_bounds__(256)
-gemm_simt_kernel(const TA* __restrict__ A, long long lda, const TW* __restrict__ W, long long ldw, TC* __restrict__ C, long long ldc,
+gemm_simt_kernel(const TA* A, long long lda, const TW* __restrict__ W, long long ldw, TC* __restrict__ C, long long ldc,
                  int M, int N, int K)
 {
     __shared__ float As[BK][BM + 4];
@@ -78,7 +78,7 @@ constexpr int SKINNY_N = 32, SKINNY_NG = 16, SKINNY_THREADS = 256;
 // a product this narrow stay in L1/L2, and the accumulators of four rows cost occupancy).
 template <typename TA, typename TW, typename TC, int ROWS>
 __global__ void __launch_bounds__(SKINNY_THREADS)
-gemm_skinny_kernel(const TA* __restrict__ A, long long lda, const TW* __restrict__ W, long long ldw, TC* __restrict__ C, long long ldc,
+gemm_skinny_kernel(const TA* A, long long lda, const TW* __restrict__ W, long long ldw, TC* __restrict__ C, long long ldc,
                    int M, int N, int K)
 {
     __shared__ float part[ROWS][SKINNY_THREADS / 32][SKINNY_NG];
@@ -144,7 +144,7 @@ __device__ __forceinline__ void load4(const bf16* p, float (&v)[4])
 
 template <typename TA, typename TW, typename TC, int NG>
 __global__ void __launch_bounds__(SKINNY_THREADS)
-gemm_skinny_quads_kernel(const TA* __restrict__ A, long long lda, const TW* __restrict__ W, long long ldw, TC* __restrict__ C, long long ldc, int N, int K)
+gemm_skinny_quads_kernel(const TA* A, long long lda, const TW* __restrict__ W, long long ldw, TC* __restrict__ C, long long ldc, int N, int K)
 {
     __shared__ float part[SKINNY_THREADS / 32][NG];
     pdl_enter();

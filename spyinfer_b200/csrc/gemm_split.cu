@@ -109,7 +109,7 @@ __device__ __noinline__ float plain_sum(const float* a, const bf16* w, int K)
 template <int BN, int HALVES>
 __global__ void __launch_bounds__(Shape<BN, HALVES>::THREADS, Shape<BN, HALVES>::PER_SM)
 gemm_split_kernel(const __grid_constant__ CUtensorMap map_w, const __grid_constant__ CUtensorMap map_a, float* __restrict__ out, long long ldc,
-                  const float* __restrict__ A, long long lda, const bf16* __restrict__ W, long long ldw, int n_rows, int m_rows, int K,
+                  const float* A, long long lda, const bf16* __restrict__ W, long long ldw, int n_rows, int m_rows, int K,
                   int k_blocks_per_slice, int tile_rows, int* status)
 {
     using S = Shape<BN, HALVES>;
@@ -355,7 +355,7 @@ __device__ __forceinline__ void split3(float a, uint32_t& p0, uint32_t& p1, uint
     p2 = __float_as_uint((r - __uint_as_float(ur & 0xffff0000u)) * PIECE_SCALE) >> 16;   // what is left has at most eight bits
 }
 
-__global__ void __launch_bounds__(256) split_rows_kernel(const float* __restrict__ A, long long lda, bf16* __restrict__ pieces, int m_rows, int K, int vec)
+__global__ void __launch_bounds__(256) split_rows_kernel(const float* A, long long lda, bf16* __restrict__ pieces, int m_rows, int K, int vec)
 {
     pdl_enter();
     const long long eights = K / 8, total = eights * m_rows, plane = (long long)m_rows * K;

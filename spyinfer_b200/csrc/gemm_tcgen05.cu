@@ -1217,7 +1217,7 @@ gemm_tcgen05_pair_kernel(const __grid_constant__ CUtensorMap map_x, const __grid
 
 // Sums the splits of a scratch buffer in ascending order and stores the output type.
 template <typename TC>
-__global__ void splitk_reduce_kernel(const float* __restrict__ partial, TC* __restrict__ out, long long elems, int splits)
+__global__ void splitk_reduce_kernel(const float* partial, TC* __restrict__ out, long long elems, int splits)
 {
     pdl_enter();
     for (long long i = (long long)blockIdx.x * blockDim.x + threadIdx.x; i < elems; i += (long long)gridDim.x * blockDim.x) {

@@ -61,8 +61,8 @@ __device__ __forceinline__ void finish_square_sums(int groups, const float* part
 // Every pass over the row goes group by group, V elements a thread and step (a run of V elements lies within one group), and
 // adds the squares of what it has just made, so the row is read from memory once and walked three times at most.
 template <typename TY, typename TW, typename TO, int V>
-__global__ void group_norm_kernel(float* __restrict__ hidden, const TY* __restrict__ y, int splits, long long split_stride,
-                                  const TW* __restrict__ y_weight, float y_scale, const int* __restrict__ rows,
+__global__ void group_norm_kernel(float* hidden, const TY* y, int splits, long long split_stride,
+                                  const TW* __restrict__ y_weight, float y_scale, const int* rows,
                                   const TW* __restrict__ weight, TO* __restrict__ out, int len, int groups, float eps, int write_back)
 {
     extern __shared__ __align__(16) float sm[];

@@ -33,9 +33,9 @@ __device__ __forceinline__ float rotated(const float* x, int j, int rot_half, in
 
 template <typename TF, typename TO, typename TC>
 __global__ void __launch_bounds__(PREP_THREADS)
-latent_prep_kernel(const TF* __restrict__ fused, long long ld, int off_q, int q_rank, const float* __restrict__ wq, TO* __restrict__ cq_out,
+latent_prep_kernel(const TF* fused, long long ld, int off_q, int q_rank, const float* __restrict__ wq, TO* __restrict__ cq_out,
                    int off_c, int kv_rank, const float* __restrict__ wc, int rot_dim, const float* __restrict__ rope, int rot_half, int table_rows,
-                   int interleaved, const int* __restrict__ positions, const int* __restrict__ seq_of_token, const int* __restrict__ block_table,
+                   int interleaved, const int* positions, const int* seq_of_token, const int* block_table,
                    int table_width, TC* __restrict__ pages, int page_size, int num_pages, int planes, float eps, int* status)
 {
     extern __shared__ float sm[];           // rot_dim floats, then 33 of scratch

@@ -46,10 +46,10 @@ template <> struct Quad<bf16> {
 // the same order either way.
 template <typename TX, typename TD, typename TW, typename TO, bool VEC, int REG>
 __global__ void __launch_bounds__(1024)
-layernorm_kernel(TX* x, const TD* __restrict__ a, int a_splits, long long a_stride, float a_scale, const TD* __restrict__ b, int b_splits,
-                 long long b_stride, float b_scale, const int* __restrict__ rows, const TW* __restrict__ w, TO* __restrict__ out, int len, float eps,
+layernorm_kernel(TX* x, const TD* a, int a_splits, long long a_stride, float a_scale, const TD* b, int b_splits,
+                 long long b_stride, float b_scale, const int* rows, const TW* __restrict__ w, TO* __restrict__ out, int len, float eps,
                  int write_back, int center, const TW* __restrict__ bias, const TW* __restrict__ a_w, const float* __restrict__ a_bias,
-                 const TO* __restrict__ a_rows, const float* __restrict__ a_row_w)
+                 const TO* a_rows, const float* a_row_w)
 {
     extern __shared__ __align__(16) float row_buf[];  // len floats, then 33 of scratch
     pdl_enter();
@@ -240,8 +240,8 @@ extern "C" int spy_layernorm_affine(void* x, int x_dtype, const void* a, int a_s
 // out = scale_a * sum_s a[s] + scale_b * sum_s b[s], element by element in 32-bit: the weighted sum of two results (each
 // one array or a stack of partial sums) for a consumer that cannot form it itself.
 template <typename TD>
-__global__ void scaled_sum_kernel(float* __restrict__ out, const TD* __restrict__ a, int a_splits, long long a_stride, float a_scale,
-                                  const TD* __restrict__ b, int b_splits, long long b_stride, float b_scale, long long total)
+__global__ void scaled_sum_kernel(float* __restrict__ out, const TD* a, int a_splits, long long a_stride, float a_scale,
+                                  const TD* b, int b_splits, long long b_stride, float b_scale, long long total)
 {
     pdl_enter();
     long long i = (long long)blockIdx.x * blockDim.x + threadIdx.x;

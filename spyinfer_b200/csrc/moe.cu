@@ -39,7 +39,7 @@ struct MoeRouting {
 };
 
 template <typename TA, typename TO>
-__global__ void moe_activation_kernel(const TA* __restrict__ gu, long long gu_ld, const float* __restrict__ logits, long long logits_ld,
+__global__ void moe_activation_kernel(const TA* gu, long long gu_ld, const float* logits, long long logits_ld,
                                       TO* __restrict__ y, long long y_ld, int experts, int top, int ff, float limit, int shared_ff, float shared_limit,
                                       float alpha, float* __restrict__ weights_out, int vec, MoeRouting r)
 {
@@ -250,7 +250,7 @@ extern "C" int spy_moe_activation_table(const void* gu, int gu_dtype, long long 
 
 // out[t, :] += w[t] * x[t, :] in 32-bit (out float32): what the identity experts of a mixture contribute.
 template <typename TX>
-__global__ void add_scaled_rows_kernel(float* __restrict__ out, const TX* __restrict__ x, const float* __restrict__ w, int width, long long total)
+__global__ void add_scaled_rows_kernel(float* out, const TX* x, const float* w, int width, long long total)
 {
     pdl_enter();
     long long i = (long long)blockIdx.x * blockDim.x + threadIdx.x;
@@ -284,7 +284,7 @@ extern "C" int spy_add_scaled_rows(float* out, const void* x, int x_dtype, const
 
 // One warp a token (a block walks over tokens with a stride): the chosen experts in ascending order with their weights, the shared
 // expert's gate, and the experts' counts (added up per block in shared memory first, so few additions meet in global memory).
-__global__ void moe_route_kernel(const float* __restrict__ logits, long long logits_ld, int tokens, int experts, int top, int has_shared,
+__global__ void moe_route_kernel(const float* logits, long long logits_ld, int tokens, int experts, int top, int has_shared,
                                  int* __restrict__ choice, float* __restrict__ choice_w, float* __restrict__ shared_w, int* __restrict__ counts)
 {
     extern __shared__ float w_all[];               // experts floats a warp, then the block's counts
@@ -341,7 +341,7 @@ __global__ void moe_route_kernel(const float* __restrict__ logits, long long log
 // whose they are (-1 behind the last run).  offsets [experts + 1]; slot [tokens * top]: the
 // row of each (token, k); row_token, row_w [tokens * top]: each row's token and weight.
 __global__ void __launch_bounds__(1024)
-moe_slots_kernel(const int* __restrict__ choice, const float* __restrict__ choice_w, const int* __restrict__ counts, int pairs,
+moe_slots_kernel(const int* choice, const float* choice_w, const int* counts, int pairs,
                  int top, int experts, int* __restrict__ offsets, int* __restrict__ slot, int* __restrict__ row_token,
                  float* __restrict__ row_w, int pad, int* __restrict__ tile_expert, int num_tiles)
 {
@@ -392,7 +392,7 @@ moe_slots_kernel(const int* __restrict__ choice, const float* __restrict__ choic
 }
 
 // out[r] = in[row_token[r]] (a row of nobody, token -1, is left as it is): rows of `len` elements of 2 bytes (bf16) or 4, copied 16 bytes at a time where the rows allow it.
-__global__ void gather_rows_kernel(const uint8_t* __restrict__ in, const int* __restrict__ row_token, uint8_t* __restrict__ out, long long row_bytes)
+__global__ void gather_rows_kernel(const uint8_t* in, const int* row_token, uint8_t* __restrict__ out, long long row_bytes)
 {
     pdl_enter();
     const int token = row_token[blockIdx.x];
@@ -408,7 +408,7 @@ __global__ void gather_rows_kernel(const uint8_t* __restrict__ in, const int* __
 
 // y[r, i] = w[r] * g * sigmoid(alpha g) * (u + 1) over rows of [gate (ff) | up (ff)], g = min(gate, limit), u = clamp(up, -limit, limit)
 template <typename TA, typename TO>
-__global__ void expert_activation_kernel(const TA* __restrict__ gu, long long gu_ld, const float* __restrict__ row_w, TO* __restrict__ y, long long y_ld,
+__global__ void expert_activation_kernel(const TA* gu, long long gu_ld, const float* row_w, TO* __restrict__ y, long long y_ld,
                                          int ff, float limit, float alpha, int vec, int act)
 {
     pdl_enter();
@@ -454,7 +454,7 @@ __global__ void expert_activation_kernel(const TA* __restrict__ gu, long long gu
 
 // out[t] = sum over k (ascending) of rows[slot[t, k]] (+ shared[t]); rows and shared float32 or bf16, out float32
 template <typename TR>
-__global__ void moe_combine_kernel(const TR* __restrict__ rows, const int* __restrict__ slot, int top, const TR* __restrict__ shared, float* __restrict__ out, int len)
+__global__ void moe_combine_kernel(const TR* rows, const int* slot, int top, const TR* shared, float* __restrict__ out, int len)
 {
     pdl_enter();
     const long long t = blockIdx.x;
@@ -522,7 +522,7 @@ extern "C" int spy_moe_route(const float* logits, long long logits_ld, int token
 // The (token, chosen expert) pairs of a step from a matrix of routing weights [tokens, ld] whose entry is the expert's weight where
 // the token chose it and 0 elsewhere (what moe_activation leaves in weights_out): a token's chosen experts in ascending order, at
 // most `top` of them; pairs beyond a token's last have the expert -1, weight 0 and no row.  One warp a token.
-__global__ void moe_pairs_kernel(const float* __restrict__ weights, long long ld, int tokens, int experts, int top, int* __restrict__ choice,
+__global__ void moe_pairs_kernel(const float* weights, long long ld, int tokens, int experts, int top, int* __restrict__ choice,
                                  float* __restrict__ choice_w, int* __restrict__ slot, int* __restrict__ counts)
 {
     extern __shared__ int hist_s[];
@@ -577,7 +577,7 @@ extern "C" int spy_moe_route_weights(const float* weights, long long ld, int tok
 }
 
 // The pairs of a step whose experts a table [vocab, top] names by token id, all with the weight 1 / top, in the table's order.
-__global__ void moe_table_kernel(const int* __restrict__ table, const int* __restrict__ ids, int vocab, long long pairs, int experts, int top,
+__global__ void moe_table_kernel(const int* __restrict__ table, const int* ids, int vocab, long long pairs, int experts, int top,
                                  int* __restrict__ choice, float* __restrict__ choice_w, int* __restrict__ slot, int* __restrict__ counts)
 {
     extern __shared__ int hist_s[];

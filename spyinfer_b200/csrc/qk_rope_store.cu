@@ -51,8 +51,8 @@ constexpr int WARPS_PER_BLOCK = 4;
 template <typename TS, typename TQ, typename TC, typename TW>
 __global__ void qk_rope_store_kernel(const TS* src, int src_splits, long long src_split_stride, TQ* q_out, long long q_out_stride, int tokens,
                                      int nh, int nkv, int hd, const TW* __restrict__ q_w, const TW* __restrict__ k_w, float eps,
-                                     const float2* __restrict__ cos_sin, int rot_half, int table_rows, const int* __restrict__ positions,
-                                     const int* __restrict__ seq_of_token, const int* __restrict__ block_table, int table_width, TC* pages,
+                                     const float2* __restrict__ cos_sin, int rot_half, int table_rows, const int* positions,
+                                     const int* seq_of_token, const int* block_table, int table_width, TC* pages,
                                      int page_size, int num_pages, int store, int pairing, int* status)
 {
     extern __shared__ float head_buf[];  // WARPS_PER_BLOCK * hd
@@ -137,8 +137,8 @@ __global__ void __launch_bounds__(256) qk_rope_store_hd128_kernel(const TS* src,
                                                                   long long q_out_stride, int tokens, int nh, int nkv,
                                                                   const TW* __restrict__ q_w, const TW* __restrict__ k_w, float eps,
                                                                   const float2* __restrict__ cos_sin, int table_rows,
-                                                                  const int* __restrict__ positions, const int* __restrict__ seq_of_token,
-                                                                  const int* __restrict__ block_table, int table_width, bf16* pages,
+                                                                  const int* positions, const int* seq_of_token,
+                                                                  const int* block_table, int table_width, bf16* pages,
                                                                   int page_size, int num_pages, int store, int* status)
 {
     constexpr int HD = 128;
@@ -256,8 +256,8 @@ template <typename TW>
 __global__ void __launch_bounds__(256, 4) qk_rope_store_hd128_x4_kernel(const bf16* src, bf16* q_out, long long q_out_stride, int tokens, int nh, int nkv,
                                                                      const TW* __restrict__ q_w, const TW* __restrict__ k_w, float eps,
                                                                      const float2* __restrict__ cos_sin, int table_rows,
-                                                                     const int* __restrict__ positions, const int* __restrict__ seq_of_token,
-                                                                     const int* __restrict__ block_table, int table_width, bf16* pages,
+                                                                     const int* positions, const int* seq_of_token,
+                                                                     const int* block_table, int table_width, bf16* pages,
                                                                      int page_size, int num_pages, int store, int* status)
 {
     constexpr int HD = 128, PER = 4;

@@ -34,7 +34,7 @@ __device__ __forceinline__ void store4(bf16* p, const float (&v)[4])
 
 // four (or one) neighbouring columns of a projection row, its parts summed, the bias added
 template <typename TP>
-__device__ __forceinline__ void columns4(const TP* __restrict__ row, int splits, long long split_stride, const float* __restrict__ bias, int col, float (&v)[4])
+__device__ __forceinline__ void columns4(const TP* row, int splits, long long split_stride, const float* __restrict__ bias, int col, float (&v)[4])
 {
     load4(row + col, v);
     float p[4];
@@ -51,7 +51,7 @@ __device__ __forceinline__ void columns4(const TP* __restrict__ row, int splits,
     }
 }
 template <typename TP>
-__device__ __forceinline__ float column(const TP* __restrict__ row, int splits, long long split_stride, const float* __restrict__ bias, int col)
+__device__ __forceinline__ float column(const TP* row, int splits, long long split_stride, const float* __restrict__ bias, int col)
 {
     float v = to_f32(row[col]);
     for (int s = 1; s < splits; ++s) v += to_f32(row[s * split_stride + col]);
@@ -75,7 +75,7 @@ struct StoreArgs {
 // (or nothing is rotated) and rot_half is even: a thread takes four neighbouring elements of a row of hd.  Else one element a thread.
 template <typename TP, typename TQ, bool VEC>
 __global__ void __launch_bounds__(128)
-qkv_store_kernel(const TP* __restrict__ proj, TQ* __restrict__ q_out, TQ* __restrict__ pages, StoreArgs A)
+qkv_store_kernel(const TP* proj, TQ* __restrict__ q_out, TQ* __restrict__ pages, StoreArgs A)
 {
     pdl_enter();
     const int t = blockIdx.x;
@@ -166,7 +166,7 @@ extern "C" int spy_qkv_store(const void* proj, int proj_dtype, long long ld, int
 
 template <typename TA, typename TG, bool VEC>
 __global__ void __launch_bounds__(128)
-gate_heads_kernel(const TA* __restrict__ attn, int hd, const TG* __restrict__ gate, long long gate_ld, int splits, long long split_stride, int gate_col,
+gate_heads_kernel(const TA* attn, int hd, const TG* gate, long long gate_ld, int splits, long long split_stride, int gate_col,
                   TA* __restrict__ out, int heads, int vdim)
 {
     pdl_enter();

@@ -1543,7 +1543,7 @@ extern "C" int spy_gla_scan(const float* proj, long long ld, int off_q, int off_
 
 // out[t, j] = act(proj[t, off + j]) for j < n: the inner activation of a two-step (low-rank) projection; act 0: tanh, 1: none.
 template <typename TO>
-__global__ void tanh_cols_kernel(const float* __restrict__ proj, long long ld, int off, int n, TO* __restrict__ out, long long total, int act)
+__global__ void tanh_cols_kernel(const float* proj, long long ld, int off, int n, TO* __restrict__ out, long long total, int act)
 {
     pdl_enter();
     long long i = (long long)blockIdx.x * blockDim.x + threadIdx.x;

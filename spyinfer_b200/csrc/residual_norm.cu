@@ -10,7 +10,7 @@
 SPY_MODULE(spy_residual_norm)
 
 template <typename TY, typename TW, typename TC>
-__global__ void __launch_bounds__(256) residual_norm_kernel(float* __restrict__ h, const TY* __restrict__ y, int splits, long long split_stride,
+__global__ void __launch_bounds__(256) residual_norm_kernel(float* h, const TY* y, int splits, long long split_stride,
                                                             const TW* __restrict__ w, float w_offset, TC* __restrict__ copy, int len, float eps)
 {
     extern __shared__ float row_buf[];   // len floats, then 33 of scratch
@@ -67,7 +67,7 @@ template <> struct Quad<bf16> {
 // tid + j * blockDim.x), the weight's quads are loaded before the wait for the kernels ahead, the stream's and every
 // part's loads are under way together, and the sums over the parts keep their order.
 template <typename TY, typename TW, typename TC, int NQ, int MAXT>
-__global__ void __launch_bounds__(MAXT) residual_norm_row_kernel(float* __restrict__ h, const TY* __restrict__ y, int splits, long long split_stride,
+__global__ void __launch_bounds__(MAXT) residual_norm_row_kernel(float* h, const TY* y, int splits, long long split_stride,
                                                                  const TW* __restrict__ w, float w_offset, TC* __restrict__ copy, int len, float eps)
 {
     __shared__ float scratch[33];
@@ -182,8 +182,8 @@ template <typename T, int V> __device__ __forceinline__ void load_run(const T* p
 
 // V = 4: runs of four where rows, parts and tensors allow them
 template <typename TA, typename TB, int V>
-__global__ void normed_sum_kernel(float* __restrict__ out, const TA* __restrict__ a, int a_splits, long long a_stride, const float* __restrict__ a_weight,
-                                  float a_scale, const TB* __restrict__ b, int b_splits, long long b_stride, const float* __restrict__ b_weight, float b_scale,
+__global__ void normed_sum_kernel(float* __restrict__ out, const TA* a, int a_splits, long long a_stride, const float* __restrict__ a_weight,
+                                  float a_scale, const TB* b, int b_splits, long long b_stride, const float* __restrict__ b_weight, float b_scale,
                                   int len, float eps)
 {
     extern __shared__ __align__(16) float rows_s[];
@@ -270,7 +270,7 @@ __device__ __forceinline__ void sum_store(T* p, const float (&v)[V])
 // next product reads: what a block does whose two sublayers read one norm.  V elements a thread.
 template <typename TA, typename TB, typename TC, int V>
 __global__ void __launch_bounds__(256)
-stream_sum_kernel(float* __restrict__ hidden, const TA* __restrict__ a, int a_splits, long long a_stride, const TB* __restrict__ b, int b_splits,
+stream_sum_kernel(float* hidden, const TA* a, int a_splits, long long a_stride, const TB* b, int b_splits,
                   long long b_stride, TC* __restrict__ copy, long long n)
 {
     pdl_enter();

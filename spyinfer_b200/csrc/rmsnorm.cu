@@ -38,7 +38,7 @@ template <> struct Quad<bf16> {
 
 
 template <typename TX, typename TD, typename TW, typename TO, bool VEC>
-__global__ void __launch_bounds__(1024) rmsnorm_kernel(TX* x, const TD* __restrict__ delta, int delta_splits, long long delta_split_stride, const int* __restrict__ rows,
+__global__ void __launch_bounds__(1024) rmsnorm_kernel(TX* x, const TD* delta, int delta_splits, long long delta_split_stride, const int* rows,
                                const TW* __restrict__ w, TO* __restrict__ out, int len, float eps, int write_back)
 {
     extern __shared__ float row_buf[];  // len floats, then 33 of scratch
@@ -120,8 +120,8 @@ __global__ void __launch_bounds__(1024) rmsnorm_kernel(TX* x, const TD* __restri
 // weights before this kernel has finished.  All partial products of a thread's elements are
 // requested together, six quads at a time.
 template <typename TX, typename TD, typename TW, typename TO, int QUADS>
-__global__ void __maxnreg__(QUADS <= 2 ? 48 : 80) rmsnorm_row_kernel(TX* x, const TD* __restrict__ delta, int delta_splits, long long delta_split_stride,
-                                                   const int* __restrict__ rows, const TW* __restrict__ w, TO* __restrict__ out, int len, float eps,
+__global__ void __maxnreg__(QUADS <= 2 ? 48 : 80) rmsnorm_row_kernel(TX* x, const TD* delta, int delta_splits, long long delta_split_stride,
+                                                   const int* rows, const TW* __restrict__ w, TO* __restrict__ out, int len, float eps,
                                                    int write_back)
 {
     __shared__ float scratch[33];

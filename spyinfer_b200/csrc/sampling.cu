@@ -67,7 +67,7 @@ __device__ __forceinline__ float from_ordered_bits(uint32_t k)
 
 // One block per row: floor[r] = the row's top_k[r]-th largest logit (-inf where top_k[r] <= 0
 // or top_k[r] >= vocab: every logit takes part).
-__global__ void topk_floor_kernel(const float* __restrict__ logits, long long row_stride, int vocab, const int* __restrict__ top_k,
+__global__ void topk_floor_kernel(const float* logits, long long row_stride, int vocab, const int* top_k,
                                   float* __restrict__ floor_out)
 {
     pdl_enter();
@@ -110,8 +110,8 @@ __global__ void topk_floor_kernel(const float* __restrict__ logits, long long ro
     if (threadIdx.x == 0) floor_out[r] = from_ordered_bits(prefix);
 }
 
-__global__ void sample_slices_kernel(const float* __restrict__ logits, long long row_stride, int vocab, int slice, const float* __restrict__ temperature,
-                                     const long long* __restrict__ seed, const long long* __restrict__ draw, const float* __restrict__ floor_in,
+__global__ void sample_slices_kernel(const float* logits, long long row_stride, int vocab, int slice, const float* temperature,
+                                     const long long* seed, const long long* draw, const float* floor_in,
                                      float* __restrict__ slice_v, int* __restrict__ slice_i)
 {
     pdl_enter();
@@ -148,7 +148,7 @@ __global__ void sample_slices_kernel(const float* __restrict__ logits, long long
     }
 }
 
-__global__ void sample_pick_kernel(const float* __restrict__ slice_v, const int* __restrict__ slice_i, int slices, int* __restrict__ tokens)
+__global__ void sample_pick_kernel(const float* slice_v, const int* slice_i, int slices, int* __restrict__ tokens)
 {
     pdl_enter();
     const int r = blockIdx.x;

@@ -43,10 +43,10 @@ __device__ __forceinline__ void store4(bf16* p, const float (&v)[4])
 // 4-element accesses: a thread takes two neighbouring pairs at a time.
 template <typename TP, typename TW, typename TQ, bool VEC>
 __global__ void __launch_bounds__(256)
-sink_qkv_store_kernel(const TP* __restrict__ proj, long long ld, int q_col, int k_col, int v_col, const TW* __restrict__ q_weight,
+sink_qkv_store_kernel(const TP* proj, long long ld, int q_col, int k_col, int v_col, const TW* __restrict__ q_weight,
                       const TW* __restrict__ k_weight, const TW* __restrict__ temp, float eps, const float* __restrict__ rope, int rot_half,
-                      int table_rows, const int* __restrict__ positions, const int* __restrict__ seq_of_token, TQ* __restrict__ q_out,
-                      const int* __restrict__ block_table, int table_width, TQ* __restrict__ pages, int page_size, int num_pages, int heads,
+                      int table_rows, const int* positions, const int* seq_of_token, TQ* __restrict__ q_out,
+                      const int* block_table, int table_width, TQ* __restrict__ pages, int page_size, int num_pages, int heads,
                       int kv_heads, int dim, int vdim, int hd, int* status)
 {
     __shared__ float scratch[33];
@@ -260,9 +260,9 @@ extern "C" int spy_sink_qkv_store(const void* proj, int proj_dtype, long long ld
 //   M = max(lse, 0, max_K score), D = exp(lse - M) + [sink] exp(-M) + sum_K exp(score - M),
 //   out = out * exp(lse - M) / D + sum_K exp(score - M) / D * v.
 template <typename TQ>
-__global__ void sink_merge_kernel(const TQ* __restrict__ q, long long q_ld, TQ* __restrict__ out, const float* __restrict__ lse,
-                                  const TQ* __restrict__ pages, const int* __restrict__ block_table, int table_width, int page_size, int num_pages,
-                                  int nh, int nkv, int hd, const int* __restrict__ positions, const int* __restrict__ seq_of_token, int tokens,
+__global__ void sink_merge_kernel(const TQ* q, long long q_ld, TQ* __restrict__ out, const float* lse,
+                                  const TQ* pages, const int* block_table, int table_width, int page_size, int num_pages,
+                                  int nh, int nkv, int hd, const int* positions, const int* seq_of_token, int tokens,
                                   int window, int keep_first, int sink, float scale, int* status)
 {
     pdl_enter();
@@ -341,9 +341,9 @@ __device__ __forceinline__ void store_lane(bf16* p, const float (&v)[V])
 }
 
 template <int V>
-__global__ void sink_merge_rows_kernel(const bf16* __restrict__ q, long long q_ld, bf16* __restrict__ out, const float* __restrict__ lse,
-                                       const bf16* __restrict__ pages, const int* __restrict__ block_table, int table_width, int page_size, int num_pages,
-                                       int nh, int nkv, const int* __restrict__ positions, const int* __restrict__ seq_of_token, int tokens,
+__global__ void sink_merge_rows_kernel(const bf16* q, long long q_ld, bf16* __restrict__ out, const float* lse,
+                                       const bf16* pages, const int* block_table, int table_width, int page_size, int num_pages,
+                                       int nh, int nkv, const int* positions, const int* seq_of_token, int tokens,
                                        int window, int keep_first, int sink, float scale, int* status, int group)
 {
     constexpr int HD = 32 * V, KB = 4;

@@ -24,7 +24,7 @@ __device__ __forceinline__ void store_quad(bf16* p, const float (&v)[4])
 }
 
 template <typename T>
-__global__ void swiglu_kernel(const T* __restrict__ gate_up, T* __restrict__ out, int inter, long long total)
+__global__ void swiglu_kernel(const T* gate_up, T* __restrict__ out, int inter, long long total)
 {
     pdl_enter();
     long long i = (long long)blockIdx.x * blockDim.x + threadIdx.x;
@@ -44,7 +44,7 @@ __global__ void swiglu_kernel(const T* __restrict__ gate_up, T* __restrict__ out
 // 300 rows of 12,288 in float32: 16.8 us and 6.9 here, between the products around it (44 MB: 6.6 at the copy's rate); a prompt of 300 tokens on the
 // float32 path 7,212 us and 7,096, a decode step of four requests 1,675 and 1,657.  The kernel above stays for the sizes and views that are not whole quads.
 template <typename T>
-__global__ void __launch_bounds__(256) swiglu_quads_kernel(const T* __restrict__ gate_up, T* __restrict__ out, unsigned quads, unsigned total)
+__global__ void __launch_bounds__(256) swiglu_quads_kernel(const T* gate_up, T* __restrict__ out, unsigned quads, unsigned total)
 {
     pdl_enter();
     const unsigned stride = gridDim.x * blockDim.x;
@@ -89,7 +89,7 @@ extern "C" int spy_swiglu(const void* gate_up, void* out, int dtype, int tokens,
 // (the reference's linear adds one when it is bound, spymaster2h/spyinfer
 // src/backends/cpu/cpu_operator.cpp:150-186; its model binds none, src/models/qwen3.hpp:39, 143).
 template <typename T, typename TB>
-__global__ void add_bias_kernel(T* __restrict__ out, const TB* __restrict__ bias, int cols, long long total)
+__global__ void add_bias_kernel(T* out, const TB* __restrict__ bias, int cols, long long total)
 {
     pdl_enter();
     long long i = (long long)blockIdx.x * blockDim.x + threadIdx.x;
@@ -118,7 +118,7 @@ extern "C" int spy_add_bias(void* out, int dtype, const void* bias, int bias_dty
 // out[i] = act(x[i]) element by element in 32-bit: the activation of a feed-forward without a gate.
 //   0: relu(x)^2    1: gelu with the tanh approximation, 0.5 x (1 + tanh(sqrt(2 / pi) (x + 0.044715 x^3)))    2: silu    3: relu
 template <typename T>
-__global__ void activation_kernel(const T* __restrict__ x, T* __restrict__ out, long long total, int act)
+__global__ void activation_kernel(const T* x, T* __restrict__ out, long long total, int act)
 {
     pdl_enter();
     long long i = (long long)blockIdx.x * blockDim.x + threadIdx.x;
@@ -149,7 +149,7 @@ extern "C" int spy_activation(const void* x, void* out, int dtype, long long tot
 }
 
 // x[i] *= scale in place (32-bit): a model whose logits carry a multiplier.
-__global__ void scale_kernel(float* __restrict__ x, long long total, float scale)
+__global__ void scale_kernel(float* x, long long total, float scale)
 {
     pdl_enter();
     long long i = (long long)blockIdx.x * blockDim.x + threadIdx.x;
@@ -171,7 +171,7 @@ extern "C" int spy_scale(float* x, long long total, float scale, cudaStream_t st
 // A gated activation on a fused gate|up tensor: out[t, i] = act(x[t, i]) * x[t, inter + i] in 32-bit.
 //   0: silu    1: gelu with the tanh approximation
 template <typename T>
-__global__ void gated_activation_kernel(const T* __restrict__ gate_up, T* __restrict__ out, int inter, long long total, int act)
+__global__ void gated_activation_kernel(const T* gate_up, T* __restrict__ out, int inter, long long total, int act)
 {
     pdl_enter();
     long long i = (long long)blockIdx.x * blockDim.x + threadIdx.x;
@@ -206,7 +206,7 @@ extern "C" int spy_gated_activation(const void* gate_up, void* out, int dtype, i
 //   g = min(x[t, i] + b[i], limit), u = clamp(x[t, inter + i] + b[inter + i], -limit, limit), out[t, i] = g * sigmoid(alpha * g) * (u + 1).
 // bias: null or [2 * inter] float32.  TI, TO: the input's and the output's type (a 32-bit product may feed a bfloat16 activation).
 template <typename TI, typename TO>
-__global__ void clamped_glu_kernel(const TI* __restrict__ gate_up, const float* __restrict__ bias, TO* __restrict__ out, int inter, long long total,
+__global__ void clamped_glu_kernel(const TI* gate_up, const float* __restrict__ bias, TO* __restrict__ out, int inter, long long total,
                                    float limit, float alpha)
 {
     pdl_enter();
@@ -229,7 +229,7 @@ __global__ void clamped_glu_kernel(const TI* __restrict__ gate_up, const float* 
 
 // The same, four neighbouring outputs a thread (inter, and with it every row pitch, a multiple of 4; arrays aligned for 4-element accesses).
 template <typename TI, typename TO>
-__global__ void clamped_glu_quads_kernel(const TI* __restrict__ gate_up, const float* __restrict__ bias, TO* __restrict__ out, int inter, long long quads,
+__global__ void clamped_glu_quads_kernel(const TI* gate_up, const float* __restrict__ bias, TO* __restrict__ out, int inter, long long quads,
                                          float limit, float alpha)
 {
     pdl_enter();
@@ -300,7 +300,7 @@ extern "C" int spy_clamped_glu(const void* gate_up, int in_dtype, const float* b
 }
 
 // x[i] = cap * tanh(x[i] / cap) in place (32-bit): logits with a soft cap.
-__global__ void softcap_kernel(float* __restrict__ x, long long total, float cap)
+__global__ void softcap_kernel(float* x, long long total, float cap)
 {
     pdl_enter();
     long long i = (long long)blockIdx.x * blockDim.x + threadIdx.x;

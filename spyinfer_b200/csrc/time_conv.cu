@@ -17,8 +17,8 @@ SPY_MODULE(spy_time_conv)
 constexpr int TC_PIECE = 16;       // tokens a thread walks; at least taps - 1, so that only a run's first piece needs the state
 
 template <int MAXT, typename TI, typename TK, typename TO>
-__global__ void time_conv_kernel(const TI* __restrict__ in, long long ld_in, const TK* __restrict__ kernel, const TK* __restrict__ bias,
-                                 float* __restrict__ state, const int* __restrict__ q_start, const int* __restrict__ state_slot, TO* __restrict__ out,
+__global__ void time_conv_kernel(const TI* in, long long ld_in, const TK* __restrict__ kernel, const TK* __restrict__ bias,
+                                 float* state, const int* q_start, const int* state_slot, TO* __restrict__ out,
                                  long long ld_out, int channels, int taps, int pieces, int residual, int act)
 {
     pdl_enter();
