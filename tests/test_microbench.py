@@ -32,3 +32,11 @@ def test_microbench_8_bit_commands_run():
     assert "GB/s" in run("quantize", "--rows", 65, "--size", 1025, "--iters", 3, "--dtype", "float32")
     out = run("step", "--batch", 2, "--context", 100, "--layers", 1, "--int8")
     assert "whole step" in out and "gemm_int8_few_kernel" in out
+
+
+def test_microbench_commands_under_lasting_load():
+    assert "TOP/s" in run("gemm", "--int8", "--m", 8, "--n", 512, "--k", 512, "--iters", 3, "--seconds", 0.3)
+    assert "GB/s" in run("rmsnorm", "--rows", 64, "--size", 1024, "--iters", 3, "--int8", "--seconds", 0.3)
+    assert "GB/s" in run("quantize", "--rows", 65, "--size", 1025, "--iters", 3, "--seconds", 0.3)
+    assert "keys, 1 layers, int8: " in run("step", "--batch", 2, "--context", 100, "--layers", 1, "--int8", "--repeats", 3)
+    assert "prompt of 40 tokens, 1 layers: " in run("step", "--prompt-tokens", 40, "--layers", 1, "--repeats", 3)
