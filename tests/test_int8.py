@@ -988,3 +988,41 @@ def test_engine_on_a_checkpoint_in_wider_types(dtype, tiny_models, tmp_path, mon
     assert float(err.max()) <= 8e-2 * float(want.abs().max()) and float(err.square().mean().sqrt()) <= 4e-2 * float(want.square().mean().sqrt())
     used = {m for layer in engine.model.layers for p in layer.parts() for m in p.modules()}
     assert {"gemm_int8", "quant_int8"} <= used and not {"gemm_tcgen05", "gemm_simt"} & used
+
+
+@gpu
+def test_engine_steps_of_wide_layers_replayed_and_launched():
+    """Layers whose products take long enough for the kernels behind them to start beside them: prompts, mixed steps and replies replayed from graphs against the
+    same steps launched one by one.  Both quantise the same numbers but for what another cut of a sum makes of a rounding to bfloat16, so the bound of
+    ``test_engine_logits`` holds between them; rows that were read too early would be of other tokens altogether."""
+    from spyinfer_b200 import LLMEngine, config_from_json
+    from spyinfer_b200.engine.batch import StepEntry
+    cfg = dict(architectures=["Qwen3ForCausalLM"], model_type="qwen3", hidden_act="silu", num_hidden_layers=3, hidden_size=2048, num_attention_heads=16,
+               num_key_value_heads=8, head_dim=128, intermediate_size=8192, vocab_size=4096, rope_theta=1000000.0, rms_norm_eps=1e-6,
+               tie_word_embeddings=False, max_position_embeddings=4096)
+    engines = [LLMEngine(model_config=config_from_json(cfg), seed=5, dtype="bfloat16", quantization="int8", use_cuda_graphs=graphs, max_num_seqs=64,
+                         max_model_len=1024, kvcache_block_size=16, num_kvcache_blocks=600, max_num_batched_tokens=1024) for graphs in (True, False)]
+    g = torch.Generator().manual_seed(3)
+
+    def tokens(n):
+        return torch.randint(0, 4096, (n,), generator=g).tolist()
+
+    def step(entries):
+        replayed, launched = (torch.as_tensor(e.step_raw(entries)).double() for e in engines)
+        err = (replayed - launched).abs()
+        assert bool(torch.isfinite(replayed).all())
+        assert float(err.max()) <= 8e-2 * float(launched.abs().max()) and float(err.square().mean().sqrt()) <= 4e-2 * float(launched.square().mean().sqrt())
+
+    for turn in range(4):
+        names = [f"{turn}.{i}" for i in range(8)]
+        step([StepEntry(names[0], tokens(300), [299])])
+        step([StepEntry(n, tokens(k), [k - 1]) for n, k in zip(names[1:], (1, 7, 33, 64, 100, 3, 40))])
+        for _ in range(5):
+            step([StepEntry(n, tokens(1), [0]) for n in names])
+        step([StepEntry(names[0], tokens(200), [0, 199]), StepEntry(names[1], tokens(1), [0])])
+        for e in engines:
+            for n in names:
+                e.runner.finish(n)
+    assert engines[0].runner.graph_steps > 20 and engines[1].runner.graph_steps == 0
+    for e in engines:
+        e.runner.check_status()
