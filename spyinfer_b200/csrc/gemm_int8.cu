@@ -14,9 +14,11 @@
 // Tails: rows beyond M or N and the end of K are zero-filled by TMA, stores are predicated.  Any K; the rows of A and of W lie a multiple of 16 bytes
 // apart.  No cluster multicast is used.
 //
-// Measured (replayed from a graph, weights cycled past L2; the floor is the bytes at 6,547 GB/s or the operations at 3,279 TOP/s): 1 x 6,144 x 4,096 6.1 us
-// (floor 3.9), 8 x 24,576 x 4,096 gated 17.6 (15.4), 64 x 4,096 x 12,288 13.2 (7.9): the first bytes' way and a microsecond behind the last ones;
-// 2,048 x 6,144 x 4,096 37.0 (31.4: 2.6 rounds of tiles where 3 are paid), 4,096 x 24,576 x 4,096 gated 242 to 247 (251).
+// Measured (replayed from a graph for some milliseconds at 1,965 MHz, weights cycled past L2; in brackets the bytes at the measured copy rate of 6,547 GB/s, or the
+// operations at 3,279 TOP/s, twice the measured bfloat16 rate: a yardstick, not a bound of the integer pipe): 1 x 6,144 x 4,096 5.9 us (3.9), 8 x 24,576 x 4,096
+// gated 17.3 (15.4), 64 x 4,096 x 12,288 13.1 (7.9): the first bytes' way and a microsecond behind the last ones; 300 x 4,096 x 4,096 10.9 (3.1) and
+// 300 x 4,096 x 12,288 23.7 (9.2): too few tiles to fill the device without low ones, and K walked whole; 2,048 x 6,144 x 4,096 36.7 (31.4: 2.6 rounds of tiles
+// where 3 are paid), 4,096 x 24,576 x 4,096 gated 244 (251).  Under lasting load the clock falls: the last two take 42.5 us at 1,597 MHz and 282 at 1,327.
 //
 // The reference has no integer product (its own are half precision: spymaster2h/spyinfer src/backends/cuda/cublas/sgemm.cu:37-55).
 #include <cuda.h>
@@ -677,7 +679,7 @@ struct Plan {
 
 // The plan is the one of the least expected time, in us, with rates in bytes a us.  Both kernels: what is fixed, plus the slowest of what the main loop
 // waits for, plus the read-out behind it.  The numbers were fitted to the measurements of 18 weight sizes (512 x 8,192 to 51,200 x 5,120) at 1 to 4,096
-// tokens with all tiles and cuts: the chosen plans take 1.4 % longer than the fastest of all measured on average, 20 % at worst (5,003 x 2,055, 512 tokens).
+// tokens with all tiles and cuts: the chosen plans take 1.4 % longer than the fastest of all measured on average, 21 % at worst (5,003 x 2,055, 512 tokens).
 // Which kernel, for instance (us, few / pairs): 6,144 x 4,096 at 128 tokens 10.7 / 11.5, 384 13.8 / 13.7; 34,816 x 5,120 gated at 64 tokens 29.5 / 31.8, 200
 // 46.2 / 37.1.  How K is cut (1 / 2 / 4 / 8 ways, 8 tokens): 6,144 x 4,096 9.0 / 7.5 / 6.7 / 9.9, 4,096 x 12,288 22.7 / 14.1 / 11.3 / 10.7, 24,576 x 4,096
 // 17.9 / 21.9 / 22.6 / -.

@@ -101,10 +101,10 @@ __device__ __forceinline__ void epilogue_barrier() { asm volatile("bar.sync 1, 1
 constexpr int PLAIN_STAGE_LD = 132;   // floats between the tokens of a staged plain tile (128 weight rows and a pad, rows 16 bytes aligned)
 constexpr int SWIGLU_STAGE_LD = 66;   // bf16 elements between the tokens of a staged SwiGLU tile (64 outputs and a pad)
 
-// silu(g) * u for a bfloat16 result: the fast exponential and division (2 ulp of float each) are far
+// silu(g) * u for a bfloat16 result: the fast exponential (about 2 + 1.2 |g| ulp of float) and division (2) are far
 // inside the result's rounding, and the accurate ones cost the epilogue warps more instructions than all
-// the rest of a tile's read-out (64 tokens: 4.0 against 1.5 microseconds).  A gate below -87 gives
-// g / inf = -0, the limit.  The 32-bit path has its own SwiGLU kernel with the accurate functions.
+// the rest of a tile's read-out (64 tokens: 4.0 against 1.5 microseconds).  A gate below about -87.3 gives -0 (the fast
+// division by 2^126 and more), the limit.  The 32-bit path has its own SwiGLU kernel with the accurate functions.
 __device__ __forceinline__ float silu_mul(float g, float u) { return __fdividef(g, 1.0f + __expf(-g)) * u; }
 // the tanh form of gelu on the gate (EPI == 3), with the hardware tanh (error below 2^-10, inside the bfloat16 result's rounding)
 __device__ __forceinline__ float gelu_tanh_mul(float g, float u)

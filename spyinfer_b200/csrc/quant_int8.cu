@@ -116,7 +116,7 @@ __device__ __forceinline__ int nearest_exact(float y, float k, float amax)
 template <bool BF16> __device__ __forceinline__ uint2 encode8(const float (&y)[8], float k, float amax)
 {
     // Numbers that are looked at together: of bfloat16 one warp in four has a half among 4 a lane, two in five among 8 (24,576 x 4,096 by 8 / 4 / 2: 50.8 / 49.4
-    // / 53.7 us).
+    // / 53.7 us, with loads that ran ahead of the wait for the kernel before; 51.5 since they do not).
     constexpr int PART = BF16 ? 4 : 8;
     uint32_t m[8];
 #pragma unroll
@@ -149,7 +149,8 @@ template <bool WHOLE> __device__ __forceinline__ void put_codes(int8_t* row, int
         if (place<true>(g, 0) < len) *reinterpret_cast<uint2*>(row + place<true>(g, 0)) = c;
     } else {
         // Four lanes hold four neighbours of each element: two exchanges give lane q of the four the neighbours of elements q and q + 4, which it stores as words.
-        // The whole warp comes here.  1,531 x 4,999 float32: 12.6 us with the codes stored one by one, 9.3 in words.
+        // The whole warp comes here.  1,531 x 4,999 float32: 12.6 us with the codes stored one by one, 9.3 in words (both with
+        // loads that ran ahead of the wait for the kernel before; 9.8 since they do not).
         const int q = threadIdx.x & 3;
         const bool far = q >= 2, odd = (q & 1) != 0;
         uint32_t keep = __byte_perm(c.x, c.y, far ? 0x7632 : 0x5410);
@@ -416,12 +417,10 @@ static int quantize(const T* x, long long ldx, int8_t* codes, long long ldc, flo
         return 0;
     }
     // Few rows: the row spread as wide as it goes.  Many: more groups a thread, as what a warp does once a row (reduction, barrier, division) is bought
-    // once for more elements.  us with 1 / 2 / 4 / 8 groups, whole rows of bfloat16: 64 x 4,096 1.9 / 1.9 / 2.1 / 2.9, 2,048 x 4,096 8.4 / 7.3 / 7.2 / 7.4,
-    // 2,048 x 12,288 - / 20.5 / 17.4 / 16.2, 24,576 x 4,096 81 / 63.7 / 59.3 / 52.9 (two thirds of the issue slots taken); with halves decided the short way 6.8, 15.3
-    // and 49.4 (0.93 of the copy rate) with the groups taken here; of float32 2,048 x 4,096 8.3 / 7.4 / 6.5 (0.98).  Others, float32, 1 / 2 / 4 groups with codes stored one
-    // by one: 1,531 x 4,999 20.8 / 12.6 / 14.6, 64 x 4,999 2.6 / 3.7 / 5.4; in words 9.3 and 2.3 with the groups taken here (bfloat16 10.7 and 2.7).
-    // All of that with loads that ran ahead of the wait; where they belong, with the groups taken here: bfloat16 2,048 x 4,096 7.0, 2,048 x 12,288 16.6, 24,576 x 4,096 51.1
-    // (0.90 of the copy rate), 1,531 x 4,999 10.4; float32 2,048 x 4,096 7.8 (0.82), 1,531 x 4,999 9.9.
+    // once for more elements.  us with 1 / 2 / 4 / 8 groups, whole rows of bfloat16: 64 x 4,096 2.0 / 2.0 / 2.2 / 2.8, 2,048 x 4,096 7.8 / 6.6 / 7.0 / 8.0,
+    // 2,048 x 12,288 - / 19.6 / 16.7 / 16.6, 24,576 x 4,096 76.3 / 58.9 / 52.9 / 51.5 (0.90 of the copy rate); of float32 64 x 4,096 1.9 / 1.9 / 2.1, 2,048 x 4,096
+    // 8.4 / 7.5 / 7.8 (0.82), 24,576 x 4,096 81.1 / 73.2 / 71.8.  Others, 1 / 2 / 4 groups: float32 1,531 x 4,999 11.4 / 9.8 / 10.5, 64 x 4,999 2.2 / 2.4 / 3.1;
+    // bfloat16 1,531 x 4,999 10.4 / 10.6 / 11.8.
     const bool packed = whole && sizeof(T) == 2;
     const int groups = row_groups(len, n < 1024 ? 1 : (!whole ? 2 : (packed && (long long)n * len >= (1 << 24) ? 8 : 4))), threads = row_threads(len, groups);
     if constexpr (sizeof(T) == 2) {
@@ -444,8 +443,8 @@ static int norm(TX* x, const TD* delta, int splits, long long split_stride, cons
                 int total, int n, int len, float eps, int write_back, int settled, int* status, cudaStream_t stream)
 {
     const bool whole = len % 8 == 0 && aligned16(x) && aligned16(delta) && aligned16(w) && split_stride * (long long)sizeof(TD) % 16 == 0;
-    // us with 1 / 2 / 4 groups a thread.  Whole rows: 64 x 5,120 3.0 / 3.1 / 3.3, 512 x 4,096 5.7 / 5.7 / 8.4, 4,096 x 5,120 36.5 / 38.1 / 42.1 (a norm with a
-    // bfloat16 result 41.8).  Others: 64 x 4,999 3.7 / 4.4 / 26.9, 1,000 x 4,999 23.7 / 17.9 / 71.0.
+    // us with 1 / 2 / 4 groups a thread.  Whole rows: 64 x 5,120 2.9 / 3.7 / 3.6, 512 x 4,096 5.7 / 6.3 / 9.3, 4,096 x 5,120 37.3 / 39.3 / 40.8 (a norm with a
+    // bfloat16 result 41.8).  Others: 64 x 4,999 3.5 / 4.8 / 26.1, 1,000 x 4,999 25.1 / 18.5 / 58.9; their scales' last bits follow the groups' order of summation.
     const int groups = row_groups(len, whole || n < 512 ? 1 : 2);
     auto kernel = whole ? (groups == 4 ? rmsnorm_int8_kernel<TX, TD, TW, true, 4> : groups == 2 ? rmsnorm_int8_kernel<TX, TD, TW, true, 2> : rmsnorm_int8_kernel<TX, TD, TW, true, 1>)
                         : (groups == 4 ? rmsnorm_int8_kernel<TX, TD, TW, false, 4> : groups == 2 ? rmsnorm_int8_kernel<TX, TD, TW, false, 2> : rmsnorm_int8_kernel<TX, TD, TW, false, 1>);
